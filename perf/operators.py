@@ -186,8 +186,7 @@ def prepare(case, seed):
     heads, nope, value = case["heads"], case["nope"], case["value"]
     return dict(op=op, q=normal(sum(queries), heads, nope + ROPE, dtype=t), k=normal(sum(keys), heads, nope, dtype=t),
                 kr=normal(sum(keys), ROPE, dtype=t), v=normal(sum(keys), heads, value, dtype=t),
-                q_starts=_starts(queries, device), k_starts=_starts(keys, device), longest=max(queries),
-                scale=1.5 * (nope + ROPE) ** -0.5)
+                q_starts=_starts(queries, device), k_starts=_starts(keys, device), scale=1.5 * (nope + ROPE) ** -0.5)
 
 
 def run(s):
@@ -228,8 +227,7 @@ def _own_absorbed(s):
 def _own_prompt(s):
     from mlxlr8_b200.latent import latent_prompt_attention
 
-    return latent_prompt_attention(s["q"], s["k"], s["kr"], s["v"], s["q_starts"], s["k_starts"], s["longest"],
-                                   s["scale"])
+    return latent_prompt_attention(s["q"], s["k"], s["kr"], s["v"], s["q_starts"], s["k_starts"], s["scale"])
 
 
 _own = dict(norm8=_own_norm8, linear4=_own_linear4, append=_own_append, absorbed=_own_absorbed, prompt=_own_prompt)
