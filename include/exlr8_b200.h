@@ -36,6 +36,7 @@ extern "C" {
 #define EXLR8_DTYPE_F32 0
 #define EXLR8_DTYPE_F16 1
 #define EXLR8_DTYPE_BF16 2
+#define EXLR8_DTYPE_E4M3 3 /* 8-bit codes with float32 group scales, where a call says so */
 
 enum exlr8_status {
   EXLR8_OK = 0,
@@ -53,7 +54,8 @@ enum exlr8_status {
   EXLR8_ERR_CUDA = 12,      /* a CUDA runtime call failed (see exlr8_last_cuda_error) */
   EXLR8_ERR_ID_RANGE = 13,  /* "Expert IDs must be in 0..256"                       experts.py:158-159 */
   EXLR8_ERR_UNSUPPORTED = 14,
-  EXLR8_ERR_STATIC_LIMIT = 15 /* needs more scratch than EXLR8_NOALLOC_SCRATCH_BYTES */
+  EXLR8_ERR_STATIC_LIMIT = 15, /* needs more scratch than EXLR8_NOALLOC_SCRATCH_BYTES */
+  EXLR8_ERR_SHAPE = 16        /* operand sizes or strides outside what the call takes */
 };
 
 /* Library ABI version (EXLR8_ABI_VERSION). */
@@ -302,7 +304,10 @@ enum exlr8_kernel_kind {
   EXLR8_KERNEL_EP_RETURN = 9,    /* expert-parallel return over peer memory (includes the wait for owners) */
   EXLR8_KERNEL_EP_COMBINE = 10,  /* expert-parallel weighted combine */
   EXLR8_KERNEL_NORM = 11,        /* residual add + RMS norm */
-  EXLR8_KERNEL_KINDS = 12
+  EXLR8_KERNEL_LINEAR4 = 12,     /* 4-bit affine linear layer */
+  EXLR8_KERNEL_APPEND = 13,      /* latent cache append */
+  EXLR8_KERNEL_ATTENTION = 14,   /* latent attention, both forms */
+  EXLR8_KERNEL_KINDS = 15
 };
 
 /* Opt-in per-launch timing (the reference prints per-layer seconds with
@@ -570,6 +575,93 @@ int exlr8_router_logits(const void* x, int x_dtype, int64_t tokens, int hidden, 
  * residual, h_out and out [rows][hidden] in x_dtype; w [hidden] in x_dtype. */
 int exlr8_residual_rms_norm(const void* x, const void* residual, const void* weight, int x_dtype, int64_t rows,
                             int hidden, float eps, void* h_out, void* out, void* stream);
+
+/* Residual add + RMS norm with an 8-bit output for products that take E4M3
+ * activations (exlr8_affine4_linear): per row, h as exlr8_residual_rms_norm,
+ *   y = h * (1 / sqrt(sum(h * h) / hidden + eps)) * w   (float32, not rounded)
+ * and per group of `group` channels (32, 64, 128 or hidden; a divisor of
+ * hidden)
+ *   scale = max|y| / 448,  code = e4m3(y / scale).
+ * A group of zeros has scale 0 and codes 0; a group with a value that is not
+ * finite has scale NaN and codes 0.  codes uint8 [rows][hidden], scales
+ * float32 [rows][hidden / group].  No counterpart in the reference, whose
+ * norm (exlr8/fast_norm.py) has 16-bit outputs. */
+int exlr8_residual_rms_norm_q8(const void* x, const void* residual, const void* weight, int x_dtype, int64_t rows,
+                               int hidden, int group, float eps, void* h_out, uint8_t* codes, float* scales,
+                               void* stream);
+
+/* ---- attention half of a decoder block ------------------------------------ */
+
+/* Linear layer with 4-bit affine weights (the affine4 dense format of
+ * exlr8/dense.py:19-67; MLX quantize(bits=4)): codes uint32 [out][in / 8], low
+ * nibble first, scales and biases [out][in / group] in scale_dtype (any
+ * EXLR8_DTYPE of 16 or 32 bits), w = scale * q + bias; biases may be null
+ * (w = scale * (q - 8)).  group 32, 64 or 128; in_features a multiple of the
+ * group.  x [rows][in] in x_dtype; for EXLR8_DTYPE_E4M3 x_scales float32
+ * [rows][in / x_group] scales its codes (x_group 32, 64, 128 or in_features,
+ * a divisor of in_features).  out [rows][out] in out_dtype.  x and codes
+ * 16-byte aligned.  Sums are float32.  Made for decode: up to 16 rows share
+ * one pass over the weights, more rows make more passes. */
+int exlr8_affine4_linear(const void* x, int x_dtype, const float* x_scales, int x_group, int64_t rows,
+                         int in_features, int out_features, const uint32_t* codes, const void* scales,
+                         const void* biases, int scale_dtype, int group, void* out, int out_dtype, void* stream);
+
+/* Latent attention (model.py:186-343: one latent vector and one rotary key a
+ * token, shared by all heads).  The paged cache is [pages][page_size]
+ * [rank + 64] in float16 or bfloat16: the latent, then the rotary key.  rank is
+ * 128, 256, 384 or 512; page_size a multiple of 16.
+ *
+ * exlr8_latent_append writes tokens into it: row slots[t] (int64, over all
+ * pages; outside [0, pages * page_size): no entry, e.g. -1 for padding) gets
+ * T(latent * (1 / sqrt(mean(latent^2) + eps)) * weight) (the latent itself
+ * without a weight) and the rotated key.  cos_sin float32 [cos_rows][32][2]
+ * holds cosine and sine of a position's 32 pairs (null: no rotation),
+ * positions int32 [tokens]; pairs are channels (2i, 2i + 1) when interleaved,
+ * else (i, i + 32).  A position outside the table writes no entry.  q_rope
+ * (nullable) [tokens][heads][64] is rotated the same way into q_out (NaN for a
+ * position outside the table).  Strides count elements; 64 channels (rank for
+ * latent) are contiguous.  Two tokens of one call with one slot leave either
+ * entry. */
+int exlr8_latent_append(const void* latent, int64_t latent_stride, const void* rope_key, int64_t rope_stride,
+                        int64_t tokens, int rank, int dtype, const void* weight, float eps, const float* cos_sin,
+                        int64_t cos_rows, const int32_t* positions, int interleaved, const int64_t* slots, void* cache,
+                        int64_t pages, int page_size, const void* q_rope, int64_t q_token_stride, int64_t q_head_stride,
+                        int heads, void* q_out, void* stream);
+
+/* Attention over the cache (absorbed form): q_latent [batch][queries][heads]
+ * [rank], q_rope [batch][queries][heads][64] and out [batch][queries][heads]
+ * [rank] contiguous in the cache's type; out = softmax(scale * q . row) of the
+ * latents.  Sequence b has lengths[b] (int32) cached tokens in the pages
+ * block_table[b][0 .. table_width) (int32); query t sees the first
+ * lengths[b] - queries + 1 + t of them, and gives zeros (lse -inf) when that
+ * is none.  Rows past a length are never used, whatever they hold; table
+ * entries outside [0, pages) hold no tokens; a length past the table's room
+ * counts as that room.  lse (nullable) float32 [batch][queries][heads] is the
+ * natural logarithm of the softmax's sum.  Every pointer 16-byte aligned.
+ * Workspace: exlr8_latent_attention_workspace. */
+size_t exlr8_latent_attention_workspace(int64_t batch, int queries, int heads, int rank);
+int exlr8_latent_attention(const void* q_latent, const void* q_rope, int64_t batch, int queries, int heads, int rank,
+                           int dtype, const void* cache, int64_t pages, int page_size, const int32_t* block_table,
+                           int table_width, const int32_t* lengths, float scale, void* out, float* lse,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal attention of ragged prompts over expanded keys and values: q
+ * [total_q][heads][nope + 64], k [total_k][heads][nope], k_rope [total_k][64]
+ * (shared by all heads), v [total_k][heads][value], with element strides per
+ * token and head (multiples of 8) and contiguous channels, 16-byte aligned;
+ * nope 64, 128 or 192, value 64, 128, 192 or 256, float16 or bfloat16.
+ * Sequence s has the queries q_starts[s] .. q_starts[s + 1] and the keys
+ * k_starts[s] .. k_starts[s + 1] (int32 [seqs + 1], ascending); with n queries
+ * and m keys, query i sees the first m - n + 1 + i keys, and gives zeros (lse
+ * -inf) when that is none.  out [total_q][heads][value] and lse (nullable,
+ * float32 [total_q][heads]) are written for the rows of the sequences only.
+ * 1 <= seqs <= 4096. */
+int exlr8_latent_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                  int64_t k_token_stride, int64_t k_head_stride, const void* k_rope,
+                                  int64_t k_rope_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                                  int64_t total_q, int64_t total_k, int heads, int nope, int value, int dtype,
+                                  const int32_t* q_starts, const int32_t* k_starts, int seqs, float scale, void* out,
+                                  float* lse, void* stream);
 
 /* Dispatch header of the last joined call that used `workspace` (sizes as
  * given to that call): [0] chunks, [1] padded rows, [2..3] GEMM unit counters,

@@ -8,6 +8,7 @@ raises if the library is missing or no CUDA device is present.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from ctypes import c_double, POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 from functools import lru_cache
 from pathlib import Path
@@ -17,10 +18,11 @@ import torch
 LIBRARY = Path(__file__).resolve().with_name("libexlr8_b200.so")
 
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+E4M3_CODE = 3  # 8-bit activations, where a call takes them
 SCALE_CODES = {torch.float32: 0, torch.float16: 1}
 
 # Status codes whose reference behaviour is a ValueError.
-VALUE_ERRORS = {1, 2, 3, 4, 5, 6, 7, 8, 13, 15}
+VALUE_ERRORS = {1, 2, 3, 4, 5, 6, 7, 8, 13, 15, 16}
 
 
 class TrellisExperts(ctypes.Structure):
@@ -149,6 +151,21 @@ _SIGNATURES = {
     "exlr8_shared_expert_workspace": (c_size_t, [c_int64, c_int, c_int]),
     "exlr8_shared_expert": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, POINTER(DenseExpert), c_void_p, c_void_p,
                                     c_size_t, c_void_p]),
+    "exlr8_residual_rms_norm_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_float,
+                                           c_void_p, c_void_p, c_void_p, c_void_p]),
+    "exlr8_affine4_linear": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p,
+                                     c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]),
+    "exlr8_latent_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_float,
+                                    c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                    c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "exlr8_latent_attention_workspace": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "exlr8_latent_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_int64,
+                                       c_int, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
+                                       c_size_t, c_void_p]),
+    "exlr8_latent_prompt_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                              c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int,
+                                              c_int, c_int, c_void_p, c_void_p, c_int, c_float, c_void_p, c_void_p,
+                                              c_void_p]),
     "exlr8_router_logits_workspace": (c_size_t, [c_int64, c_int, c_int]),
     "exlr8_router_logits": (c_int, [c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_size_t,
                                     c_void_p]),
@@ -211,12 +228,24 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def on_device(device: torch.device):
+    """Context in which ``device`` is current: a launch on another device's
+    stream than the current one's would fail."""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def host_device_pointer(t: torch.Tensor) -> int:
     """Device-accessible address of a page-locked host tensor's data, for a
     kernel that reads or writes it over PCIe (pageable memory is refused)."""
     ptr = c_void_p(0)
     check(load().exlr8_host_device_pointer(t.data_ptr(), ctypes.byref(ptr)))
     return int(ptr.value)
+
+
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and on a 16-byte boundary (a copy when it is neither)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def act_code(t: torch.Tensor) -> int:
@@ -234,7 +263,7 @@ def scale_code(t: torch.Tensor) -> int:
 
 
 KERNEL_KINDS = ("router", "plan", "prep", "gate_up", "gate_finish", "down", "finish", "dense", "ep_send",
-                "ep_return", "ep_combine", "norm")
+                "ep_return", "ep_combine", "norm", "linear4", "append", "attention")
 
 
 def profile_enable(enable: bool, capacity: int = 65536) -> None:

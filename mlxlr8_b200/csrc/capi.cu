@@ -475,6 +475,7 @@ const char* exlr8_status_string(int status) {
     case EXLR8_ERR_UNSUPPORTED: return "unsupported configuration";
     case EXLR8_ERR_STATIC_LIMIT:
       return "request needs more scratch than the fixed no-allocation buffer (EXLR8_NOALLOC_SCRATCH_BYTES)";
+    case EXLR8_ERR_SHAPE: return "operand sizes or strides are outside what the operator takes";
     default: return "unknown status";
   }
 }

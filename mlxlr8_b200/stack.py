@@ -1,13 +1,16 @@
-"""A stack of MoE decoder blocks with the attention stubbed (exlr8 model.py:373-418).
+"""A stack of MoE decoder blocks (exlr8 model.py:373-418).
 
 Each block of the reference decoder layer is
 
-    r, _ = self_attn(rms_norm(x, input_norm))       (stubbed: r = 0)
+    r, _ = self_attn(rms_norm(x, input_norm))       a block's attention (without one: r = 0)
     h = x + r
     x = rms_norm(h, post_norm, eps)                  exlr8_residual_rms_norm
     return h + moe(x)                                the MoE layer, residual h
 
-so with the attention stubbed the stack threads the hidden state through
+A block's attention is any callable ``attention(h, step) -> r`` that norms its
+own input, such as ``latent.LatentSelfAttention``, and ``step`` is what the
+stack's call hands to every block's attention (``latent.LatentStep``).  With
+the attention stubbed the stack threads the hidden state through
 ``rms_norm`` and one MoE layer per block: ``MoELayer`` (one GPU, resident
 trellis experts), ``JoinedMoELayer`` (MXFP4) or ``ExpertParallelMoE``
 (experts sharded over the node's GPUs).  The reference model runs layers
@@ -43,23 +46,61 @@ def residual_rms_norm(x, weight, eps: float = 1e-5, residual=None, return_sum: b
     return (h, out) if return_sum else out
 
 
+def residual_rms_norm_q8(x, weight, eps: float = 1e-5, residual=None, group: int = 128, return_sum: bool = False):
+    """``rms_norm(x + residual, weight, eps)`` as E4M3 codes with a float32
+    scale per ``group`` channels (32, 64, 128 or all of a row's): the input of
+    a product that takes 8-bit activations (``affine4.affine4_linear``).
+
+    Returns ``(codes float8_e4m3fn [..., hidden], scales float32 [..., hidden
+    // group])``, with ``return_sum`` the rounded sum ``h`` in front of them.
+    The norm of ``h`` stays in float32 until ``code = e4m3(y / scale)``, ``scale
+    = max|y| / 448``.  A group of zeros has scale 0; a group with a value that
+    is not finite has scale NaN and codes 0."""
+    device = _lib.require_cuda(x, weight, residual)
+    hidden = x.shape[-1]
+    if weight.shape != (hidden,):
+        raise ValueError("norm weight must have one entry per hidden channel")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError("the residual must have the shape of x")
+    if group != hidden and (group not in (32, 64, 128) or hidden % group):
+        raise ValueError("group must be 32, 64, 128 or the row's width, and divide it")
+    code = _lib.act_code(x)
+    x = x.contiguous()
+    rows = x.numel() // hidden
+    w = weight.to(x.dtype).contiguous()
+    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty(x.shape[:-1] + (hidden // group,), dtype=torch.float32, device=device)
+    h = torch.empty_like(x) if return_sum else None
+    res = residual.to(x.dtype).contiguous() if residual is not None else None
+    with _lib.on_device(device):
+        _lib.check(_lib.lib().exlr8_residual_rms_norm_q8(x.data_ptr(), _lib.ptr(res), w.data_ptr(), code, rows, hidden,
+                                                         group, float(eps), _lib.ptr(h), codes.data_ptr(),
+                                                         scales.data_ptr(), _lib.stream_handle(device)))
+    return (h, codes, scales) if return_sum else (codes, scales)
+
+
 class MoEStack:
-    """Blocks of (post-attention norm weight [hidden], MoE layer) applied in
-    order to the hidden state [tokens, hidden]."""
+    """Blocks of (post-attention norm weight [hidden], MoE layer) or (weight,
+    MoE layer, attention) applied in order to the hidden state [tokens,
+    hidden]."""
 
     def __init__(self, blocks, eps: float = 1e-5):
-        self.blocks = [(w, layer) for w, layer in blocks]
+        self.blocks = [tuple(block) if len(block) == 3 else (*block, None) for block in blocks]
         self.eps = eps
 
     def __len__(self):
         return len(self.blocks)
 
-    def __call__(self, h, trace: bool = False):
+    def __call__(self, h, trace: bool = False, step=None):
         """The hidden state after every block; with ``trace`` also the list of
-        (block input, normalised input, block output) per block."""
+        (MoE residual, normalised input, block output) per block.  ``step`` is
+        passed to the blocks' attentions."""
         steps = []
-        for w, layer in self.blocks:
-            xn = residual_rms_norm(h, w, self.eps)
+        for w, layer, attention in self.blocks:
+            if attention is None:
+                xn = residual_rms_norm(h, w, self.eps)
+            else:
+                h, xn = residual_rms_norm(attention(h, step), w, self.eps, residual=h, return_sum=True)
             out = layer(xn, h)
             if trace:
                 steps.append((h, xn, out))

@@ -1,0 +1,130 @@
+"""Host-side checks of the attention half's C entry points (nothing is
+launched: every call is refused or empty) and the page bookkeeping."""
+
+import ctypes
+
+import pytest
+
+from mlxlr8_b200 import _lib
+
+P = 1 << 20  # a 16-byte aligned address that no refused call touches
+
+
+def _norm(x=P, w=P, dtype=2, rows=1, hidden=256, group=128, eps=1e-5, codes=P, scales=P):
+    return _lib.load().exlr8_residual_rms_norm_q8(x, None, w, dtype, rows, hidden, group, eps, None, codes, scales, None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(rows=0), 0), (dict(rows=0, x=None), 0), (dict(dtype=3), 8), (dict(dtype=7), 8), (dict(rows=-1), 16),
+    (dict(hidden=0), 16), (dict(group=48), 16), (dict(group=0), 16), (dict(hidden=200), 16), (dict(rows=1 << 40), 16),
+    (dict(x=None), 11), (dict(w=None), 11), (dict(codes=None), 11), (dict(scales=None), 11),
+    (dict(eps=float("nan")), 11), (dict(eps=-1.0), 11),
+])
+def test_norm_refusals(change, status):
+    assert _norm(**change) == status
+
+
+def _linear(x=P, x_dtype=2, xs=None, xg=0, rows=1, inner=256, outer=8, codes=P, scales=P, sdt=1, group=64, out=P, odt=2):
+    return _lib.load().exlr8_affine4_linear(x, x_dtype, xs, xg, rows, inner, outer, codes, scales, None, sdt, group, out,
+                                            odt, None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(rows=0), 0), (dict(x_dtype=4), 8), (dict(sdt=3), 8), (dict(odt=3), 8), (dict(inner=0), 16),
+    (dict(inner=224), 16), (dict(group=16), 16), (dict(group=256), 16), (dict(outer=0), 16), (dict(rows=-3), 16),
+    (dict(rows=(1 << 20) + 1), 16), (dict(x_dtype=3, xs=P, xg=96), 16), (dict(x_dtype=3, xs=P, xg=0), 16),
+    (dict(x_dtype=3, xg=128), 11), (dict(xs=P), 11), (dict(x=None), 11), (dict(codes=None), 11), (dict(out=None), 11),
+    (dict(x=P + 8), 9), (dict(codes=P + 4), 9),
+])
+def test_linear_refusals(change, status):
+    assert _linear(**change) == status
+
+
+def _append(latent=P, tokens=1, rank=512, dtype=2, cos=None, cos_rows=0, positions=None, slots=P, cache=P, pages=4,
+            page=16, q=None, heads=0, q_out=None, eps=1e-5):
+    return _lib.load().exlr8_latent_append(latent, rank, P, 64, tokens, rank, dtype, None, eps, cos, cos_rows, positions,
+                                           1, slots, cache, pages, page, q, 64, 64, heads, q_out, None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(tokens=0), 0), (dict(dtype=0), 8), (dict(rank=192), 16), (dict(rank=640), 16), (dict(rank=0), 16),
+    (dict(page=8), 16), (dict(page=0), 16), (dict(page=24), 16), (dict(pages=-1), 16), (dict(pages=1 << 60), 16),
+    (dict(tokens=-1), 16), (dict(latent=None), 11), (dict(slots=None), 11), (dict(cache=None), 11), (dict(cos=P), 11),
+    (dict(q=P, heads=0), 16), (dict(q=P, heads=2), 11), (dict(eps=float("nan")), 11), (dict(cos_rows=-1), 16),
+])
+def test_append_refusals(change, status):
+    assert _append(**change) == status
+
+
+def _attend(ql=P, batch=1, queries=1, heads=8, rank=512, dtype=2, cache=P, pages=4, page=16, table=P, width=4, lengths=P,
+            scale=0.1, out=P, ws=P, ws_bytes=1 << 40):
+    return _lib.load().exlr8_latent_attention(ql, P, batch, queries, heads, rank, dtype, cache, pages, page, table, width,
+                                              lengths, scale, out, None, ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(batch=0), 0), (dict(dtype=0), 8), (dict(dtype=3), 8), (dict(rank=100), 16), (dict(queries=0), 16),
+    (dict(heads=0), 16), (dict(page=20), 16), (dict(batch=-1), 16), (dict(batch=1 << 30), 16), (dict(width=-1), 16),
+    (dict(pages=1 << 40), 16), (dict(width=1 << 30), 16), (dict(queries=1 << 30, heads=1 << 16), 16),
+    (dict(ql=None), 11), (dict(table=None), 11), (dict(lengths=None), 11), (dict(cache=None), 11), (dict(out=None), 11),
+    (dict(scale=float("inf")), 11), (dict(scale=float("nan")), 11), (dict(ql=P + 2), 9), (dict(cache=P + 8), 9),
+])
+def test_attention_refusals(change, status):
+    assert _attend(**change) == status
+
+
+def test_attention_workspace_refuses_unusable_sizes():
+    query = _lib.load().exlr8_latent_attention_workspace
+    bad = ctypes.c_size_t(-1).value
+    for args in ((-1, 1, 8, 512), (1, 0, 8, 512), (1, 1, 0, 512), (1, 1, 8, 500), (1 << 20, 1 << 20, 1 << 15, 512)):
+        assert query(*args) == bad
+    assert query(0, 1, 8, 512) != bad and query(4, 2, 64, 512) != bad
+
+
+def _prompt(q=P, qs=(192 * 4, 192), k=P, ks=(128 * 4, 128), rs=64, vs=(128 * 4, 128), total_q=5, total_k=7, heads=4,
+            nope=128, value=128, dtype=1, starts=P, seqs=1, scale=0.1, out=P):
+    return _lib.load().exlr8_latent_prompt_attention(q, *qs, k, *ks, P, rs, P, *vs, total_q, total_k, heads, nope, value,
+                                                     dtype, starts, P, seqs, scale, out, None, None)
+
+
+@pytest.mark.parametrize("change, status", [
+    (dict(total_q=0), 0), (dict(dtype=0), 8), (dict(nope=96), 16), (dict(nope=256), 16), (dict(value=320), 16),
+    (dict(value=0), 16), (dict(heads=0), 16), (dict(heads=70000), 16), (dict(seqs=0), 16), (dict(seqs=5000), 16),
+    (dict(total_q=-1), 16), (dict(total_k=1 << 33), 16), (dict(qs=(770, 192)), 16), (dict(ks=(512, 4)), 16),
+    (dict(rs=65), 16), (dict(vs=(-8, 128)), 16), (dict(q=None), 11), (dict(k=None), 11), (dict(starts=None), 11),
+    (dict(out=None), 11), (dict(scale=float("nan")), 11), (dict(q=P + 2), 9), (dict(out=P + 4), 9),
+])
+def test_prompt_refusals(change, status):
+    assert _prompt(**change) == status
+
+
+def test_shape_status_is_a_value_error():
+    with pytest.raises(ValueError, match="sizes or strides"):
+        _lib.check(16)
+
+
+def test_pages_are_handed_out_and_given_back():
+    from mlxlr8_b200.latent import LatentPages
+
+    pages = LatentPages(6, 16, device="cpu")
+    step = pages.step(["a", "b"], 10)
+    assert step.lengths.tolist() == [10, 10] and step.queries == 10
+    assert step.positions.tolist() == 2 * list(range(10))
+    a, b = step.block_table[:, 0].tolist()
+    assert a != b and step.slots.tolist() == [16 * a + i for i in range(10)] + [16 * b + i for i in range(10)]
+    step = pages.step(["b"], 7)
+    assert step.lengths.tolist() == [17] and step.block_table.shape == (1, 2)
+    assert step.slots.tolist()[:6] == [16 * b + i for i in range(10, 16)] and step.slots[6] % 16 == 0
+    step = pages.step(["a", "b"])
+    assert step.block_table.tolist()[0][1] == -1 and step.lengths.tolist() == [11, 18]
+    with pytest.raises(ValueError, match="no free pages"):
+        pages.step(["c", "b"], 40)
+    assert pages.length("c") == 0 and pages.length("b") == 18
+    pages.release("b")
+    assert pages.length("b") == 0
+    step = pages.step(["c"], 80)
+    assert sorted(step.block_table[0].tolist()) == sorted(set(range(6)) - {a})
+    for bad in (lambda: pages.step([]), lambda: pages.step(["a", "a"]), lambda: pages.step(["a"], 0),
+                lambda: LatentPages(4, 24)):
+        with pytest.raises(ValueError):
+            bad()

@@ -1,0 +1,195 @@
+"""The 4-bit affine linear layer against its formula in 64 bits.
+
+Tolerance of an output: half a step of its type, and the float32 error of the
+sums.  The kernel adds products of q - 8 (and of the folded bias) with x; a
+chain of n additions is off by at most n 2^-23 of the sum of their magnitudes
+(2^-23, a whole step: matrix instructions cut off where a float addition
+rounds), and no chain is longer than in / 8 + 64."""
+
+import pytest
+
+from helpers import torch_dtype
+
+pytestmark = pytest.mark.gpu
+
+
+def _weights(g, outer, inner, group, dtype, biases):
+    import torch
+
+    codes = torch.randint(-(1 << 31), 1 << 31, (outer, inner // 8), generator=g, device="cuda", dtype=torch.int32)
+    scales = (torch.randn(outer, inner // group, generator=g, device="cuda") * 0.02).to(dtype)
+    b = (torch.randn(outer, inner // group, generator=g, device="cuda") * 0.1).to(dtype) if biases else None
+    return codes, scales, b
+
+
+def _values(codes):
+    import torch
+
+    words = codes.view(torch.int32).long() & 0xFFFFFFFF
+    return torch.stack([(words >> (4 * j)) & 15 for j in range(8)], -1).flatten(1).double()
+
+
+def _check(x, codes, scales, biases, x_scales=None, out_dtype=None, out=None):
+    import torch
+
+    from mlxlr8_b200.affine4 import affine4_linear
+
+    got = affine4_linear(x, codes, scales, biases, x_scales=x_scales, out_dtype=out_dtype, out=out)
+    inner = codes.shape[1] * 8
+    group = inner // scales.shape[1]
+    xv = x.float().double().reshape(-1, inner)
+    if x_scales is not None:
+        xs = x_scales.double().reshape(xv.shape[0], -1)
+        xv = xv * xs.repeat_interleave(inner // xs.shape[1], 1)
+    s = scales.double().repeat_interleave(group, 1)
+    b = -8.0 * s if biases is None else biases.double().repeat_interleave(group, 1)
+    q = _values(codes)
+    expected = xv @ (q * s + b).t()
+    magnitude = xv.abs() @ (((q - 8.0) * s).abs() + (b + 8.0 * s).abs()).t()
+    tol = expected.abs() * torch.finfo(got.dtype).eps / 2 * 1.001 + (inner / 8 + 64) * 2.0 ** -23 * magnitude + 1e-30
+    if got.dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    assert got.shape == x.shape[:-1] + (codes.shape[0],)
+    assert bool(((got.double().reshape(expected.shape) - expected).abs() <= tol).all())
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("rows, inner, outer, group, biases", [
+    (1, 6144, 576, 64, True), (1, 512, 1000, 128, False), (2, 32, 1, 32, True), (3, 96, 33, 32, True),
+    (8, 2080, 130, 32, False), (9, 1024, 64, 128, True), (16, 1152, 257, 64, True), (17, 640, 48, 128, False),
+    (33, 256, 31, 64, True), (1, 128, 5, 128, True), (5, 64, 16, 64, False), (4, 16384, 70, 128, True),
+])
+def test_float_activations(dtype, rows, inner, outer, group, biases):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(rows + inner + outer)
+    td = torch_dtype(dtype)
+    x = torch.randn(rows, inner, generator=g, device="cuda").to(td)
+    for scale_dtype in (torch.float16, torch.bfloat16, torch.float32):
+        _check(x, *_weights(g, outer, inner, group, scale_dtype, biases))
+
+
+@pytest.mark.parametrize("x_group", [32, 64, 128, 0])
+@pytest.mark.parametrize("rows, inner, outer, group", [(1, 1536, 100, 128), (8, 768, 65, 64), (11, 384, 40, 32),
+                                                       (2, 6144, 576, 128)])
+def test_8_bit_activations(x_group, rows, inner, outer, group):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(rows * inner + x_group)
+    x = (torch.randn(rows, inner, generator=g, device="cuda") * 100).to(torch.float8_e4m3fn)
+    xs = torch.rand(rows, inner // (x_group or inner), generator=g, device="cuda") + 0.1
+    for biases, out_dtype in ((True, torch.bfloat16), (False, torch.float32), (True, torch.float16)):
+        _check(x, *_weights(g, outer, inner, group, torch.float16, biases), x_scales=xs, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("x_dtype, out_dtype", [("bfloat16", "float32"), ("float16", "bfloat16"), ("float32", "float16")])
+def test_other_output_types(x_dtype, out_dtype):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(3, 512, generator=g, device="cuda").to(torch_dtype(x_dtype))
+    _check(x, *_weights(g, 77, 512, 64, torch.bfloat16, True), out_dtype=torch_dtype(out_dtype))
+
+
+def test_all_codes_in_every_place():
+    """Each nibble of a word reaches its own channel: one channel of x at a time."""
+    import torch
+
+    from mlxlr8_b200.affine4 import affine4_linear
+
+    codes = torch.randint(-(1 << 31), 1 << 31, (16, 32), device="cuda", dtype=torch.int32)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = torch.eye(256, device="cuda", dtype=dtype)
+        for group in (32, 64, 128):
+            scales = torch.ones(16, 256 // group, device="cuda")
+            got = affine4_linear(x, codes, scales, out_dtype=torch.float32)
+            assert torch.equal(got.t().double(), _values(codes) - 8.0)
+
+
+def test_large_and_small_channels_and_infinities():
+    import torch
+
+    from mlxlr8_b200.affine4 import affine4_linear
+
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.randn(2, 1024, generator=g, device="cuda")
+        x[:, 7] = 1e30
+        x[:, 500:600] = 1e-30
+        weights = _weights(g, 40, 1024, 64, torch.float32, True)
+        _check(x.to(dtype), *weights)
+        x[1, 900] = float("nan")
+        got = affine4_linear(x.to(dtype), *weights)
+        assert bool(got[0].isfinite().all()) and bool(got[1].isnan().all())
+
+
+def test_views_out_streams_and_leading_dimensions():
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(10)
+    weights = _weights(g, 96, 256, 64, torch.float16, True)
+    x = torch.randn(256, 6, generator=g, device="cuda").bfloat16().t()
+    _check(x, *weights)
+    _check(torch.randn(2, 3, 256, generator=g, device="cuda").bfloat16(), *weights)
+    _check(torch.randn(256, generator=g, device="cuda").half(), *weights)
+    flat = torch.randn(3 * 256 + 1, generator=g, device="cuda").bfloat16()
+    _check(flat[1:].view(3, 256), *weights)
+    out = torch.empty(6, 96, device="cuda", dtype=torch.float32)
+    assert _check(x, *weights, out=out).data_ptr() == out.data_ptr()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        _check(x, *weights)
+    side.synchronize()
+    codes = weights[0].repeat(1, 2)[:, ::2].contiguous()
+    wide = torch.stack([codes, codes], -1)[..., 0]
+    _check(x, wide, *weights[1:])
+    _check(x, weights[0].view(torch.uint32), *weights[1:])
+
+
+def test_results_do_not_change_between_runs_and_replays():
+    import torch
+
+    from mlxlr8_b200.affine4 import Affine4Linear
+
+    g = torch.Generator(device="cuda").manual_seed(11)
+    layer = Affine4Linear(*_weights(g, 4096, 2048, 64, torch.bfloat16, True))
+    x = torch.randn(3, 2048, generator=g, device="cuda").bfloat16()
+    out = torch.empty(3, 4096, device="cuda", dtype=torch.bfloat16)
+    first = layer(x).clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(x, out=out)
+    for _ in range(5):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, first) and torch.equal(layer(x), first)
+
+
+def test_no_rows_and_refusals():
+    import torch
+
+    from mlxlr8_b200.affine4 import Affine4Linear, affine4_linear
+
+    g = torch.Generator(device="cuda").manual_seed(12)
+    codes, scales, biases = _weights(g, 8, 256, 64, torch.float16, True)
+    x = torch.randn(2, 256, device="cuda").bfloat16()
+    assert affine4_linear(x[:0], codes, scales, biases).shape == (0, 8)
+    x8, xs = x.to(torch.float8_e4m3fn), torch.ones(2, 2, device="cuda")
+    for call in (lambda: affine4_linear(x[:, :128], codes, scales, biases),
+                 lambda: affine4_linear(x, codes.long(), scales, biases),
+                 lambda: affine4_linear(x, codes, scales[:, :3], biases),
+                 lambda: affine4_linear(x, codes, scales, biases.float()),
+                 lambda: affine4_linear(x, codes, scales[:, :1], biases[:, :1]),
+                 lambda: affine4_linear(x, codes, scales, biases, x_scales=xs),
+                 lambda: affine4_linear(x8, codes, scales, biases),
+                 lambda: affine4_linear(x8, codes, scales, biases, x_scales=xs.half()),
+                 lambda: affine4_linear(x8, codes, scales, biases, x_scales=torch.ones(2, 16, device="cuda")),
+                 lambda: affine4_linear(x.double(), codes, scales, biases),
+                 lambda: affine4_linear(x, codes, scales, biases, out=torch.empty(2, 7, device="cuda")),
+                 lambda: affine4_linear(x, codes, scales, biases, out_dtype=torch.int8),
+                 lambda: affine4_linear(x, codes, scales.cpu(), biases),
+                 lambda: Affine4Linear(codes, scales[:4])):
+        with pytest.raises(ValueError):
+            call()
