@@ -125,6 +125,11 @@ int exlr8_latent_prompt_attention(const void* q, int64_t q_token_stride, int64_t
   for (const int64_t stride : {q_token_stride, q_head_stride, k_token_stride, k_head_stride, k_rope_stride,
                                v_token_stride, v_head_stride})
     if (stride < 0 || stride % 8 || stride >= (int64_t{1} << 38)) return EXLR8_ERR_SHAPE;
+  // Broadcast rows have no tile of their own; a grid holds 2^31 CTAs.
+  if ((heads > 1 && (!q_head_stride || !k_head_stride || !v_head_stride)) || (total_q > 1 && !q_token_stride) ||
+      (total_k > 1 && (!k_token_stride || !k_rope_stride || !v_token_stride)))
+    return EXLR8_ERR_SHAPE;
+  if (((total_q + 255) / 256 + seqs) * heads * 2 > kMaxGrid) return EXLR8_ERR_SHAPE;
   if (total_q == 0) return EXLR8_OK;
   if (!q || !out || !q_starts || !k_starts || (total_k > 0 && (!k || !k_rope || !v)) || !std::isfinite(scale))
     return EXLR8_ERR_ARG;

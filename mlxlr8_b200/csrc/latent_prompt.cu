@@ -2,105 +2,420 @@
 // key j is [k_j,h, k_rope_j] (the rotary part is shared by all heads) and its
 // value v_j,h.  Query i of a sequence with n queries and m keys sees its
 // first m - n + 1 + i keys, so a chunk with a history ends with its keys.  A
-// query that sees none gives zeros (and lse -inf).  Statistics in float32.
+// query that sees none gives zeros (and lse -inf).
+//
+// One CTA takes 256 queries of one head, as two tiles of 128 rows, and walks
+// the keys in tiles.  For each query tile q and key tile j
+//   S_q = Q_q K_j^T                      tcgen05, both operands in shared memory
+//   P_q = 2^(c S_q - c m + 6)            one thread per row, float32
+//   O_q += P_q V_j                       tcgen05, P_q from tensor memory
+// with c = |scale| log2(e) (a negative scale negates Q in the instruction),
+// m a running maximum and l = sum P the float32 sum of the unrounded weights.
+// m is raised only when a row's maximum has grown by more than 2^8 (then O and
+// l are multiplied once), so P stays below 2^14 and float16 weights keep their
+// full precision down to 2^-20 of the largest.  Tensor memory is full: S_0,
+// S_1, O_0, O_1 of 128 columns each, P_q over S_q.  While the threads of one
+// query tile form its weights the tensor pipe works for the other one, which
+// is why two tiles share a CTA (and why each K and V tile is read from L2
+// once for 256 queries).
+//
+// Warp 0 loads (TMA), warp 1 issues the matrix instructions, warps 2-5 and
+// 6-9 are the softmax of query tiles 0 and 1.  Value channels beyond 128 are
+// a second CTA's (the scores are formed again there).  Rows of the last key
+// tile that belong to no key of the sequence are zeroed in the V tile, since
+// 0 x NaN would reach the sum.  Waits are bounded; one that runs out leaves
+// NaN in the CTA's output.
+
+#include <cuda.h>
 
 #include "common.cuh"
 #include "latent.cuh"
+#include "tensor_map.cuh"
+#include "umma.cuh"
 
 namespace exlr8 {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kThreads = 320;
+constexpr int kTileQ = 128;
+constexpr float kLift = 6.0f;       // weights are 2^6 of their share of the maximum
+constexpr float kLag = 8.0f;        // log2 by which a maximum may lag
+constexpr uint32_t kRing = 229376;  // 224 KB of operand tiles
 
-// The sequence of query `row`, or -1 (a row behind the last sequence).
-__device__ __forceinline__ int sequence_of(const int32_t* starts, int seqs, int64_t row) {
-  for (int s = 0; s < seqs; ++s)
-    if (row >= starts[s] && row < starts[s + 1]) return s;
-  return -1;
+template <int kBlocks>  // 64-channel blocks of a key: 2, 3 or 4
+struct Tiles {
+  static constexpr int kKeys = kBlocks == 4 ? 64 : 128;
+  static constexpr uint32_t kQ = kBlocks * 16384;         // one query tile
+  static constexpr uint32_t kK = kBlocks * kKeys * 128;   // one key tile
+  static constexpr uint32_t kV = 2 * kKeys * 128;         // one value tile
+  static constexpr int kKStages = 2;
+  static constexpr int kVStages = kBlocks == 3 ? 1 : 2;
+  static_assert(2 * kQ + kKStages * kK + kVStages * kV <= kRing, "operand tiles exceed shared memory");
+};
+
+struct Shared {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_ready[2], o_done[2];
+  uint32_t tmem;
+  int seq, tile;
+};
+
+struct Maps {
+  CUtensorMap q, k, r, v;
+  int q_swap, k_swap, v_swap;  // dimension order (channels, tokens, heads)
+};
+
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, int swap, int channel, int head, int row,
+                                          uint64_t* bar) {
+  if (swap) tma_load_3d(dst, map, channel, row, head, bar);
+  else tma_load_3d(dst, map, channel, head, row, bar);
 }
 
-// One CTA per query and head; a warp takes every fourth key.
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 template <int kAct>
-__global__ void __launch_bounds__(32 * kWarps) latent_prompt_kernel(const LatentPromptArgs a) {
-  __shared__ float s_m[kWarps], s_l[kWarps], s_o[kWarps][256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x;
-  const int h = blockIdx.y;
-  const int seq = sequence_of(a.q_starts, a.seqs, row);
-  if (seq < 0) return;
-  const int64_t k0 = min(static_cast<int64_t>(max(a.k_starts[seq], 0)), a.total_k);
-  const int64_t k1 = min(static_cast<int64_t>(a.k_starts[seq + 1]), a.total_k);
-  const int64_t queries = a.q_starts[seq + 1] - a.q_starts[seq];
-  const int64_t seen = k1 - k0 - queries + 1 + (row - a.q_starts[seq]);
-  const int nb = a.nope / 64, vb = a.value / 64;
-  float q[8], o[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    for (int e = 0; e < 2; ++e) {
-      q[2 * i + e] =
-          i <= nb ? load_act(a.q, kAct, row * a.q_token + h * a.q_head + 64 * i + 2 * lane + e) : 0.0f;
-      o[2 * i + e] = 0.0f;
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t r;
+  if (kAct == kF16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int kAct, int kBlocks>
+__global__ void __launch_bounds__(kThreads, 1)
+    latent_prompt_kernel(const __grid_constant__ Maps maps, const LatentPromptArgs a, int value_parts) {
+  using T = Tiles<kBlocks>;
+  constexpr int kKeys = T::kKeys;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared sh;
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* const k_ring = smem + 2 * T::kQ;
+  uint8_t* const v_ring = k_ring + T::kKStages * T::kK;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int columns = a.heads * value_parts;
+  const int head = blockIdx.x % columns / value_parts, part = blockIdx.x % value_parts;
+
+  // The CTA's sequence and its tile of 256 queries: tiles are numbered over
+  // the sequences and taken from the last (its rows see the most keys).
+  if (warp == 0) {
+    int total = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+      const int s = s0 + lane;
+      int n = s < a.seqs ? (max(a.q_starts[s + 1] - a.q_starts[s], 0) + 255) / 256 : 0;
+      total += __reduce_add_sync(0xffffffffu, n);
     }
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = warp; j < seen; j += kWarps) {
-    float dot = 0.0f;
+    int at = total - 1 - static_cast<int>(blockIdx.x / columns), found = -1, tile = 0;
+    for (int s0 = 0; s0 < a.seqs && at >= 0 && found < 0; s0 += 32) {
+      const int s = s0 + lane;
+      const int n = s < a.seqs ? (max(a.q_starts[s + 1] - a.q_starts[s], 0) + 255) / 256 : 0;
+      int end = n;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      for (int e = 0; e < 2; ++e) {
-        float k = 0.0f;
-        if (i < nb) k = load_act(a.k, kAct, (k0 + j) * a.k_token + h * a.k_head + 64 * i + 2 * lane + e);
-        else if (i == nb) k = load_act(a.k_rope, kAct, (k0 + j) * a.kr_token + 2 * lane + e);
-        dot = fmaf(q[2 * i + e], k, dot);
+      for (int off = 1; off < 32; off <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, end, off);
+        if (lane >= off) end += other;
+      }
+      const uint32_t mine = __ballot_sync(0xffffffffu, at < end);
+      if (mine) {
+        const int which = __ffs(mine) - 1;
+        tile = at - __shfl_sync(0xffffffffu, end - n, which);
+        found = s0 + which;
+      } else {
+        at -= __shfl_sync(0xffffffffu, end, 31);
       }
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    const float s = dot * a.scale;
-    const float top = fmaxf(m, s);
-    if (top == -INFINITY) continue;
-    const float keep = expf(m - top), p = expf(s - top);
-    m = top;
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      for (int e = 0; e < 2; ++e) {
-        if (i >= vb) continue;
-        const float v = load_act(a.v, kAct, (k0 + j) * a.v_token + h * a.v_head + 64 * i + 2 * lane + e);
-        o[2 * i + e] = fmaf(p, v, o[2 * i + e] * keep);
+    if (lane == 0) {
+      sh.seq = found;
+      sh.tile = tile;
+      mbar_init(&sh.q_full, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh.k_full[i], 1);
+        mbar_init(&sh.k_empty[i], 1);
+        mbar_init(&sh.v_full[i], 1);
+        mbar_init(&sh.v_empty[i], 1);
+        mbar_init(&sh.s_full[i], 1);
+        mbar_init(&sh.p_ready[i], kTileQ);
+        mbar_init(&sh.o_done[i], 1);
       }
+      mbar_fence_init();
     }
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    s_o[warp][64 * i + 2 * lane] = o[2 * i];
-    s_o[warp][64 * i + 2 * lane + 1] = o[2 * i + 1];
   }
   __syncthreads();
-  float top = -INFINITY, sum = 0.0f;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w]);
-  for (int w = 0; w < kWarps; ++w) sum += s_l[w] > 0.0f ? s_l[w] * expf(s_m[w] - top) : 0.0f;
-  for (int i = threadIdx.x; i < a.value; i += 32 * kWarps) {
-    float v = 0.0f;
-    for (int w = 0; w < kWarps; ++w) v += s_l[w] > 0.0f ? s_o[w][i] * expf(s_m[w] - top) : 0.0f;
-    store_act(a.out, kAct, (row * a.heads + h) * a.value + i, sum > 0.0f ? v / sum : 0.0f);
+  if (sh.seq < 0) return;
+  const int q0 = min(max(a.q_starts[sh.seq], 0), static_cast<int>(a.total_q));
+  const int queries = min(a.q_starts[sh.seq + 1], static_cast<int>(a.total_q)) - q0;
+  const int k0 = min(max(a.k_starts[sh.seq], 0), static_cast<int>(a.total_k));
+  const int keys = max(min(a.k_starts[sh.seq + 1], static_cast<int>(a.total_k)) - k0, 0);
+  const int first = sh.tile * 256;
+  const int vb = min(2, a.value / 64 - 2 * part);  // 64-channel value blocks of this CTA
+  // Key tiles of each query tile: its last query sees the most keys.
+  int tiles[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int last = min(first + (q + 1) * kTileQ, queries) - 1;
+    const int seen = last >= first + q * kTileQ ? min(keys - queries + 1 + last, keys) : 0;
+    tiles[q] = seen > 0 ? (seen + kKeys - 1) / kKeys : 0;
   }
-  if (a.lse && threadIdx.x == 0) a.lse[row * a.heads + h] = sum > 0.0f ? top + logf(sum) : -INFINITY;
+  const int all = max(tiles[0], tiles[1]);
+  if (warp == 1) tmem_alloc(&sh.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == 0) {
+    if (lane == 0 && all > 0) {
+      bool ok = true;
+      mbar_arrive_expect_tx(&sh.q_full, 2 * T::kQ);
+      for (int q = 0; q < 2; ++q)
+        for (int b = 0; b < kBlocks; ++b)
+          load_tile(smem + q * T::kQ + b * 16384, &maps.q, maps.q_swap, 64 * b, head, q0 + first + q * kTileQ,
+                    &sh.q_full);
+      int j = 0;
+      for (; j < all && ok; ++j) {
+        const int ks = j % T::kKStages, vs = j % T::kVStages;
+        if (j >= T::kKStages) ok = mbar_wait(&sh.k_empty[ks], (j / T::kKStages - 1) & 1);
+        if (!ok) break;
+        uint8_t* kt = k_ring + ks * T::kK;
+        mbar_arrive_expect_tx(&sh.k_full[ks], T::kK);
+        for (int b = 0; b < kBlocks - 1; ++b)
+          load_tile(kt + b * kKeys * 128, &maps.k, maps.k_swap, 64 * b, head, k0 + j * kKeys, &sh.k_full[ks]);
+        tma_load_2d(kt + (kBlocks - 1) * kKeys * 128, &maps.r, 0, k0 + j * kKeys, &sh.k_full[ks]);
+        if (j >= T::kVStages) ok = mbar_wait(&sh.v_empty[vs], (j / T::kVStages - 1) & 1);
+        if (!ok) {
+          mbar_wait(&sh.k_full[ks], (j / T::kKStages) & 1);
+          break;
+        }
+        uint8_t* vt = v_ring + vs * T::kV;
+        mbar_arrive_expect_tx(&sh.v_full[vs], vb * kKeys * 128);
+        for (int b = 0; b < vb; ++b)
+          load_tile(vt + b * kKeys * 128, &maps.v, maps.v_swap, 128 * part + 64 * b, head, k0 + j * kKeys,
+                    &sh.v_full[vs]);
+      }
+      // Copies still in flight land before the CTA's memory is given back.
+      mbar_wait(&sh.q_full, 0);
+      for (int u = max(0, j - 2); u < j; ++u) mbar_wait(&sh.k_full[u % T::kKStages], (u / T::kKStages) & 1);
+      for (int u = max(0, j - T::kVStages); u < j; ++u) mbar_wait(&sh.v_full[u % T::kVStages], (u / T::kVStages) & 1);
+    }
+  } else if (warp == 1) {
+    const uint32_t score_desc = half_idesc(kAct == kBF16, kKeys, a.scale < 0.0f, false, false);
+    const uint32_t value_desc = half_idesc(kAct == kBF16, 64 * vb, false, false, true);
+    const uint32_t sq = smem_u32(smem), sk = smem_u32(k_ring), sv = smem_u32(v_ring);
+    bool ok = all == 0 || mbar_wait(&sh.q_full, 0);
+    // S_q of key tile j.
+    auto scores = [&](int q, int j) {
+      const uint32_t kt = sk + (j % T::kKStages) * T::kK;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          tc_mma_f16(tmem + q * 128, umma_desc_sw128(sq + q * T::kQ + b * 16384 + kk * 32),
+                     umma_desc_sw128(kt + b * kKeys * 128 + kk * 32), score_desc, (b | kk) != 0);
+      tc_commit(&sh.s_full[q]);
+    };
+    if (ok && all > 0) ok = mbar_wait(&sh.k_full[0], 0);
+    if (ok && all > 0 && lane == 0) {
+      tc_fence_after();
+      for (int q = 0; q < 2; ++q)
+        if (tiles[q] > 0) scores(q, 0);
+      tc_commit(&sh.k_empty[0]);
+    }
+    for (int j = 0; j < all && ok; ++j) {
+      const int vs = j % T::kVStages;
+      ok = mbar_wait(&sh.v_full[vs], (j / T::kVStages) & 1);
+      if (!ok) break;
+      const int valid = keys - j * kKeys;
+      if (valid < kKeys) {  // rows behind the sequence's last key
+        for (int i = lane; i < (kKeys - valid) * 8; i += 32)
+          for (int b = 0; b < vb; ++b)
+            reinterpret_cast<uint4*>(v_ring + vs * T::kV + (b * kKeys + valid) * 128)[i] = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+        __syncwarp();
+      }
+      bool next = j + 1 >= all;  // key tile j + 1 has arrived
+      for (int q = 0; q < 2 && ok; ++q) {
+        if (j >= tiles[q]) continue;
+        ok = mbar_wait(&sh.p_ready[q], j & 1);
+        if (ok && !next) {
+          ok = mbar_wait(&sh.k_full[(j + 1) % T::kKStages], ((j + 1) / T::kKStages) & 1);
+          next = true;
+        }
+        if (!ok) break;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint32_t vt = sv + vs * T::kV;
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            tc_mma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + kk * 8,
+                          umma_desc_rows128(vt + kk * 2048, kKeys * 128), value_desc, (j | kk) != 0);
+          if (j + 1 < tiles[q]) scores(q, j + 1);
+          else tc_commit(&sh.o_done[q]);
+        }
+      }
+      if (ok && lane == 0) {
+        tc_commit(&sh.v_empty[vs]);
+        if (j + 1 < all) tc_commit(&sh.k_empty[(j + 1) % T::kKStages]);
+      }
+    }
+  } else {
+    const int q = (warp - 2) / 4, quad = warp & 3;
+    const int row = first + q * kTileQ + quad * 32 + lane;
+    const int seen = row < queries ? min(keys - queries + 1 + row, keys) : 0;
+    const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
+    const uint32_t ts = tmem + lanes + q * 128, to = tmem + lanes + 256 + q * 128;
+    const float c = fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < tiles[q]; ++j) {
+      ok = mbar_wait(&sh.s_full[q], j & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[kKeys];
+#pragma unroll
+      for (int i = 0; i < kKeys; i += 32) tc_ld32(ts + i, s + i);
+      tc_wait_ld();
+      tc_settle<kKeys>(s);
+      const int left = seen - j * kKeys;
+      if (__any_sync(0xffffffffu, left < kKeys)) {
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i)
+          if (i >= left) s[i] = 0xff800000u;
+      }
+      float top[4] = {m, m, m, m};
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
+      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      // PV of tile j - 1 is complete: this tile's scores were committed after it.
+      if (j == 0) {
+        m = best;
+      } else if (__any_sync(0xffffffffu, (best - m) * c > kLag)) {
+        const float keep = best > m ? exp2_fast((m - best) * c) : 1.0f;
+        m = best;
+        l *= keep;
+#pragma unroll 1
+        for (int i = 0; i < 64 * vb; i += 32) {
+          uint32_t o[32];
+          tc_ld32(to + i, o);
+          tc_wait_ld();
+          tc_settle<32>(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+          tc_st32(to + i, o);
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : kLift - m * c;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < kKeys; i += 32) {
+        uint32_t p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float u = exp2_fast(fmaf(__uint_as_float(s[i + 2 * e]), c, base));
+          const float v = exp2_fast(fmaf(__uint_as_float(s[i + 2 * e + 1]), c, base));
+          sum[(2 * e) & 3] += u;
+          sum[(2 * e + 1) & 3] += v;
+          p[e] = pack<kAct>(u, v);
+        }
+        tc_st16(ts + i / 2, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(&sh.p_ready[q]);
+    }
+    if (tiles[q] > 0 && ok) ok = mbar_wait(&sh.o_done[q], 0);
+    tc_fence_after();
+    const bool store = row < queries;
+    const int64_t at = (static_cast<int64_t>(q0) + row) * a.heads + head;
+    if (a.lse && part == 0 && store)
+      a.lse[at] = l > 0.0f ? (m * c - kLift + log2f(l)) * 0.6931471805599453f : (l == 0.0f ? -INFINITY : l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    for (int i = 0; i < 64 * vb; i += 32) {
+      uint32_t o[32];
+      if (tiles[q] > 0) {
+        tc_ld32(to + i, o);
+        tc_wait_ld();
+        tc_settle<32>(o);
+      }
+      if (!store) continue;
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * a.value + 128 * part + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t w[4];
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          float u = __uint_as_float(o[8 * e + 2 * f]) * inv, v = __uint_as_float(o[8 * e + 2 * f + 1]) * inv;
+          if (seen <= 0) u = v = 0.0f;
+          if (!ok) u = v = __int_as_float(0x7fc00000);
+          w[f] = pack<kAct>(u, v);
+        }
+        dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_free(tmem, 512);
+}
+
+// A map over [tokens][heads][channels] rows, boxes of 64 channels x `rows`
+// tokens; the two outer dimensions in ascending order of their strides.
+bool encode_rows(CUtensorMap* map, int* swap, CUtensorMapDataType type, const void* base, int channels, int heads,
+                 int64_t tokens, int64_t token_stride, int64_t head_stride, uint32_t rows) {
+  const uint64_t least = (static_cast<uint64_t>(channels) * 2 + 15) / 16 * 16;
+  uint64_t hs = heads > 1 ? static_cast<uint64_t>(head_stride) * 2 : least;
+  uint64_t ts = tokens > 1 ? static_cast<uint64_t>(token_stride) * 2 : hs * heads;
+  *swap = ts < hs;
+  const uint64_t n = static_cast<uint64_t>(tokens), h = static_cast<uint64_t>(heads), d = static_cast<uint64_t>(channels);
+  if (*swap) return encode_tiled_3d(map, type, base, {d, n, h}, {ts, hs}, {64, rows, 1}, CU_TENSOR_MAP_SWIZZLE_128B);
+  return encode_tiled_3d(map, type, base, {d, h, n}, {hs, ts}, {64, 1, rows}, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int kAct, int kBlocks>
+cudaError_t launch(const LatentPromptArgs& a, cudaStream_t s) {
+  using T = Tiles<kBlocks>;
+  const CUtensorMapDataType type =
+      kAct == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  Maps maps;
+  // Without keys no tile is loaded; the maps then describe the queries.
+  const bool empty = a.total_k == 0;
+  const int64_t keys = empty ? a.total_q : a.total_k;
+  if (!encode_rows(&maps.q, &maps.q_swap, type, a.q, a.nope + kLatentRope, a.heads, a.total_q, a.q_token, a.q_head,
+                   kTileQ) ||
+      !encode_rows(&maps.k, &maps.k_swap, type, empty ? a.q : a.k, empty ? 64 : a.nope, a.heads, keys,
+                   empty ? a.q_token : a.k_token, empty ? a.q_head : a.k_head, T::kKeys) ||
+      !encode_tiled_2d(&maps.r, type, empty ? a.q : a.k_rope, 64, keys,
+                       2 * (empty ? a.q_token : (keys > 1 ? a.kr_token : 64)), 64, T::kKeys,
+                       CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_rows(&maps.v, &maps.v_swap, type, empty ? a.q : a.v, empty ? 64 : a.value, a.heads, keys,
+                   empty ? a.q_token : a.v_token, empty ? a.q_head : a.v_head, T::kKeys))
+    return cudaErrorInvalidValue;
+  auto kernel = latent_prompt_kernel<kAct, kBlocks>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing + 1024);
+  if (err != cudaSuccess) return err;
+  const int parts = (a.value + 127) / 128;
+  const int64_t tiles = (a.total_q + 255) / 256 + a.seqs;
+  kernel<<<static_cast<unsigned>(tiles * a.heads * parts), kThreads, kRing + 1024, s>>>(maps, a, parts);
+  return cudaGetLastError();
+}
+
+template <int kAct>
+cudaError_t launch_blocks(const LatentPromptArgs& a, cudaStream_t s) {
+  if (a.nope == 64) return launch<kAct, 2>(a, s);
+  if (a.nope == 128) return launch<kAct, 3>(a, s);
+  return launch<kAct, 4>(a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_latent_prompt(const LatentPromptArgs& a, cudaStream_t s) {
-  if (a.total_q == 0 || a.seqs == 0) return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>(a.total_q), a.heads);
-  if (a.dtype == kF16) latent_prompt_kernel<kF16><<<grid, 32 * kWarps, 0, s>>>(a);
-  else latent_prompt_kernel<kBF16><<<grid, 32 * kWarps, 0, s>>>(a);
-  return cudaGetLastError();
+  if (a.total_q == 0) return cudaSuccess;
+  return a.dtype == kF16 ? launch_blocks<kF16>(a, s) : launch_blocks<kBF16>(a, s);
 }
 
 }  // namespace exlr8

@@ -153,13 +153,15 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
 
 def _heads_first(name, t, dtype):
     """``t [tokens, heads, channels]`` as the kernel takes it: contiguous
-    channels, 16-byte rows (a copy where a view has neither)."""
+    channels, rows of their own on 16 bytes (a copy of any other view)."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, channels]")
     _half(name, t, dtype)
     a, b, c = t.stride()
-    return t if c == 1 and a % 8 == 0 and b % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(
-        memory_format=torch.contiguous_format)
+    if c == 1 and a % 8 == 0 and b % 8 == 0 and (a > 0 or t.shape[0] < 2) and (b > 0 or t.shape[1] < 2) \
+            and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def latent_prompt_attention(q, k, k_rope, v, q_starts, k_starts, scale: float, *, out=None, return_lse: bool = False):
@@ -186,7 +188,8 @@ def latent_prompt_attention(q, k, k_rope, v, q_starts, k_starts, scale: float, *
     if width != nope + ROPE or heads == 0 or tuple(k.shape[:2]) != (total_k, heads) \
             or tuple(v.shape[:2]) != (total_k, heads) or tuple(k_rope.shape) != (total_k, ROPE):
         raise ValueError("q, k, k_rope and v do not match")
-    if k_rope.stride(1) != 1 or k_rope.stride(0) % 8 or k_rope.data_ptr() % 16:
+    if k_rope.stride(1) != 1 or k_rope.stride(0) % 8 or (k_rope.stride(0) == 0 and total_k > 1) \
+            or k_rope.data_ptr() % 16:
         k_rope = k_rope.clone(memory_format=torch.contiguous_format)
     seqs = q_starts.numel() - 1
     if not 1 <= seqs <= 4096:
