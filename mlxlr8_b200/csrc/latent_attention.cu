@@ -1,99 +1,722 @@
 // Attention over the paged latent cache (absorbed form): every head of a
 // query attends the same row [c_j, k_j] of a token,
-//   s_j = scale * (ql . c_j + qr . k_j),  out = sum_j softmax(s)_j c_j,
-// in one pass with the running maximum and sum of the softmax in float32.
+//   s_j = scale * (ql . c_j + qr . k_j),  out = sum_j softmax(s)_j c_j.
 // Query t of T sees the first length - T + 1 + t tokens; a query that sees
 // none gives zeros (and lse -inf).  Table entries outside the cache hold no
 // tokens.
+//
+// The rows (query, head) of a sequence are the narrow side, so both products
+// are taken transposed, with 128 tokens or 128 latent channels on the tensor
+// core's M side and kN = 16, 32 or 64 rows on its N side:
+//   S^T [128 tokens][kN]  = C Q^T       cache tile as loaded (channels contiguous)
+//   P^T = 2^(c S^T + base)              one thread per token, float32, to shared memory
+//   O^T [rank][kN]       += C^T P^T     the same tile, taken with its tokens contracted
+// A cache tile is read from memory once and feeds both products.  base = 6 -
+// c m with c = |scale| log2(e) (a negative scale negates the cache tile in the
+// instruction) and m a row's maximum when it was last raised: it is raised,
+// and O and the sums multiplied, only when a score has grown past it by 2^8,
+// so a tile needs no maximum over its tokens, only the vote that none has.
+// Weights stay below 2^14 and float16 ones keep full precision down to 2^-20
+// of the largest.  Sums are float32, of the unrounded weights.
+//
+// Work is the flat list of (sequence, row tile, 128 tokens), cut evenly over
+// the CTAs (one per SM) whatever the lengths; a sequence cut in two or more
+// leaves float32 parts in the workspace, which a second kernel joins.
+//
+// Warp 0 loads (TMA; one box per page or 16 to 128 of its tokens), warp 1
+// issues the matrix instructions, warps 2-5 and 6-9 each take half of the
+// rows for all 128 tokens.  The latent is loaded as pairs of 64-channel
+// blocks (one M = 128 of the second product) into a ring; a pair is given back
+// as soon as its product is done.  Where shared memory has no room for the
+// rotary block it shares P's buffer: the scores are done with it before P is
+// written.  Token rows that belong to no token are zeroed in the tile, since
+// 0 x NaN would reach the sum.  Waits are bounded; one that runs out leaves NaN
+// in the rows that it concerns.
+
+#include <cuda.h>
 
 #include "common.cuh"
 #include "latent.cuh"
+#include "launch.cuh"
+#include "tensor_map.cuh"
+#include "umma.cuh"
 
 namespace exlr8 {
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kThreads = 320;
+constexpr int kTile = 128;  // tokens
+constexpr float kLift = 6.0f;
+constexpr float kLag = 8.0f;
+constexpr uint32_t kBlock = kTile * 128;  // 128 tokens x 64 channels
+constexpr uint32_t kPair = 2 * kBlock;
+constexpr int kMaxPairs = 8;        // ring slots
+constexpr int kMinTiles = 2;        // tiles a CTA takes at least, where there are as many
+constexpr uint32_t kSmem = 229888;  // dynamic shared memory, with 1 KB for its alignment
 
-// One CTA per query and head; a warp takes every eighth token, a lane two
-// channels of each 64, and the warps' states join in shared memory.
-template <int kAct>
-__global__ void __launch_bounds__(32 * kWarps) latent_attention_kernel(const LatentAttentionArgs a) {
-  __shared__ float s_m[kWarps], s_l[kWarps], s_o[kWarps][kLatentMaxRank];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x;
-  const int64_t b = row / (static_cast<int64_t>(a.queries) * a.heads);
-  const int t = static_cast<int>(row / a.heads % a.queries);
-  const int nb = a.rank / 64;
-  float q[2 * (kLatentMaxRank / 64 + 1)], o[2 * (kLatentMaxRank / 64)];
+// ---- the flat list of tiles -----------------------------------------------------
+
+struct Work {
+  int64_t batch;
+  int queries, heads, row_tiles;
+  int64_t room;  // tokens a table holds
+  const int32_t* lengths;
+};
+
+__device__ __forceinline__ int tokens_of(const Work& w, int64_t b) {
+  return static_cast<int>(min(static_cast<int64_t>(max(w.lengths[b], 0)), w.room));
+}
+__device__ __forceinline__ int tiles_of(const Work& w, int64_t b) { return (tokens_of(w, b) + kTile - 1) / kTile; }
+
+// Tiles of all sequences; the calling warp takes part as a whole.
+__device__ int64_t total_tiles(const Work& w, int lane) {
+  int64_t n = 0;
+  for (int64_t b = lane; b < w.batch; b += 32) n += tiles_of(w, b);
 #pragma unroll
-  for (int i = 0; i < kLatentMaxRank / 64 + 1; ++i) {
-    for (int e = 0; e < 2; ++e)
-      q[2 * i + e] = i < nb ? load_act(a.q_latent, kAct, row * a.rank + 64 * i + 2 * lane + e) : 0.0f;
+  for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+  return n * w.row_tiles;
+}
+
+// The sequence of flat tile `at` (at < total), and the tiles before it.
+__device__ void find_sequence(const Work& w, int64_t at, int lane, int64_t* sequence, int64_t* before) {
+  int64_t base = 0;
+  for (int64_t b0 = 0; b0 < w.batch; b0 += 32) {
+    const int64_t b = b0 + lane;
+    const int64_t n = b < w.batch ? static_cast<int64_t>(tiles_of(w, b)) * w.row_tiles : 0;
+    int64_t end = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, end, off);
+      if (lane >= off) end += other;
+    }
+    const uint32_t mine = __ballot_sync(0xffffffffu, at < base + end);
+    if (mine) {
+      const int which = __ffs(mine) - 1;
+      *sequence = b0 + which;
+      *before = base + __shfl_sync(0xffffffffu, end - n, which);
+      return;
+    }
+    base += __shfl_sync(0xffffffffu, end, 31);
   }
-  const float r0 = load_act(a.q_rope, kAct, row * 64 + 2 * lane), r1 = load_act(a.q_rope, kAct, row * 64 + 2 * lane + 1);
-#pragma unroll
-  for (int i = 0; i < 2 * (kLatentMaxRank / 64); ++i) o[i] = 0.0f;
-  const int64_t room = static_cast<int64_t>(a.table_width) * a.page_size;
-  const int64_t length = min(static_cast<int64_t>(a.lengths[b]), room);
-  const int64_t seen = length - a.queries + 1 + t;
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = warp; j < seen; j += kWarps) {
-    const int page = a.block_table[b * a.table_width + j / a.page_size];
-    if (page < 0 || page >= a.pages) continue;
-    const int64_t at = (static_cast<int64_t>(page) * a.page_size + j % a.page_size) * (a.rank + kLatentRope);
-    float c[2 * (kLatentMaxRank / 64)];
-    float dot = r0 * load_act(a.cache, kAct, at + a.rank + 2 * lane) +
-                r1 * load_act(a.cache, kAct, at + a.rank + 2 * lane + 1);
-#pragma unroll
-    for (int i = 0; i < kLatentMaxRank / 64; ++i) {
-      for (int e = 0; e < 2; ++e) {
-        c[2 * i + e] = i < nb ? load_act(a.cache, kAct, at + 64 * i + 2 * lane + e) : 0.0f;
-        dot = fmaf(q[2 * i + e], c[2 * i + e], dot);
+  *sequence = w.batch;
+  *before = base;
+}
+
+// CTAs that share `total` tiles, and the first tile of one of them.
+__device__ __forceinline__ int64_t sharers(int64_t total, int ctas) {
+  const int64_t n = (total + kMinTiles - 1) / kMinTiles;
+  return n < ctas ? n : ctas;
+}
+__device__ __forceinline__ int64_t first_tile(int64_t i, int64_t total, int64_t n) { return i * total / n; }
+
+// A CTA's walk over its share: one segment per (sequence, row tile).
+struct Walk {
+  int64_t b, left;  // sequence, tiles of the share not yet taken
+  int rt, tile;     // row tile, first tile of the next segment
+  // the segment
+  int64_t sb;
+  int srt, begin, end, tokens, tiles;
+  __device__ __forceinline__ bool next(const Work& w) {
+    if (left <= 0) return false;
+    tokens = tokens_of(w, b);
+    tiles = (tokens + kTile - 1) / kTile;
+    while (tile >= tiles) {  // on to the next row tile, then the next sequence that has tokens
+      tile = 0;
+      if (++rt >= w.row_tiles) {
+        rt = 0;
+        if (++b >= w.batch) return false;
+        tokens = tokens_of(w, b);
+        tiles = (tokens + kTile - 1) / kTile;
+      } else if (tiles == 0) {
+        rt = w.row_tiles - 1;
       }
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    const float s = dot * a.scale;
-    const float top = fmaxf(m, s);
-    if (top == -INFINITY) continue;
-    const float keep = expf(m - top), p = expf(s - top);
-    m = top;
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < 2 * (kLatentMaxRank / 64); ++i) o[i] = fmaf(p, c[i], o[i] * keep);
+    sb = b;
+    srt = rt;
+    begin = tile;
+    end = static_cast<int>(min(static_cast<int64_t>(tiles), begin + left));
+    left -= end - begin;
+    tile = end;
+    return true;
   }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < kLatentMaxRank / 64; ++i) {
-    s_o[warp][64 * i + 2 * lane] = o[2 * i];
-    s_o[warp][64 * i + 2 * lane + 1] = o[2 * i + 1];
+};
+
+// ---- the main kernel -------------------------------------------------------------
+
+struct Layout {
+  uint32_t q, p, rope, ring;  // byte offsets in shared memory
+  int pairs, ropes;           // ring slots; rotary buffers (0: it shares P's)
+};
+
+struct Shared {
+  uint64_t q_full, q_empty, s_full, p_ready, o_done;
+  uint64_t full[kMaxPairs], empty[kMaxPairs], rope_full[2], rope_empty[2];
+  uint32_t tmem;
+  Walk walk;
+  __align__(16) float base[64];
+  __align__(16) float factor[64];
+  float m[64];
+  float top[4][64];
+  int limit[64];
+};
+
+struct Maps {
+  CUtensorMap q, r, cache;
+};
+
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool group_any(int id, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n bar.red.or.pred q, %1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(id), "r"(static_cast<uint32_t>(v))
+      : "memory");
+  return r != 0;
+}
+
+template <int kAct>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t r;
+  if (kAct == kF16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int kCols>
+__device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[kCols]) {
+  if constexpr (kCols == 32) tc_ld32(taddr, v);
+  else if constexpr (kCols == 16) tc_ld16(taddr, v);
+  else tc_ld8(taddr, v);
+}
+template <int kCols>
+__device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&v)[kCols]) {
+  if constexpr (kCols == 32) tc_st32(taddr, v);
+  else if constexpr (kCols == 16) tc_st16(taddr, v);
+  else tc_st8(taddr, v);
+}
+
+// parts: [2 * CTAs][kN][rank] float32, then [2 * CTAs][kN] pairs (log2 of the
+// unit of O and the sum, sum).
+template <int kAct, int kN>
+__global__ void __launch_bounds__(kThreads, 1)
+    latent_attention_kernel(const __grid_constant__ Maps maps, const LatentAttentionArgs a, const Work w, const Layout lay,
+                            int box, uint32_t columns, float* __restrict__ parts, float2* __restrict__ sums) {
+  pdl_launch_dependents();
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared sh;
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int blocks = a.rank / 64, tile_pairs = a.rank / 128;
+  if (warp == 0) {
+    const int64_t total = total_tiles(w, lane);
+    const int64_t n = sharers(total, gridDim.x);
+    Walk walk{};
+    if (blockIdx.x < n) {
+      const int64_t at = first_tile(blockIdx.x, total, n);
+      int64_t sequence, before;
+      find_sequence(w, at, lane, &sequence, &before);
+      const int tiles = tiles_of(w, sequence);
+      walk.b = sequence;
+      walk.left = first_tile(blockIdx.x + 1, total, n) - at;
+      walk.rt = static_cast<int>((at - before) / tiles);
+      walk.tile = static_cast<int>((at - before) % tiles);
+    }
+    if (lane == 0) {
+      sh.walk = walk;
+      mbar_init(&sh.q_full, 1);
+      mbar_init(&sh.q_empty, 1);
+      mbar_init(&sh.s_full, 1);
+      mbar_init(&sh.p_ready, 256);
+      mbar_init(&sh.o_done, 1);
+      for (int i = 0; i < kMaxPairs; ++i) {
+        mbar_init(&sh.full[i], 1);
+        mbar_init(&sh.empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh.rope_full[i], 1);
+        mbar_init(&sh.rope_empty[i], 1);
+      }
+      mbar_fence_init();
+    }
   }
   __syncthreads();
-  float top = -INFINITY, sum = 0.0f;
-  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w]);
-  for (int w = 0; w < kWarps; ++w) sum += s_l[w] > 0.0f ? s_l[w] * expf(s_m[w] - top) : 0.0f;
-  for (int i = threadIdx.x; i < a.rank; i += 32 * kWarps) {
-    float v = 0.0f;
-    for (int w = 0; w < kWarps; ++w) v += s_l[w] > 0.0f ? s_o[w][i] * expf(s_m[w] - top) : 0.0f;
-    store_act(a.out, kAct, row * a.rank + i, sum > 0.0f ? v / sum : 0.0f);
+  Walk walk = sh.walk;
+  if (walk.left <= 0) return;
+  if (warp == 1) tmem_alloc(&sh.tmem, columns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem, t_scores = tmem + tile_pairs * kN;
+  const int ropes = lay.ropes > 0 ? lay.ropes : 1;
+  const uint32_t rope_at = lay.ropes > 0 ? lay.rope : lay.p;
+  bool ok = true;
+
+  if (warp == 0) {
+    int u = 0, pair = 0;  // tiles and pairs loaded so far
+    int segment = 0;
+    for (; ok && walk.next(w); ++segment) {
+      if (segment > 0) ok = mbar_wait(&sh.q_empty, (segment - 1) & 1);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sh.q_full, (blocks + 1) * kN * 128);
+        for (int i = 0; i < blocks; ++i)
+          tma_load_3d(smem + lay.q + i * kN * 128, &maps.q, 64 * i, walk.srt * kN, static_cast<int>(walk.sb), &sh.q_full);
+        tma_load_3d(smem + lay.q + blocks * kN * 128, &maps.r, 0, walk.srt * kN, static_cast<int>(walk.sb), &sh.q_full);
+      }
+      for (int t = walk.begin; ok && t < walk.end; ++t, ++u) {
+        // Lane i fetches the tokens [i * box, (i + 1) * box) of the tile.
+        const int token = t * kTile + lane * box;
+        int row = -1;
+        if (lane * box < kTile && token < walk.tokens) {
+          const int page = a.block_table[walk.sb * a.table_width + token / a.page_size];
+          if (page >= 0 && page < a.pages) row = page * a.page_size + token % a.page_size;
+        }
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row >= 0)) * box * 128;
+        for (int i = 0; ok && i < tile_pairs; ++i, ++pair) {
+          const int slot = pair % lay.pairs;
+          if (pair >= lay.pairs) ok = mbar_wait(&sh.empty[slot], (pair / lay.pairs - 1) & 1);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], 2 * bytes);
+          __syncwarp();
+          if (row >= 0) {
+            uint8_t* dst = smem + lay.ring + slot * kPair + lane * box * 128;
+            tma_load_2d(dst, &maps.cache, 128 * i, row, &sh.full[slot]);
+            tma_load_2d(dst + kBlock, &maps.cache, 128 * i + 64, row, &sh.full[slot]);
+          }
+        }
+        if (!ok) break;
+        const int r = u % ropes;
+        if (u >= ropes) ok = mbar_wait(&sh.rope_empty[r], (u / ropes - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&sh.rope_full[r], bytes);
+        __syncwarp();
+        if (row >= 0) tma_load_2d(smem + rope_at + r * kBlock + lane * box * 128, &maps.cache, a.rank, row, &sh.rope_full[r]);
+      }
+    }
+    // Copies still in flight land before the CTA's memory is given back.
+    if (segment > 0) mbar_wait(&sh.q_full, (segment - 1) & 1);
+    for (int i = max(0, pair - lay.pairs); i < pair; ++i) mbar_wait(&sh.full[i % lay.pairs], (i / lay.pairs) & 1);
+    for (int i = max(0, u - ropes); i < u; ++i) mbar_wait(&sh.rope_full[i % ropes], (i / ropes) & 1);
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t score_desc = half_idesc(kAct == kBF16, kN, a.scale < 0.0f, false, false);
+      const uint32_t value_desc = half_idesc(kAct == kBF16, kN, false, true, true);
+      const uint32_t sq = smem_u32(smem + lay.q), sp = smem_u32(smem + lay.p), ring = smem_u32(smem + lay.ring),
+                     sr = smem_u32(smem + rope_at);
+      int u = 0, pair = 0;
+      for (int segment = 0; ok && walk.next(w); ++segment) {
+        ok = mbar_wait(&sh.q_full, segment & 1);
+        for (int t = walk.begin; ok && t < walk.end; ++t, ++u, pair += tile_pairs) {
+          for (int i = 0; ok && i < tile_pairs; ++i) {
+            const int slot = (pair + i) % lay.pairs;
+            ok = mbar_wait(&sh.full[slot], ((pair + i) / lay.pairs) & 1);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              tc_mma_f16(t_scores, umma_desc_sw128(ring + slot * kPair + (k / 4) * kBlock + (k % 4) * 32),
+                         umma_desc_sw128(sq + (2 * i + k / 4) * kN * 128 + (k % 4) * 32), score_desc, (i | k) != 0);
+          }
+          const int r = u % ropes;
+          if (ok) ok = mbar_wait(&sh.rope_full[r], (u / ropes) & 1);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16(t_scores, umma_desc_sw128(sr + r * kBlock + k * 32),
+                       umma_desc_sw128(sq + blocks * kN * 128 + k * 32), score_desc, 1);
+          tc_commit(&sh.s_full);
+          if (lay.ropes > 0) tc_commit(&sh.rope_empty[r]);
+          if (t + 1 == walk.end) tc_commit(&sh.q_empty);
+          ok = mbar_wait(&sh.p_ready, u & 1);
+          if (!ok) break;
+          tc_fence_after();
+          for (int i = 0; i < tile_pairs; ++i) {
+            const int slot = (pair + i) % lay.pairs;
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+              tc_mma_f16(tmem + i * kN, umma_desc_rows128(ring + slot * kPair + k * 2048, kBlock),
+                         umma_desc_rows128(sp + k * 2048, kBlock), value_desc, t > walk.begin || k > 0);
+            tc_commit(&sh.empty[slot]);
+          }
+          if (lay.ropes == 0) tc_commit(&sh.rope_empty[r]);
+          if (t + 1 == walk.end) tc_commit(&sh.o_done);
+        }
+      }
+    }
+  } else {
+    constexpr int kCols = kN / 2;
+    const int half = (warp - 2) / 4, quad = warp & 3, bar = 1 + half;
+    const int token_row = quad * 32 + lane, col0 = half * kCols;
+    const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
+    const float c = fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f;
+    const int rows = a.queries * a.heads;
+    int u = 0, pair = 0;
+    for (int segment = 0; walk.next(w); ++segment) {
+      // One warp of each half keeps its rows' maxima and limits.
+      if (quad == 0 && lane < kCols) {
+        const int row = walk.srt * kN + col0 + lane;
+        sh.base[col0 + lane] = INFINITY;
+        sh.m[col0 + lane] = -INFINITY;
+        sh.limit[col0 + lane] = row < rows ? walk.tokens - a.queries + 1 + row / a.heads : walk.tokens;
+      }
+      group_sync(bar);
+      const int least = walk.tokens - a.queries + 1 + walk.srt * kN / a.heads;
+      float l[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) l[i] = 0.0f;
+      for (int t = walk.begin; t < walk.end; ++t, ++u, pair += tile_pairs) {
+        const int token = t * kTile + token_row;
+        bool held = token < walk.tokens;
+        if (held) {
+          const int page = a.block_table[walk.sb * a.table_width + token / a.page_size];
+          held = page >= 0 && page < a.pages;
+        }
+        if (ok) ok = mbar_wait(&sh.s_full, u & 1);
+        tc_fence_after();
+        uint32_t s[kCols];
+        load_columns<kCols>(t_scores + lanes + col0, s);
+        tc_wait_ld();
+        tc_settle<kCols>(s);
+        if (!held && ok) {
+          for (int i = half * blocks / 2; i < (half + 1) * blocks / 2; ++i) {
+            uint4* line = reinterpret_cast<uint4*>(smem + lay.ring + (pair + i / 2) % lay.pairs * kPair +
+                                                   (i & 1) * kBlock + token_row * 128);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) line[e] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        if (__any_sync(0xffffffffu, !held || token >= least)) {
+#pragma unroll
+          for (int i = 0; i < kCols; ++i)
+            if (!held || token >= sh.limit[col0 + i]) s[i] = 0xff800000u;
+        }
+        float grown = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kCols; i += 4) {
+          const float4 base = *reinterpret_cast<const float4*>(&sh.base[col0 + i]);
+          grown = fmaxf(grown, fmaxf(fmaf(__uint_as_float(s[i]), c, base.x), fmaf(__uint_as_float(s[i + 1]), c, base.y)));
+          grown = fmaxf(grown, fmaxf(fmaf(__uint_as_float(s[i + 2]), c, base.z), fmaf(__uint_as_float(s[i + 3]), c, base.w)));
+        }
+        if (group_any(bar, grown > kLift + kLag)) {
+          float mine = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) {
+            const float top = warp_max(__uint_as_float(s[i]));
+            if (lane == i) mine = top;
+          }
+          if (lane < kCols) sh.top[quad][col0 + lane] = mine;
+          group_sync(bar);
+          if (quad == 0 && lane < kCols) {
+            const int i = col0 + lane;
+            const float old = sh.m[i];
+            const float m = fmaxf(fmaxf(fmaxf(sh.top[0][i], sh.top[1][i]), fmaxf(sh.top[2][i], sh.top[3][i])), old);
+            sh.m[i] = m;
+            sh.factor[i] = m > old ? exp2_fast((old - m) * c) : 1.0f;
+            sh.base[i] = m == -INFINITY ? INFINITY : kLift - m * c;
+          }
+          group_sync(bar);
+#pragma unroll
+          for (int i = 0; i < kCols; i += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(&sh.factor[col0 + i]);
+            l[i] *= f.x;
+            l[i + 1] *= f.y;
+            l[i + 2] *= f.z;
+            l[i + 3] *= f.w;
+          }
+          // The products of the tiles before are complete: this tile's scores
+          // were committed after them.
+          if (t > walk.begin) {
+#pragma unroll 1
+            for (int k = 0; k < tile_pairs; ++k) {
+              uint32_t o[kCols];
+              load_columns<kCols>(tmem + lanes + k * kN + col0, o);
+              tc_wait_ld();
+              tc_settle<kCols>(o);
+#pragma unroll
+              for (int i = 0; i < kCols; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * sh.factor[col0 + i]);
+              store_columns<kCols>(tmem + lanes + k * kN + col0, o);
+            }
+            tc_wait_st();
+          }
+        }
+        uint8_t* line = smem + lay.p + token_row * 128;
+#pragma unroll
+        for (int i = 0; i < kCols; i += 8) {
+          uint32_t p[4];
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const float4 base = *reinterpret_cast<const float4*>(&sh.base[col0 + i + e]);
+            // a row without a maximum has only hidden tokens: -inf + inf would be NaN
+            const float p0 = exp2_fast(fmaf(__uint_as_float(s[i + e]), c, base.x == INFINITY ? 0.0f : base.x));
+            const float p1 = exp2_fast(fmaf(__uint_as_float(s[i + e + 1]), c, base.y == INFINITY ? 0.0f : base.y));
+            const float p2 = exp2_fast(fmaf(__uint_as_float(s[i + e + 2]), c, base.z == INFINITY ? 0.0f : base.z));
+            const float p3 = exp2_fast(fmaf(__uint_as_float(s[i + e + 3]), c, base.w == INFINITY ? 0.0f : base.w));
+            l[i + e] += p0;
+            l[i + e + 1] += p1;
+            l[i + e + 2] += p2;
+            l[i + e + 3] += p3;
+            p[e / 2] = pack<kAct>(p0, p1);
+            p[e / 2 + 1] = pack<kAct>(p2, p3);
+          }
+          const int chunk = (half * kCols + i) / 8;
+          *reinterpret_cast<uint4*>(line + ((chunk ^ (token_row & 7)) * 16)) = make_uint4(p[0], p[1], p[2], p[3]);
+        }
+        fence_async_smem();
+        tc_fence_before();
+        mbar_arrive(&sh.p_ready);
+      }
+      // The segment's sums over the tokens, then its output.
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) {
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+        if (lane == i) sh.top[quad][col0 + i] = l[i];
+      }
+      group_sync(bar);
+      const bool whole = walk.begin == 0 && walk.end == walk.tiles;
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (segment > 0);
+      if (quad == 0 && lane < kCols) {
+        const int i = col0 + lane, row = walk.srt * kN + i;
+        const float sum = (sh.top[0][i] + sh.top[1][i]) + (sh.top[2][i] + sh.top[3][i]);
+        const float unit = sh.m[i] * c - kLift;
+        if (!whole) sums[slot * kN + i] = make_float2(unit, ok ? sum : NAN);
+        else if (a.lse && row < rows)
+          a.lse[walk.sb * rows + row] = sum == 0.0f ? -INFINITY : (unit + log2f(sum)) * 0.6931471805599453f;
+        sh.factor[i] = sum == 0.0f ? 0.0f : 1.0f / sum;
+      }
+      group_sync(bar);
+      if (ok) ok = mbar_wait(&sh.o_done, segment & 1);
+      tc_fence_after();
+      for (int k = 0; k < tile_pairs; ++k) {
+        uint32_t o[kCols];
+        load_columns<kCols>(tmem + lanes + k * kN + col0, o);
+        tc_wait_ld();
+        tc_settle<kCols>(o);
+        const int channel = 128 * k + token_row;
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) {
+          const float v = ok ? __uint_as_float(o[i]) : NAN;
+          const int row = walk.srt * kN + col0 + i;
+          if (!whole) parts[(slot * kN + col0 + i) * a.rank + channel] = v;
+          else if (row < rows) store_act(a.out, kAct, (walk.sb * rows + row) * a.rank + channel, v * sh.factor[col0 + i]);
+        }
+      }
+      group_sync(bar);  // the shared rows are free for the next segment
+    }
   }
-  if (a.lse && threadIdx.x == 0) a.lse[row] = sum > 0.0f ? top + logf(sum) : -INFINITY;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_free(tmem, columns);
+}
+
+// ---- joining the parts ---------------------------------------------------------------
+
+constexpr int kJoinGroups = 8;  // threads that share a channel's parts
+
+// One CTA per (sequence, row tile, row): nothing to do where one CTA of the
+// main kernel had the whole sequence.
+template <int kAct>
+__global__ void __launch_bounds__(128 * kJoinGroups)
+    latent_join_kernel(const LatentAttentionArgs a, const Work w, int kn, int ctas, const float* __restrict__ parts,
+                       const float2* __restrict__ sums) {
+  __shared__ int64_t s_first, s_last, s_total, s_sharers, s_start;
+  __shared__ float s_top, s_sum;
+  __shared__ float4 s_o[kJoinGroups][128];
+  const int rows = w.queries * w.heads;
+  const int64_t b = blockIdx.x / (static_cast<int64_t>(w.row_tiles) * kn);
+  const int rt = static_cast<int>(blockIdx.x / kn % w.row_tiles), i = blockIdx.x % kn;
+  const int row = rt * kn + i, lane = threadIdx.x & 31;
+  const int thread = threadIdx.x & 127, group = threadIdx.x >> 7;
+  if (threadIdx.x < 32) {
+    const int64_t total = total_tiles(w, lane);
+    int64_t before = 0;
+    for (int64_t j = lane; j < b; j += 32) before += tiles_of(w, j);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
+    const int tiles = tiles_of(w, b);
+    const int64_t n = sharers(total, ctas), start = before * w.row_tiles + static_cast<int64_t>(rt) * tiles;
+    if (lane == 0) {
+      s_total = total;
+      s_sharers = n;
+      s_start = start;
+      // the CTA of tile x is the last whose first tile is not behind x
+      s_first = tiles ? ((start + 1) * n - 1) / total : 0;
+      s_last = tiles ? ((start + tiles) * n - 1) / total : -1;
+    }
+  }
+  __syncthreads();
+  pdl_wait();
+  const int64_t first = s_first, last = s_last, at = b * rows + row;
+  if (row >= rows) return;
+  if (last < first) {  // no tokens
+    for (int j = threadIdx.x; j < a.rank; j += 128 * kJoinGroups) store_act(a.out, kAct, at * a.rank + j, 0.0f);
+    if (a.lse && threadIdx.x == 0) a.lse[at] = -INFINITY;
+    return;
+  }
+  if (first == last) return;
+  auto slot_of = [&](int64_t cta) { return 2 * cta + (first_tile(cta, s_total, s_sharers) < s_start ? 1 : 0); };
+  if (threadIdx.x < 32) {
+    float top = -INFINITY;
+    for (int64_t k = first + lane; k <= last; k += 32) {
+      const float2 v = sums[slot_of(k) * kn + i];
+      if (v.y != 0.0f) top = fmaxf(top, v.x);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    float sum = 0.0f;
+    for (int64_t k = first + lane; k <= last; k += 32) {
+      const float2 v = sums[slot_of(k) * kn + i];
+      if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) {
+      s_top = top;
+      s_sum = sum;
+      if (a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    }
+  }
+  __syncthreads();
+  const float top = s_top, sum = s_sum;
+  if (4 * thread < a.rank) {
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int64_t k = first + group; k <= last; k += kJoinGroups) {
+      const int64_t slot = slot_of(k) * kn + i;
+      const float2 v = sums[slot];
+      const float4 part = *reinterpret_cast<const float4*>(parts + slot * a.rank + 4 * thread);
+      const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
+      o.x = fmaf(part.x, f, o.x);
+      o.y = fmaf(part.y, f, o.y);
+      o.z = fmaf(part.z, f, o.z);
+      o.w = fmaf(part.w, f, o.w);
+    }
+    s_o[group][thread] = o;
+  }
+  __syncthreads();
+  if (group == 0 && 4 * thread < a.rank) {
+    float4 o = s_o[0][thread];
+#pragma unroll
+    for (int g = 1; g < kJoinGroups; ++g) {
+      const float4 v = s_o[g][thread];
+      o.x += v.x;
+      o.y += v.y;
+      o.z += v.z;
+      o.w += v.w;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int64_t to = at * a.rank + 4 * thread;
+    store_act(a.out, kAct, to, o.x * inv);
+    store_act(a.out, kAct, to + 1, o.y * inv);
+    store_act(a.out, kAct, to + 2, o.z * inv);
+    store_act(a.out, kAct, to + 3, o.w * inv);
+  }
+}
+
+int rows_per_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+Layout layout(int rank, int kn) {
+  const uint32_t room = kSmem - 1024, q = (rank / 64 + 1) * kn * 128;
+  const int tile_pairs = rank / 128;
+  Layout l{};
+  l.q = 0;
+  l.p = q;  // a multiple of 1 KB: kn * 128 is one of 2 KB
+  l.rope = l.p + kBlock;
+  // Rotary buffers of their own where the ring still holds a pair more than a
+  // tile; without them the rotary block waits for P's buffer.
+  for (l.ropes = 2; l.ropes >= 0; --l.ropes) {
+    l.ring = l.rope + l.ropes * kBlock;
+    l.pairs = static_cast<int>((room - l.ring) / kPair);
+    if (l.pairs > kMaxPairs) l.pairs = kMaxPairs;
+    if (l.pairs > tile_pairs || l.ropes == 0) break;
+  }
+  return l;
+}
+
+template <int kAct, int kN>
+cudaError_t launch(const LatentAttentionArgs& a, cudaStream_t s) {
+  const CUtensorMapDataType type =
+      kAct == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const int rows = a.queries * a.heads, row_tiles = (rows + kN - 1) / kN, ctas = sm_count();
+  const Work w{a.batch, a.queries, a.heads, row_tiles, static_cast<int64_t>(a.table_width) * a.page_size, a.lengths};
+  float* parts = static_cast<float*>(a.workspace);
+  float2* sums = reinterpret_cast<float2*>(parts + 2ll * ctas * kN * a.rank);
+  cudaError_t err;
+  if (a.pages > 0 && a.table_width > 0) {
+    // The largest power of two (16 to 128) that divides a page: no box crosses one.
+    int box = 16;
+    while (box < kTile && a.page_size % (2 * box) == 0) box *= 2;
+    Maps maps;
+    const uint64_t n = static_cast<uint64_t>(rows), b = static_cast<uint64_t>(a.batch),
+                   d = static_cast<uint64_t>(a.rank);
+    if (!encode_tiled_3d(&maps.q, type, a.q_latent, {d, n, b}, {d * 2, d * n * 2}, {64, kN, 1},
+                         CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_tiled_3d(&maps.r, type, a.q_rope, {64, n, b}, {128, 128 * n}, {64, kN, 1}, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !encode_tiled_2d(&maps.cache, type, a.cache, d + kLatentRope, static_cast<uint64_t>(a.pages) * a.page_size,
+                         2 * (d + kLatentRope), 64, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return cudaErrorInvalidValue;
+    uint32_t columns = 32;
+    while (columns < static_cast<uint32_t>(kN * (a.rank / 128 + 1))) columns *= 2;
+    auto kernel = latent_attention_kernel<kAct, kN>;
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (err != cudaSuccess) return err;
+    kernel<<<ctas, kThreads, kSmem, s>>>(maps, a, w, layout(a.rank, kN), box, columns, parts, sums);
+    err = cudaGetLastError();
+    if (err != cudaSuccess) return err;
+  }
+  const dim3 grid(static_cast<unsigned>(a.batch * row_tiles * kN)), block(128 * kJoinGroups);
+  if (a.pages > 0 && a.table_width > 0)
+    return launch_pdl(latent_join_kernel<kAct>, grid, block, 0, s, a, w, kN, ctas, static_cast<const float*>(parts),
+                      static_cast<const float2*>(sums));
+  // No page exists, so every sequence is empty: nothing ran before that the
+  // early launch could follow.
+  Work none = w;
+  none.room = 0;
+  latent_join_kernel<kAct><<<grid, block, 0, s>>>(a, none, kN, ctas, parts, sums);
+  return cudaGetLastError();
+}
+
+template <int kAct>
+cudaError_t launch_rows(const LatentAttentionArgs& a, cudaStream_t s) {
+  switch (rows_per_tile(a.queries * a.heads)) {
+    case 16: return launch<kAct, 16>(a, s);
+    case 32: return launch<kAct, 32>(a, s);
+    default: return launch<kAct, 64>(a, s);
+  }
 }
 
 }  // namespace
 
-size_t latent_attention_workspace(int64_t, int, int, int) { return 0; }
+size_t latent_attention_workspace(int64_t, int queries, int heads, int rank) {
+  const size_t kn = rows_per_tile(queries * heads);
+  return 2ull * sm_count() * kn * (rank * sizeof(float) + sizeof(float2));
+}
 
 cudaError_t launch_latent_attention(const LatentAttentionArgs& a, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>(a.batch * a.queries * a.heads);
-  if (grid == 0) return cudaSuccess;
-  if (a.dtype == kF16) latent_attention_kernel<kF16><<<grid, 32 * kWarps, 0, s>>>(a);
-  else latent_attention_kernel<kBF16><<<grid, 32 * kWarps, 0, s>>>(a);
-  return cudaGetLastError();
+  if (a.batch == 0) return cudaSuccess;
+  return a.dtype == kF16 ? launch_rows<kF16>(a, s) : launch_rows<kBF16>(a, s);
 }
 
 }  // namespace exlr8

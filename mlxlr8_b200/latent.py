@@ -137,12 +137,12 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
         raise ValueError("out must be a contiguous tensor like q_latent")
     lse = torch.empty((batch, queries, heads), dtype=torch.float32, device=device) if return_lse else None
     lib = _lib.lib()
-    need = lib.exlr8_latent_attention_workspace(batch, queries, heads, rank)
-    if need >= 1 << 62:
-        raise ValueError("operand sizes or strides are outside what the operator takes")
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = _lib.workspace(need, device)
     with _lib.on_device(device):
+        need = lib.exlr8_latent_attention_workspace(batch, queries, heads, rank)
+        if need >= 1 << 62:
+            raise ValueError("operand sizes or strides are outside what the operator takes")
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = _lib.workspace(need, device)
         _lib.check(lib.exlr8_latent_attention(
             q_latent.data_ptr(), q_rope.data_ptr(), batch, queries, heads, rank, _lib.act_code(cache), cache.data_ptr(),
             cache.shape[0], cache.shape[1], block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
