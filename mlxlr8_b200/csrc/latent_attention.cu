@@ -112,34 +112,34 @@ __device__ __forceinline__ int64_t first_tile(int64_t i, int64_t total, int64_t 
 
 // A CTA's walk over its share: one segment per (sequence, row tile).
 struct Walk {
-  int64_t b, left;  // sequence, tiles of the share not yet taken
-  int rt, tile;     // row tile, first tile of the next segment
-  // the segment
-  int64_t sb;
-  int srt, begin, end, tokens, tiles;
+  int64_t b, left;    // sequence, tiles of the share not yet taken
+  int rt, tile;       // row tile, first tile of the next segment
+  int tokens, tiles;  // of the sequence
+  int begin, end;     // the segment's tiles
   __device__ __forceinline__ bool next(const Work& w) {
     if (left <= 0) return false;
-    tokens = tokens_of(w, b);
-    tiles = (tokens + kTile - 1) / kTile;
     while (tile >= tiles) {  // on to the next row tile, then the next sequence that has tokens
       tile = 0;
-      if (++rt >= w.row_tiles) {
+      if (tiles == 0 || ++rt >= w.row_tiles) {
         rt = 0;
         if (++b >= w.batch) return false;
         tokens = tokens_of(w, b);
         tiles = (tokens + kTile - 1) / kTile;
-      } else if (tiles == 0) {
-        rt = w.row_tiles - 1;
       }
     }
-    sb = b;
-    srt = rt;
     begin = tile;
     end = static_cast<int>(min(static_cast<int64_t>(tiles), begin + left));
     left -= end - begin;
     tile = end;
     return true;
   }
+};
+
+// What a CTA leaves for the join: the (sequence, row tile) of its first tile,
+// where that begins, and the cut of the list.
+struct Cut {
+  int64_t start, total, sharers, sequence;
+  int rt, tiles;
 };
 
 // ---- the main kernel -------------------------------------------------------------
@@ -159,6 +159,20 @@ struct Shared {
   float m[64];
   float top[4][64];
   int limit[64];
+};
+
+// A place in the ring and the parity of its round.  (Slots are counted, not
+// divided: a division per pair made the issuing warp the bound.)
+struct Place {
+  int slot = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void advance(int by, int slots) {
+    slot += by;
+    if (slot >= slots) {
+      slot -= slots;
+      round ^= 1;
+    }
+  }
 };
 
 struct Maps {
@@ -214,12 +228,13 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&v
 template <int kAct, int kN>
 __global__ void __launch_bounds__(kThreads, 1)
     latent_attention_kernel(const __grid_constant__ Maps maps, const LatentAttentionArgs a, const Work w, const Layout lay,
-                            int box, uint32_t columns, float* __restrict__ parts, float2* __restrict__ sums) {
+                            int box, uint32_t columns, float* __restrict__ parts, float2* __restrict__ sums,
+                            Cut* __restrict__ cuts) {
   pdl_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int blocks = a.rank / 64, tile_pairs = a.rank / 128;
   if (warp == 0) {
     const int64_t total = total_tiles(w, lane);
@@ -229,78 +244,91 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t at = first_tile(blockIdx.x, total, n);
       int64_t sequence, before;
       find_sequence(w, at, lane, &sequence, &before);
-      const int tiles = tiles_of(w, sequence);
       walk.b = sequence;
       walk.left = first_tile(blockIdx.x + 1, total, n) - at;
-      walk.rt = static_cast<int>((at - before) / tiles);
-      walk.tile = static_cast<int>((at - before) % tiles);
+      walk.tokens = tokens_of(w, sequence);
+      walk.tiles = (walk.tokens + kTile - 1) / kTile;
+      walk.rt = static_cast<int>((at - before) / walk.tiles);
+      walk.tile = static_cast<int>((at - before) % walk.tiles);
+      if (lane == 0) cuts[blockIdx.x] = Cut{at - walk.tile, total, n, sequence, walk.rt, walk.tiles};
+    } else if (lane == 0) {
+      cuts[blockIdx.x] = Cut{};
     }
-    if (lane == 0) {
-      sh.walk = walk;
-      mbar_init(&sh.q_full, 1);
-      mbar_init(&sh.q_empty, 1);
-      mbar_init(&sh.s_full, 1);
-      mbar_init(&sh.p_ready, 256);
-      mbar_init(&sh.o_done, 1);
-      for (int i = 0; i < kMaxPairs; ++i) {
-        mbar_init(&sh.full[i], 1);
-        mbar_init(&sh.empty[i], 1);
-      }
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&sh.rope_full[i], 1);
-        mbar_init(&sh.rope_empty[i], 1);
-      }
-      mbar_fence_init();
+    if (lane == 0) sh.walk = walk;
+  } else if (warp == 1) {
+    tmem_alloc(&sh.tmem, columns);
+  } else if (warp == 2 && lane == 0) {
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.s_full, 1);
+    mbar_init(&sh.p_ready, 256);
+    mbar_init(&sh.o_done, 1);
+    for (int i = 0; i < kMaxPairs; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.rope_full[i], 1);
+      mbar_init(&sh.rope_empty[i], 1);
+    }
+    mbar_fence_init();
+  } else if (warp > 2) {
+    // Sequences without tokens are no CTA's work: their rows are zeroed here.
+    const int64_t rows = static_cast<int64_t>(a.queries) * a.heads;
+    for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
+      if (tokens_of(w, b) > 0) continue;
+      for (int64_t i = threadIdx.x - 96; i < rows * a.rank / 8; i += kThreads - 96)
+        reinterpret_cast<uint4*>(a.out)[b * (rows * a.rank / 8) + i] = make_uint4(0, 0, 0, 0);
+      if (a.lse)
+        for (int64_t i = threadIdx.x - 96; i < rows; i += kThreads - 96) a.lse[b * rows + i] = -INFINITY;
     }
   }
-  __syncthreads();
-  Walk walk = sh.walk;
-  if (walk.left <= 0) return;
-  if (warp == 1) tmem_alloc(&sh.tmem, columns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  Walk walk = sh.walk;
   const uint32_t tmem = sh.tmem, t_scores = tmem + tile_pairs * kN;
   const int ropes = lay.ropes > 0 ? lay.ropes : 1;
   const uint32_t rope_at = lay.ropes > 0 ? lay.rope : lay.p;
   bool ok = true;
 
   if (warp == 0) {
-    int u = 0, pair = 0;  // tiles and pairs loaded so far
-    int segment = 0;
+    int u = 0, segment = 0, loaded = 0;  // tiles, segments and pairs so far
+    Place place;
     for (; ok && walk.next(w); ++segment) {
       if (segment > 0) ok = mbar_wait(&sh.q_empty, (segment - 1) & 1);
       if (!ok) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(&sh.q_full, (blocks + 1) * kN * 128);
         for (int i = 0; i < blocks; ++i)
-          tma_load_3d(smem + lay.q + i * kN * 128, &maps.q, 64 * i, walk.srt * kN, static_cast<int>(walk.sb), &sh.q_full);
-        tma_load_3d(smem + lay.q + blocks * kN * 128, &maps.r, 0, walk.srt * kN, static_cast<int>(walk.sb), &sh.q_full);
+          tma_load_3d(smem + lay.q + i * kN * 128, &maps.q, 64 * i, walk.rt * kN, static_cast<int>(walk.b), &sh.q_full);
+        tma_load_3d(smem + lay.q + blocks * kN * 128, &maps.r, 0, walk.rt * kN, static_cast<int>(walk.b), &sh.q_full);
       }
       for (int t = walk.begin; ok && t < walk.end; ++t, ++u) {
         // Lane i fetches the tokens [i * box, (i + 1) * box) of the tile.
         const int token = t * kTile + lane * box;
         int row = -1;
         if (lane * box < kTile && token < walk.tokens) {
-          const int page = a.block_table[walk.sb * a.table_width + token / a.page_size];
+          const int page = a.block_table[walk.b * a.table_width + token / a.page_size];
           if (page >= 0 && page < a.pages) row = page * a.page_size + token % a.page_size;
         }
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row >= 0)) * box * 128;
-        for (int i = 0; ok && i < tile_pairs; ++i, ++pair) {
-          const int slot = pair % lay.pairs;
-          if (pair >= lay.pairs) ok = mbar_wait(&sh.empty[slot], (pair / lay.pairs - 1) & 1);
+        for (int i = 0; ok && i < tile_pairs; ++i, ++loaded) {
+          uint64_t* full = &sh.full[place.slot];
+          ok = mbar_wait(&sh.empty[place.slot], place.round ^ 1);  // (passes in the first round)
           if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], 2 * bytes);
+          if (lane == 0) mbar_arrive_expect_tx(full, 2 * bytes);
           __syncwarp();
           if (row >= 0) {
-            uint8_t* dst = smem + lay.ring + slot * kPair + lane * box * 128;
-            tma_load_2d(dst, &maps.cache, 128 * i, row, &sh.full[slot]);
-            tma_load_2d(dst + kBlock, &maps.cache, 128 * i + 64, row, &sh.full[slot]);
+            uint8_t* dst = smem + lay.ring + place.slot * kPair + lane * box * 128;
+            tma_load_2d(dst, &maps.cache, 128 * i, row, full);
+            tma_load_2d(dst + kBlock, &maps.cache, 128 * i + 64, row, full);
           }
+          place.advance(1, lay.pairs);
         }
         if (!ok) break;
-        const int r = u % ropes;
-        if (u >= ropes) ok = mbar_wait(&sh.rope_empty[r], (u / ropes - 1) & 1);
+        const int r = u & (ropes - 1);
+        ok = mbar_wait(&sh.rope_empty[r], ((u >> (ropes - 1)) & 1) ^ 1);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sh.rope_full[r], bytes);
         __syncwarp();
@@ -309,53 +337,72 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // Copies still in flight land before the CTA's memory is given back.
     if (segment > 0) mbar_wait(&sh.q_full, (segment - 1) & 1);
-    for (int i = max(0, pair - lay.pairs); i < pair; ++i) mbar_wait(&sh.full[i % lay.pairs], (i / lay.pairs) & 1);
-    for (int i = max(0, u - ropes); i < u; ++i) mbar_wait(&sh.rope_full[i % ropes], (i / ropes) & 1);
+    for (int i = max(0, loaded - lay.pairs); i < loaded; ++i) mbar_wait(&sh.full[i % lay.pairs], (i / lay.pairs) & 1);
+    for (int i = max(0, u - ropes); i < u; ++i) mbar_wait(&sh.rope_full[i & (ropes - 1)], (i >> (ropes - 1)) & 1);
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t score_desc = half_idesc(kAct == kBF16, kN, a.scale < 0.0f, false, false);
-      const uint32_t value_desc = half_idesc(kAct == kBF16, kN, false, true, true);
-      const uint32_t sq = smem_u32(smem + lay.q), sp = smem_u32(smem + lay.p), ring = smem_u32(smem + lay.ring),
-                     sr = smem_u32(smem + rope_at);
-      int u = 0, pair = 0;
-      for (int segment = 0; ok && walk.next(w); ++segment) {
-        ok = mbar_wait(&sh.q_full, segment & 1);
-        for (int t = walk.begin; ok && t < walk.end; ++t, ++u, pair += tile_pairs) {
-          for (int i = 0; ok && i < tile_pairs; ++i) {
-            const int slot = (pair + i) % lay.pairs;
-            ok = mbar_wait(&sh.full[slot], ((pair + i) / lay.pairs) & 1);
-            if (!ok) break;
-            tc_fence_after();
+    const uint32_t score_desc = half_idesc(kAct == kBF16, kN, a.scale < 0.0f, false, false);
+    const uint32_t value_desc = half_idesc(kAct == kBF16, kN, false, true, true);
+    const uint32_t td = uniform(tmem), ts = td + tile_pairs * kN;
+    const uint32_t sq = uniform(desc_lo_sw128(smem_u32(smem + lay.q))),
+                   sp = uniform(desc_lo_rows128(smem_u32(smem + lay.p), kBlock)),
+                   sc = uniform(desc_lo_sw128(smem_u32(smem + lay.ring))),
+                   sv = uniform(desc_lo_rows128(smem_u32(smem + lay.ring), kBlock)),
+                   sr = uniform(desc_lo_sw128(smem_u32(smem + rope_at)));
+    int u = 0;
+    Place first;  // of the tile
+    for (int segment = 0; ok && uniform(walk.next(w)); ++segment) {
+      const int begin = uniform(walk.begin), end = uniform(walk.end);
+      ok = warp_wait(&sh.q_full, segment & 1);
+      for (int t = begin; ok && t < end; ++t, ++u, first.advance(tile_pairs, lay.pairs)) {
+        Place place = first;
+        for (int i = 0; ok && i < tile_pairs; ++i, place.advance(1, lay.pairs)) {
+          ok = warp_wait(&sh.full[place.slot], place.round);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t ct = uniform(sc + place.slot * (kPair >> 4)), qt = uniform(sq + i * (2 * kN * 128 >> 4));
+          if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              tc_mma_f16(t_scores, umma_desc_sw128(ring + slot * kPair + (k / 4) * kBlock + (k % 4) * 32),
-                         umma_desc_sw128(sq + (2 * i + k / 4) * kN * 128 + (k % 4) * 32), score_desc, (i | k) != 0);
+              tc_mma_f16(ts, desc_of(ct + (((k / 4) * kBlock + (k % 4) * 32) >> 4)),
+                         desc_of(qt + (((k / 4) * kN * 128 + (k % 4) * 32) >> 4)), score_desc, k > 0 || i > 0);
           }
-          const int r = u % ropes;
-          if (ok) ok = mbar_wait(&sh.rope_full[r], (u / ropes) & 1);
-          if (!ok) break;
-          tc_fence_after();
+          __syncwarp();
+        }
+        const int r = u & (ropes - 1);
+        if (ok) ok = warp_wait(&sh.rope_full[r], (u >> (ropes - 1)) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t rt = uniform(sr + r * (kBlock >> 4)), qr = uniform(sq + blocks * (kN * 128 >> 4));
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tc_mma_f16(t_scores, umma_desc_sw128(sr + r * kBlock + k * 32),
-                       umma_desc_sw128(sq + blocks * kN * 128 + k * 32), score_desc, 1);
+            tc_mma_f16(ts, desc_of(rt + (k * 32 >> 4)), desc_of(qr + (k * 32 >> 4)), score_desc, 1);
           tc_commit(&sh.s_full);
           if (lay.ropes > 0) tc_commit(&sh.rope_empty[r]);
-          if (t + 1 == walk.end) tc_commit(&sh.q_empty);
-          ok = mbar_wait(&sh.p_ready, u & 1);
-          if (!ok) break;
-          tc_fence_after();
-          for (int i = 0; i < tile_pairs; ++i) {
-            const int slot = (pair + i) % lay.pairs;
+          if (t + 1 == end) tc_commit(&sh.q_empty);
+        }
+        __syncwarp();
+        ok = warp_wait(&sh.p_ready, u & 1);
+        if (!ok) break;
+        tc_fence_after();
+        place = first;
+        for (int i = 0; i < tile_pairs; ++i, place.advance(1, lay.pairs)) {
+          const uint32_t ct = uniform(sv + place.slot * (kPair >> 4)), to = uniform(td + i * kN);
+          const uint32_t more = t > begin;
+          if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              tc_mma_f16(tmem + i * kN, umma_desc_rows128(ring + slot * kPair + k * 2048, kBlock),
-                         umma_desc_rows128(sp + k * 2048, kBlock), value_desc, t > walk.begin || k > 0);
-            tc_commit(&sh.empty[slot]);
+              tc_mma_f16(to, desc_of(ct + (k * 2048 >> 4)), desc_of(sp + (k * 2048 >> 4)), value_desc,
+                         k > 0 ? 1 : more);
+            tc_commit(&sh.empty[place.slot]);
           }
-          if (lay.ropes == 0) tc_commit(&sh.rope_empty[r]);
-          if (t + 1 == walk.end) tc_commit(&sh.o_done);
+          __syncwarp();
         }
+        if (elect_one()) {
+          if (lay.ropes == 0) tc_commit(&sh.rope_empty[r]);
+          if (t + 1 == end) tc_commit(&sh.o_done);
+        }
+        __syncwarp();
       }
     }
   } else {
@@ -365,25 +412,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
     const float c = fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f;
     const int rows = a.queries * a.heads;
-    int u = 0, pair = 0;
+    int u = 0;
+    Place first;
     for (int segment = 0; walk.next(w); ++segment) {
       // One warp of each half keeps its rows' maxima and limits.
       if (quad == 0 && lane < kCols) {
-        const int row = walk.srt * kN + col0 + lane;
+        const int row = walk.rt * kN + col0 + lane;
         sh.base[col0 + lane] = INFINITY;
         sh.m[col0 + lane] = -INFINITY;
         sh.limit[col0 + lane] = row < rows ? walk.tokens - a.queries + 1 + row / a.heads : walk.tokens;
       }
       group_sync(bar);
-      const int least = walk.tokens - a.queries + 1 + walk.srt * kN / a.heads;
+      const int least = walk.tokens - a.queries + 1 + walk.rt * kN / a.heads;
       float l[kCols];
 #pragma unroll
       for (int i = 0; i < kCols; ++i) l[i] = 0.0f;
-      for (int t = walk.begin; t < walk.end; ++t, ++u, pair += tile_pairs) {
+      for (int t = walk.begin; t < walk.end; ++t, ++u, first.advance(tile_pairs, lay.pairs)) {
         const int token = t * kTile + token_row;
         bool held = token < walk.tokens;
         if (held) {
-          const int page = a.block_table[walk.sb * a.table_width + token / a.page_size];
+          const int page = a.block_table[walk.b * a.table_width + token / a.page_size];
           held = page >= 0 && page < a.pages;
         }
         if (ok) ok = mbar_wait(&sh.s_full, u & 1);
@@ -394,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_settle<kCols>(s);
         if (!held && ok) {
           for (int i = half * blocks / 2; i < (half + 1) * blocks / 2; ++i) {
-            uint4* line = reinterpret_cast<uint4*>(smem + lay.ring + (pair + i / 2) % lay.pairs * kPair +
+            uint4* line = reinterpret_cast<uint4*>(smem + lay.ring + (first.slot + i / 2) % lay.pairs * kPair +
                                                    (i & 1) * kBlock + token_row * 128);
 #pragma unroll
             for (int e = 0; e < 8; ++e) line[e] = make_uint4(0, 0, 0, 0);
@@ -491,12 +539,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool whole = walk.begin == 0 && walk.end == walk.tiles;
       const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (segment > 0);
       if (quad == 0 && lane < kCols) {
-        const int i = col0 + lane, row = walk.srt * kN + i;
+        const int i = col0 + lane, row = walk.rt * kN + i;
         const float sum = (sh.top[0][i] + sh.top[1][i]) + (sh.top[2][i] + sh.top[3][i]);
         const float unit = sh.m[i] * c - kLift;
         if (!whole) sums[slot * kN + i] = make_float2(unit, ok ? sum : NAN);
         else if (a.lse && row < rows)
-          a.lse[walk.sb * rows + row] = sum == 0.0f ? -INFINITY : (unit + log2f(sum)) * 0.6931471805599453f;
+          a.lse[walk.b * rows + row] = sum == 0.0f ? -INFINITY : (unit + log2f(sum)) * 0.6931471805599453f;
         sh.factor[i] = sum == 0.0f ? 0.0f : 1.0f / sum;
       }
       group_sync(bar);
@@ -507,13 +555,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         load_columns<kCols>(tmem + lanes + k * kN + col0, o);
         tc_wait_ld();
         tc_settle<kCols>(o);
-        const int channel = 128 * k + token_row;
+        if (!ok) {
 #pragma unroll
-        for (int i = 0; i < kCols; ++i) {
-          const float v = ok ? __uint_as_float(o[i]) : NAN;
-          const int row = walk.srt * kN + col0 + i;
-          if (!whole) parts[(slot * kN + col0 + i) * a.rank + channel] = v;
-          else if (row < rows) store_act(a.out, kAct, (walk.sb * rows + row) * a.rank + channel, v * sh.factor[col0 + i]);
+          for (int i = 0; i < kCols; ++i) o[i] = 0x7fc00000u;
+        }
+        const int channel = 128 * k + token_row;
+        if (!whole) {
+          float* dst = parts + (slot * kN + col0) * a.rank + channel;
+#pragma unroll
+          for (int i = 0; i < kCols; ++i, dst += a.rank) *dst = __uint_as_float(o[i]);
+        } else {
+          const int row = walk.rt * kN + col0;
+          const int64_t first = (walk.b * rows + row) * a.rank + channel;
+#pragma unroll
+          for (int i = 0; i < kCols; ++i)
+            if (row + i < rows)
+              store_act(a.out, kAct, first + static_cast<int64_t>(i) * a.rank, __uint_as_float(o[i]) * sh.factor[col0 + i]);
         }
       }
       group_sync(bar);  // the shared rows are free for the next segment
@@ -527,105 +584,86 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ---- joining the parts ---------------------------------------------------------------
 
-constexpr int kJoinGroups = 8;  // threads that share a channel's parts
+constexpr int kJoinGroups = 4;   // rows a CTA takes; threads that share a channel of many parts
+constexpr int kJoinThreads = 128 * kJoinGroups;
+constexpr int kJoinMany = 8;     // parts from which the groups share a row
 
-// One CTA per (sequence, row tile, row): nothing to do where one CTA of the
-// main kernel had the whole sequence.
+// A sequence is cut where a CTA's share begins inside it; the first such CTA's
+// index, blockIdx.x + 1, joins its parts, four rows a CTA.
 template <int kAct>
-__global__ void __launch_bounds__(128 * kJoinGroups)
-    latent_join_kernel(const LatentAttentionArgs a, const Work w, int kn, int ctas, const float* __restrict__ parts,
-                       const float2* __restrict__ sums) {
-  __shared__ int64_t s_first, s_last, s_total, s_sharers, s_start;
-  __shared__ float s_top, s_sum;
+__global__ void __launch_bounds__(kJoinThreads)
+    latent_join_kernel(const LatentAttentionArgs a, const Work w, int kn, const float* __restrict__ parts,
+                       const float2* __restrict__ sums, const Cut* __restrict__ cuts) {
   __shared__ float4 s_o[kJoinGroups][128];
-  const int rows = w.queries * w.heads;
-  const int64_t b = blockIdx.x / (static_cast<int64_t>(w.row_tiles) * kn);
-  const int rt = static_cast<int>(blockIdx.x / kn % w.row_tiles), i = blockIdx.x % kn;
-  const int row = rt * kn + i, lane = threadIdx.x & 31;
-  const int thread = threadIdx.x & 127, group = threadIdx.x >> 7;
-  if (threadIdx.x < 32) {
-    const int64_t total = total_tiles(w, lane);
-    int64_t before = 0;
-    for (int64_t j = lane; j < b; j += 32) before += tiles_of(w, j);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
-    const int tiles = tiles_of(w, b);
-    const int64_t n = sharers(total, ctas), start = before * w.row_tiles + static_cast<int64_t>(rt) * tiles;
-    if (lane == 0) {
-      s_total = total;
-      s_sharers = n;
-      s_start = start;
-      // the CTA of tile x is the last whose first tile is not behind x
-      s_first = tiles ? ((start + 1) * n - 1) / total : 0;
-      s_last = tiles ? ((start + tiles) * n - 1) / total : -1;
-    }
-  }
-  __syncthreads();
   pdl_wait();
-  const int64_t first = s_first, last = s_last, at = b * rows + row;
-  if (row >= rows) return;
-  if (last < first) {  // no tokens
-    for (int j = threadIdx.x; j < a.rank; j += 128 * kJoinGroups) store_act(a.out, kAct, at * a.rank + j, 0.0f);
-    if (a.lse && threadIdx.x == 0) a.lse[at] = -INFINITY;
+  const int64_t cta = blockIdx.x + 1;
+  const Cut cut = cuts[cta];
+  if (cta >= cut.sharers) return;
+  if (first_tile(cta, cut.total, cut.sharers) <= cut.start ||
+      first_tile(cta - 1, cut.total, cut.sharers) > cut.start)
     return;
-  }
-  if (first == last) return;
-  auto slot_of = [&](int64_t cta) { return 2 * cta + (first_tile(cta, s_total, s_sharers) < s_start ? 1 : 0); };
-  if (threadIdx.x < 32) {
-    float top = -INFINITY;
-    for (int64_t k = first + lane; k <= last; k += 32) {
+  // The part of CTA k lies in its first slot where the sequence is what its
+  // share begins with, else in its second.
+  const int64_t last = ((cut.start + cut.tiles) * cut.sharers - 1) / cut.total;
+  const int64_t slot0 = 2 * (cta - 1) + (first_tile(cta - 1, cut.total, cut.sharers) < cut.start ? 1 : 0);
+  auto slot_of = [&](int64_t k) { return k == cta - 1 ? slot0 : 2 * k; };
+  const int rows = w.queries * w.heads;
+  const int thread = threadIdx.x & 127, group = threadIdx.x >> 7, lane = threadIdx.x & 31;
+  const int row0 = blockIdx.y * kJoinGroups;
+  const bool many = last - cta + 2 > kJoinMany;
+  for (int pass = 0; pass < (many ? kJoinGroups : 1); ++pass) {
+    const int i = row0 + (many ? pass : group), row = cut.rt * kn + i;
+    // The largest unit and the sum, by every warp for itself.
+    float top = -INFINITY, sum = 0.0f;
+    for (int64_t k = cta - 1 + lane; k <= last; k += 32) {
       const float2 v = sums[slot_of(k) * kn + i];
       if (v.y != 0.0f) top = fmaxf(top, v.x);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    float sum = 0.0f;
-    for (int64_t k = first + lane; k <= last; k += 32) {
+    for (int64_t k = cta - 1 + lane; k <= last; k += 32) {
       const float2 v = sums[slot_of(k) * kn + i];
       if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) {
-      s_top = top;
-      s_sum = sum;
-      if (a.lse) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-    }
-  }
-  __syncthreads();
-  const float top = s_top, sum = s_sum;
-  if (4 * thread < a.rank) {
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (4 * thread < a.rank) {
 #pragma unroll 4
-    for (int64_t k = first + group; k <= last; k += kJoinGroups) {
-      const int64_t slot = slot_of(k) * kn + i;
-      const float2 v = sums[slot];
-      const float4 part = *reinterpret_cast<const float4*>(parts + slot * a.rank + 4 * thread);
-      const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
-      o.x = fmaf(part.x, f, o.x);
-      o.y = fmaf(part.y, f, o.y);
-      o.z = fmaf(part.z, f, o.z);
-      o.w = fmaf(part.w, f, o.w);
+      for (int64_t k = cta - 1 + (many ? group : 0); k <= last; k += many ? kJoinGroups : 1) {
+        const int64_t at = slot_of(k) * kn + i;
+        const float2 v = sums[at];
+        const float4 part = *reinterpret_cast<const float4*>(parts + at * a.rank + 4 * thread);
+        const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
+        o.x = fmaf(part.x, f, o.x);
+        o.y = fmaf(part.y, f, o.y);
+        o.z = fmaf(part.z, f, o.z);
+        o.w = fmaf(part.w, f, o.w);
+      }
     }
-    s_o[group][thread] = o;
-  }
-  __syncthreads();
-  if (group == 0 && 4 * thread < a.rank) {
-    float4 o = s_o[0][thread];
+    if (many) {
+      s_o[group][thread] = o;
+      __syncthreads();
+      if (group == 0) {
 #pragma unroll
-    for (int g = 1; g < kJoinGroups; ++g) {
-      const float4 v = s_o[g][thread];
-      o.x += v.x;
-      o.y += v.y;
-      o.z += v.z;
-      o.w += v.w;
+        for (int g = 1; g < kJoinGroups; ++g) {
+          const float4 v = s_o[g][thread];
+          o.x += v.x;
+          o.y += v.y;
+          o.z += v.z;
+          o.w += v.w;
+        }
+      }
+      __syncthreads();
+      if (group != 0) continue;
     }
+    if (row >= rows) continue;
+    const int64_t at = cut.sequence * rows + row;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t to = at * a.rank + 4 * thread;
-    store_act(a.out, kAct, to, o.x * inv);
-    store_act(a.out, kAct, to + 1, o.y * inv);
-    store_act(a.out, kAct, to + 2, o.z * inv);
-    store_act(a.out, kAct, to + 3, o.w * inv);
+    if (a.lse && thread == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    if (4 * thread < a.rank)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * a.rank + 4 * thread) =
+          make_uint2(pack<kAct>(o.x * inv, o.y * inv), pack<kAct>(o.z * inv, o.w * inv));
   }
 }
 
@@ -660,42 +698,36 @@ cudaError_t launch(const LatentAttentionArgs& a, cudaStream_t s) {
   const CUtensorMapDataType type =
       kAct == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int rows = a.queries * a.heads, row_tiles = (rows + kN - 1) / kN, ctas = sm_count();
-  const Work w{a.batch, a.queries, a.heads, row_tiles, static_cast<int64_t>(a.table_width) * a.page_size, a.lengths};
+  const Work w{a.batch, a.queries, a.heads, row_tiles,
+               a.pages > 0 ? static_cast<int64_t>(a.table_width) * a.page_size : 0, a.lengths};
   float* parts = static_cast<float*>(a.workspace);
   float2* sums = reinterpret_cast<float2*>(parts + 2ll * ctas * kN * a.rank);
-  cudaError_t err;
-  if (a.pages > 0 && a.table_width > 0) {
-    // The largest power of two (16 to 128) that divides a page: no box crosses one.
-    int box = 16;
-    while (box < kTile && a.page_size % (2 * box) == 0) box *= 2;
-    Maps maps;
-    const uint64_t n = static_cast<uint64_t>(rows), b = static_cast<uint64_t>(a.batch),
-                   d = static_cast<uint64_t>(a.rank);
-    if (!encode_tiled_3d(&maps.q, type, a.q_latent, {d, n, b}, {d * 2, d * n * 2}, {64, kN, 1},
-                         CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_tiled_3d(&maps.r, type, a.q_rope, {64, n, b}, {128, 128 * n}, {64, kN, 1}, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !encode_tiled_2d(&maps.cache, type, a.cache, d + kLatentRope, static_cast<uint64_t>(a.pages) * a.page_size,
-                         2 * (d + kLatentRope), 64, box, CU_TENSOR_MAP_SWIZZLE_128B))
-      return cudaErrorInvalidValue;
-    uint32_t columns = 32;
-    while (columns < static_cast<uint32_t>(kN * (a.rank / 128 + 1))) columns *= 2;
-    auto kernel = latent_attention_kernel<kAct, kN>;
-    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (err != cudaSuccess) return err;
-    kernel<<<ctas, kThreads, kSmem, s>>>(maps, a, w, layout(a.rank, kN), box, columns, parts, sums);
-    err = cudaGetLastError();
-    if (err != cudaSuccess) return err;
-  }
-  const dim3 grid(static_cast<unsigned>(a.batch * row_tiles * kN)), block(128 * kJoinGroups);
-  if (a.pages > 0 && a.table_width > 0)
-    return launch_pdl(latent_join_kernel<kAct>, grid, block, 0, s, a, w, kN, ctas, static_cast<const float*>(parts),
-                      static_cast<const float2*>(sums));
-  // No page exists, so every sequence is empty: nothing ran before that the
-  // early launch could follow.
-  Work none = w;
-  none.room = 0;
-  latent_join_kernel<kAct><<<grid, block, 0, s>>>(a, none, kN, ctas, parts, sums);
-  return cudaGetLastError();
+  Cut* cuts = reinterpret_cast<Cut*>(sums + 2ll * ctas * kN);
+  // The largest power of two (16 to 128) that divides a page: no box crosses one.
+  int box = 16;
+  while (box < kTile && a.page_size % (2 * box) == 0) box *= 2;
+  Maps maps;
+  const uint64_t n = static_cast<uint64_t>(rows), b = static_cast<uint64_t>(a.batch), d = static_cast<uint64_t>(a.rank);
+  // Without pages nothing is loaded; the map then describes the queries.
+  const bool empty = w.room == 0;
+  if (!encode_tiled_3d(&maps.q, type, a.q_latent, {d, n, b}, {d * 2, d * n * 2}, {64, kN, 1},
+                       CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_tiled_3d(&maps.r, type, a.q_rope, {64, n, b}, {128, 128 * n}, {64, kN, 1}, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_tiled_2d(&maps.cache, type, empty ? a.q_latent : a.cache, empty ? d : d + kLatentRope,
+                       empty ? n : static_cast<uint64_t>(a.pages) * a.page_size, 2 * (empty ? d : d + kLatentRope), 64,
+                       box, CU_TENSOR_MAP_SWIZZLE_128B))
+    return cudaErrorInvalidValue;
+  uint32_t columns = 32;
+  while (columns < static_cast<uint32_t>(kN * (a.rank / 128 + 1))) columns *= 2;
+  auto kernel = latent_attention_kernel<kAct, kN>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (err != cudaSuccess) return err;
+  kernel<<<ctas, kThreads, kSmem, s>>>(maps, a, w, layout(a.rank, kN), box, columns, parts, sums, cuts);
+  err = cudaGetLastError();
+  if (err != cudaSuccess || ctas < 2) return err;
+  return launch_pdl(latent_join_kernel<kAct>, dim3(ctas - 1, kN / kJoinGroups), dim3(kJoinThreads), 0, s, a, w, kN,
+                    static_cast<const float*>(parts), static_cast<const float2*>(sums),
+                    static_cast<const Cut*>(cuts));
 }
 
 template <int kAct>
@@ -711,7 +743,7 @@ cudaError_t launch_rows(const LatentAttentionArgs& a, cudaStream_t s) {
 
 size_t latent_attention_workspace(int64_t, int queries, int heads, int rank) {
   const size_t kn = rows_per_tile(queries * heads);
-  return 2ull * sm_count() * kn * (rank * sizeof(float) + sizeof(float2));
+  return sm_count() * (2 * kn * (rank * sizeof(float) + sizeof(float2)) + sizeof(Cut));
 }
 
 cudaError_t launch_latent_attention(const LatentAttentionArgs& a, cudaStream_t s) {

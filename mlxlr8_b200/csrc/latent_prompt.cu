@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* const k_ring = smem + 2 * T::kQ;
   uint8_t* const v_ring = k_ring + T::kKStages * T::kK;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int columns = a.heads * value_parts;
   const int head = blockIdx.x % columns / value_parts, part = blockIdx.x % value_parts;
 
@@ -204,31 +204,37 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     const uint32_t score_desc = half_idesc(kAct == kBF16, kKeys, a.scale < 0.0f, false, false);
     const uint32_t value_desc = half_idesc(kAct == kBF16, 64 * vb, false, false, true);
-    const uint32_t sq = smem_u32(smem), sk = smem_u32(k_ring), sv = smem_u32(v_ring);
-    bool ok = all == 0 || mbar_wait(&sh.q_full, 0);
+    const uint32_t td = uniform(tmem), sq = uniform(desc_lo_sw128(smem_u32(smem))),
+                   sk = uniform(desc_lo_sw128(smem_u32(k_ring))),
+                   sv = uniform(desc_lo_rows128(smem_u32(v_ring), kKeys * 128));
+    const int n0 = uniform(tiles[0]), n1 = uniform(tiles[1]), steps = max(n0, n1);
+    bool ok = steps == 0 || warp_wait(&sh.q_full, 0);
     // S_q of key tile j.
     auto scores = [&](int q, int j) {
-      const uint32_t kt = sk + (j % T::kKStages) * T::kK;
+      const uint32_t qt = sq + q * (T::kQ >> 4), kt = uniform(sk + (j % T::kKStages) * (T::kK >> 4));
+      if (elect_one()) {
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
+        for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          tc_mma_f16(tmem + q * 128, umma_desc_sw128(sq + q * T::kQ + b * 16384 + kk * 32),
-                     umma_desc_sw128(kt + b * kKeys * 128 + kk * 32), score_desc, (b | kk) != 0);
-      tc_commit(&sh.s_full[q]);
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_f16(td + q * 128, desc_of(qt + ((b * 16384 + kk * 32) >> 4)),
+                       desc_of(kt + ((b * kKeys * 128 + kk * 32) >> 4)), score_desc, (b | kk) != 0);
+        tc_commit(&sh.s_full[q]);
+      }
+      __syncwarp();
     };
-    if (ok && all > 0) ok = mbar_wait(&sh.k_full[0], 0);
-    if (ok && all > 0 && lane == 0) {
+    if (ok && steps > 0) ok = warp_wait(&sh.k_full[0], 0);
+    if (ok && steps > 0) {
       tc_fence_after();
-      for (int q = 0; q < 2; ++q)
-        if (tiles[q] > 0) scores(q, 0);
-      tc_commit(&sh.k_empty[0]);
+      if (n0 > 0) scores(0, 0);
+      if (n1 > 0) scores(1, 0);
+      if (elect_one()) tc_commit(&sh.k_empty[0]);
     }
-    for (int j = 0; j < all && ok; ++j) {
+    for (int j = 0; j < steps && ok; ++j) {
       const int vs = j % T::kVStages;
-      ok = mbar_wait(&sh.v_full[vs], (j / T::kVStages) & 1);
+      ok = warp_wait(&sh.v_full[vs], (j / T::kVStages) & 1);
       if (!ok) break;
-      const int valid = keys - j * kKeys;
+      const int valid = uniform(keys) - j * kKeys;
       if (valid < kKeys) {  // rows behind the sequence's last key
         for (int i = lane; i < (kKeys - valid) * 8; i += 32)
           for (int b = 0; b < vb; ++b)
@@ -236,30 +242,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_async_smem();
         __syncwarp();
       }
-      bool next = j + 1 >= all;  // key tile j + 1 has arrived
-      for (int q = 0; q < 2 && ok; ++q) {
-        if (j >= tiles[q]) continue;
-        ok = mbar_wait(&sh.p_ready[q], j & 1);
+      bool next = j + 1 >= steps;  // key tile j + 1 has arrived
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int n = q ? n1 : n0;
+        if (!ok || j >= n) continue;
+        ok = warp_wait(&sh.p_ready[q], j & 1);
         if (ok && !next) {
-          ok = mbar_wait(&sh.k_full[(j + 1) % T::kKStages], ((j + 1) / T::kKStages) & 1);
+          ok = warp_wait(&sh.k_full[(j + 1) % T::kKStages], ((j + 1) / T::kKStages) & 1);
           next = true;
         }
-        if (!ok) break;
-        if (lane == 0) {
-          tc_fence_after();
-          const uint32_t vt = sv + vs * T::kV;
+        if (!ok) continue;
+        tc_fence_after();
+        const uint32_t vt = uniform(sv + vs * (T::kV >> 4));
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk)
-            tc_mma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + kk * 8,
-                          umma_desc_rows128(vt + kk * 2048, kKeys * 128), value_desc, (j | kk) != 0);
-          if (j + 1 < tiles[q]) scores(q, j + 1);
-          else tc_commit(&sh.o_done[q]);
+            tc_mma_f16_ts(td + 256 + q * 128, td + q * 128 + kk * 8, desc_of(vt + (kk * 2048 >> 4)), value_desc,
+                          kk > 0 || j > 0);
+          if (j + 1 >= n) tc_commit(&sh.o_done[q]);
         }
+        __syncwarp();
+        if (j + 1 < n) scores(q, j + 1);
       }
-      if (ok && lane == 0) {
+      if (ok && elect_one()) {
         tc_commit(&sh.v_empty[vs]);
-        if (j + 1 < all) tc_commit(&sh.k_empty[(j + 1) % T::kKStages]);
+        if (j + 1 < steps) tc_commit(&sh.k_empty[(j + 1) % T::kKStages]);
       }
+      __syncwarp();
     }
   } else {
     const int q = (warp - 2) / 4, quad = warp & 3;

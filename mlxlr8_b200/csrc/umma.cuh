@@ -76,6 +76,30 @@ __device__ __forceinline__ uint64_t umma_desc_rows128(uint32_t saddr, uint32_t b
          (static_cast<uint64_t>(2) << 61);
 }
 
+// The 64-bit descriptors above, by their low words: the high word of both
+// 128-byte forms is kDescHi, and a step of `bytes` along a tile adds bytes / 16
+// to the low word.  Matrix instructions take their operands from uniform
+// registers, so a loop that issues them runs on a whole warp, with low words
+// made uniform by `uniform` and the instructions under `elect_one`: built from
+// per-thread values, each instruction took 108 cycles to issue instead of the
+// 48 to 64 that it takes to run.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo_sw128(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_lo_rows128(uint32_t saddr, uint32_t block) {
+  return ((saddr & 0x3FFFFu) >> 4) | ((block >> 4) << 16);
+}
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | lo; }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+// mbar_wait by a whole warp with one answer, so that what follows stays uniform.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
 // D += A . B with A in tensor memory (two 16-bit values per column).
 __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
