@@ -207,17 +207,17 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     """All operands must live on one CUDA device; there is no CPU path."""
     if not torch.cuda.is_available():
         raise RuntimeError("the exlr8 B200 operators need a CUDA device (no CPU fallback)")
-    device = None
+    first = index = None
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise ValueError("exlr8 B200 operators take CUDA tensors")
-        if device is None:
-            device = t.device
-        elif t.device != device:
+        if first is None:
+            first, index = t, t.get_device()
+        elif t.get_device() != index:
             raise ValueError("operands are on different devices")
-    return device if device is not None else torch.device("cuda", torch.cuda.current_device())
+    return first.device if first is not None else torch.device("cuda", torch.cuda.current_device())
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -225,13 +225,17 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # The handle itself: a torch Stream object per call costs 2 us on the host.
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_HERE = nullcontext()
 
 
 def on_device(device: torch.device):
     """Context in which ``device`` is current: a launch on another device's
     stream than the current one's would fail."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def host_device_pointer(t: torch.Tensor) -> int:
@@ -240,6 +244,13 @@ def host_device_pointer(t: torch.Tensor) -> int:
     ptr = c_void_p(0)
     check(load().exlr8_host_device_pointer(t.data_ptr(), ctypes.byref(ptr)))
     return int(ptr.value)
+
+
+def like(t: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor | None:
+    """``t`` contiguous in ``dtype``."""
+    if t is None:
+        return None
+    return (t if t.dtype == dtype else t.to(dtype)).contiguous()
 
 
 def aligned(t: torch.Tensor) -> torch.Tensor:

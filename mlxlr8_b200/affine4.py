@@ -61,7 +61,7 @@ def affine4_linear(x, codes, scales, biases=None, *, x_scales=None, out_dtype=No
         x_code = _lib.act_code(x)
     if out is None:
         dtype = out_dtype or (torch.bfloat16 if x_scales is not None else x.dtype)
-        out = torch.empty(lead + (out_features,), dtype=dtype, device=device)
+        out = scales.new_empty(lead + (out_features,), dtype=dtype)
     elif out.shape != lead + (out_features,) or not out.is_contiguous() or out_dtype not in (None, out.dtype):
         raise ValueError("out must be a contiguous [..., out] tensor")
     x, codes, scales = _lib.aligned(x), _lib.aligned(codes), scales.contiguous()

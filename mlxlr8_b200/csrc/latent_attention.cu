@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int blocks = a.rank / 64, tile_pairs = a.rank / 128;
   if (warp == 0) {
+    pdl_wait();
     const int64_t total = total_tiles(w, lane);
     const int64_t n = sharers(total, gridDim.x);
     Walk walk{};
@@ -274,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_fence_init();
   } else if (warp > 2) {
     // Sequences without tokens are no CTA's work: their rows are zeroed here.
+    pdl_wait();
     const int64_t rows = static_cast<int64_t>(a.queries) * a.heads;
     for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
       if (tokens_of(w, b) > 0) continue;
@@ -283,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int64_t i = threadIdx.x - 96; i < rows; i += kThreads - 96) a.lse[b * rows + i] = -INFINITY;
     }
   }
+  pdl_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -584,64 +587,71 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ---- joining the parts ---------------------------------------------------------------
 
-constexpr int kJoinGroups = 4;   // rows a CTA takes; threads that share a channel of many parts
+constexpr int kJoinGroups = 4;  // rows a CTA takes at a time, or threads that share a channel's parts
 constexpr int kJoinThreads = 128 * kJoinGroups;
-constexpr int kJoinMany = 8;     // parts from which the groups share a row
+constexpr int kJoinShare = 4;   // CTAs per cut
 
-// A sequence is cut where a CTA's share begins inside it; the first such CTA's
-// index, blockIdx.x + 1, joins its parts, four rows a CTA.
+// A sequence is cut where a CTA's share begins inside it, and cut n of c cuts
+// joins every c-th row of it: blockIdx.x + 1 is that CTA, blockIdx.y one of
+// the four that divide its rows again.
 template <int kAct>
 __global__ void __launch_bounds__(kJoinThreads)
     latent_join_kernel(const LatentAttentionArgs a, const Work w, int kn, const float* __restrict__ parts,
                        const float2* __restrict__ sums, const Cut* __restrict__ cuts) {
   __shared__ float4 s_o[kJoinGroups][128];
+  pdl_launch_dependents();
   pdl_wait();
   const int64_t cta = blockIdx.x + 1;
   const Cut cut = cuts[cta];
-  if (cta >= cut.sharers) return;
-  if (first_tile(cta, cut.total, cut.sharers) <= cut.start ||
-      first_tile(cta - 1, cut.total, cut.sharers) > cut.start)
-    return;
-  // The part of CTA k lies in its first slot where the sequence is what its
-  // share begins with, else in its second.
+  if (cta >= cut.sharers || first_tile(cta, cut.total, cut.sharers) <= cut.start) return;
+  // The sequence's CTAs: `first` has its first tile, `last` its last.  A part
+  // lies in its CTA's first slot where the share begins with the sequence,
+  // else in the second.
+  const int64_t first = ((cut.start + 1) * cut.sharers - 1) / cut.total;
   const int64_t last = ((cut.start + cut.tiles) * cut.sharers - 1) / cut.total;
-  const int64_t slot0 = 2 * (cta - 1) + (first_tile(cta - 1, cut.total, cut.sharers) < cut.start ? 1 : 0);
-  auto slot_of = [&](int64_t k) { return k == cta - 1 ? slot0 : 2 * k; };
+  const int64_t slot0 = 2 * first + (first_tile(first, cut.total, cut.sharers) < cut.start ? 1 : 0);
+  auto slot_of = [&](int64_t k) { return k == first ? slot0 : 2 * k; };
   const int rows = w.queries * w.heads;
   const int thread = threadIdx.x & 127, group = threadIdx.x >> 7, lane = threadIdx.x & 31;
-  const int row0 = blockIdx.y * kJoinGroups;
-  const bool many = last - cta + 2 > kJoinMany;
-  for (int pass = 0; pass < (many ? kJoinGroups : 1); ++pass) {
-    const int i = row0 + (many ? pass : group), row = cut.rt * kn + i;
+  const int workers = static_cast<int>(last - first) * kJoinShare;
+  const int worker = static_cast<int>(cta - first - 1) * kJoinShare + blockIdx.y;
+  // Few rows a worker: the groups share a row's parts, else a row each.
+  const bool shared = kn < workers * kJoinGroups;
+  for (int i0 = worker; i0 < kn; i0 += workers * (shared ? 1 : kJoinGroups)) {
+    const int i = shared ? i0 : i0 + group * workers;
+    const int row = cut.rt * kn + i;
+    const bool there = i < kn && row < rows;
     // The largest unit and the sum, by every warp for itself.
     float top = -INFINITY, sum = 0.0f;
-    for (int64_t k = cta - 1 + lane; k <= last; k += 32) {
-      const float2 v = sums[slot_of(k) * kn + i];
-      if (v.y != 0.0f) top = fmaxf(top, v.x);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    for (int64_t k = cta - 1 + lane; k <= last; k += 32) {
-      const float2 v = sums[slot_of(k) * kn + i];
-      if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (4 * thread < a.rank) {
-#pragma unroll 4
-      for (int64_t k = cta - 1 + (many ? group : 0); k <= last; k += many ? kJoinGroups : 1) {
-        const int64_t at = slot_of(k) * kn + i;
-        const float2 v = sums[at];
-        const float4 part = *reinterpret_cast<const float4*>(parts + at * a.rank + 4 * thread);
-        const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
-        o.x = fmaf(part.x, f, o.x);
-        o.y = fmaf(part.y, f, o.y);
-        o.z = fmaf(part.z, f, o.z);
-        o.w = fmaf(part.w, f, o.w);
+    if (there) {
+      for (int64_t k = first + lane; k <= last; k += 32) {
+        const float2 v = sums[slot_of(k) * kn + i];
+        if (v.y != 0.0f) top = fmaxf(top, v.x);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      for (int64_t k = first + lane; k <= last; k += 32) {
+        const float2 v = sums[slot_of(k) * kn + i];
+        if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (4 * thread < a.rank) {
+#pragma unroll 8
+        for (int64_t k = first + (shared ? group : 0); k <= last; k += shared ? kJoinGroups : 1) {
+          const int64_t at = slot_of(k) * kn + i;
+          const float2 v = sums[at];
+          const float4 part = *reinterpret_cast<const float4*>(parts + at * a.rank + 4 * thread);
+          const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
+          o.x = fmaf(part.x, f, o.x);
+          o.y = fmaf(part.y, f, o.y);
+          o.z = fmaf(part.z, f, o.z);
+          o.w = fmaf(part.w, f, o.w);
+        }
       }
     }
-    if (many) {
+    if (shared) {
       s_o[group][thread] = o;
       __syncthreads();
       if (group == 0) {
@@ -657,7 +667,7 @@ __global__ void __launch_bounds__(kJoinThreads)
       __syncthreads();
       if (group != 0) continue;
     }
-    if (row >= rows) continue;
+    if (!there) continue;
     const int64_t at = cut.sequence * rows + row;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (a.lse && thread == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
@@ -720,12 +730,13 @@ cudaError_t launch(const LatentAttentionArgs& a, cudaStream_t s) {
   uint32_t columns = 32;
   while (columns < static_cast<uint32_t>(kN * (a.rank / 128 + 1))) columns *= 2;
   auto kernel = latent_attention_kernel<kAct, kN>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t err = allow_shared_memory(kernel, kSmem, ready);
   if (err != cudaSuccess) return err;
-  kernel<<<ctas, kThreads, kSmem, s>>>(maps, a, w, layout(a.rank, kN), box, columns, parts, sums, cuts);
-  err = cudaGetLastError();
+  err = launch_pdl(kernel, dim3(ctas), dim3(kThreads), kSmem, s, maps, a, w, layout(a.rank, kN), box, columns, parts,
+                   sums, cuts);
   if (err != cudaSuccess || ctas < 2) return err;
-  return launch_pdl(latent_join_kernel<kAct>, dim3(ctas - 1, kN / kJoinGroups), dim3(kJoinThreads), 0, s, a, w, kN,
+  return launch_pdl(latent_join_kernel<kAct>, dim3(ctas - 1, kJoinShare), dim3(kJoinThreads), 0, s, a, w, kN,
                     static_cast<const float*>(parts), static_cast<const float2*>(sums),
                     static_cast<const Cut*>(cuts));
 }

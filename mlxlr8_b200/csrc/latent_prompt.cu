@@ -30,6 +30,7 @@
 
 #include "common.cuh"
 #include "latent.cuh"
+#include "launch.cuh"
 #include "tensor_map.cuh"
 #include "umma.cuh"
 
@@ -102,6 +103,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // The CTA's sequence and its tile of 256 queries: tiles are numbered over
   // the sequences and taken from the last (its rows see the most keys).
+  pdl_launch_dependents();
+  pdl_wait();
   if (warp == 0) {
     int total = 0;
     for (int s0 = 0; s0 < a.seqs; s0 += 32) {
@@ -406,12 +409,13 @@ cudaError_t launch(const LatentPromptArgs& a, cudaStream_t s) {
                    empty ? a.q_token : a.v_token, empty ? a.q_head : a.v_head, T::kKeys))
     return cudaErrorInvalidValue;
   auto kernel = latent_prompt_kernel<kAct, kBlocks>;
-  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing + 1024);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t err = allow_shared_memory(kernel, kRing + 1024, ready);
   if (err != cudaSuccess) return err;
   const int parts = (a.value + 127) / 128;
   const int64_t tiles = (a.total_q + 255) / 256 + a.seqs;
-  kernel<<<static_cast<unsigned>(tiles * a.heads * parts), kThreads, kRing + 1024, s>>>(maps, a, parts);
-  return cudaGetLastError();
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * a.heads * parts)), dim3(kThreads), kRing + 1024, s, maps,
+                    a, parts);
 }
 
 template <int kAct>

@@ -12,7 +12,9 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <stdint.h>
 
+#include <atomic>
 #include <utility>
 
 namespace exlr8 {
@@ -30,6 +32,20 @@ template <typename Kernel>
 inline cudaError_t prefer_shared_carveout(Kernel kernel) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
                               static_cast<int>(cudaSharedmemCarveoutMaxShared));
+}
+
+// Allow `kernel` `bytes` of dynamic shared memory on the current device; asked
+// of the driver once per device (`done` is the kernel's own word of devices).
+template <typename Kernel>
+inline cudaError_t allow_shared_memory(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return err;
 }
 
 // `kernel<<<grid, block, smem, s>>>(args...)` with programmatic stream

@@ -41,7 +41,7 @@ def _check_cache(cache):
 
 
 def _index(name, t, shape, dtype):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+    if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} of shape {list(shape)}")
     return t.contiguous()
 
@@ -74,7 +74,7 @@ def latent_append(latent, rope_key, cache, slots, *, weight=None, eps: float = 1
     if weight is not None:
         if tuple(weight.shape) != (rank,):
             raise ValueError("the latent norm's weight must have one entry per latent channel")
-        weight = weight.to(cache.dtype).contiguous()
+        weight = _lib.like(weight, cache.dtype)
     if (cos_sin is None) != (positions is None):
         raise ValueError("cos_sin and positions go together")
     if cos_sin is not None:
@@ -90,7 +90,7 @@ def latent_append(latent, rope_key, cache, slots, *, weight=None, eps: float = 1
         _half("q_rope", q_rope, cache.dtype)
         q_rope, heads = _rows(q_rope), q_rope.shape[1]
         q_strides = q_rope.stride()[:2]
-        q_out = torch.empty((tokens, heads, ROPE), dtype=cache.dtype, device=device)
+        q_out = cache.new_empty((tokens, heads, ROPE))
     with _lib.on_device(device):
         _lib.check(_lib.lib().exlr8_latent_append(
             latent.data_ptr(), latent.stride(0), rope_key.data_ptr(), rope_key.stride(0), tokens, rank,
@@ -117,7 +117,7 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
     when it is large enough; calls that overlap need one each."""
     device = _lib.require_cuda(q_latent, q_rope, cache, block_table, lengths, out, workspace)
     rank = _check_cache(cache)
-    if q_latent.dim() != 4 or q_latent.shape[3] != rank or tuple(q_rope.shape) != tuple(q_latent.shape[:3]) + (ROPE,):
+    if q_latent.dim() != 4 or q_latent.shape[3] != rank or q_rope.shape != q_latent.shape[:3] + (ROPE,):
         raise ValueError("q_latent must be [batch, queries, heads, rank] and q_rope [batch, queries, heads, 64]")
     _half("q_latent", q_latent, cache.dtype)
     _half("q_rope", q_rope, cache.dtype)
@@ -135,7 +135,7 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
         out = torch.empty_like(q_latent)
     elif out.shape != q_latent.shape or out.dtype != cache.dtype or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous tensor like q_latent")
-    lse = torch.empty((batch, queries, heads), dtype=torch.float32, device=device) if return_lse else None
+    lse = q_latent.new_empty((batch, queries, heads), dtype=torch.float32) if return_lse else None
     lib = _lib.lib()
     with _lib.on_device(device):
         need = lib.exlr8_latent_attention_workspace(batch, queries, heads, rank)
@@ -197,11 +197,11 @@ def latent_prompt_attention(q, k, k_rope, v, q_starts, k_starts, scale: float, *
     q_starts = _index("q_starts", q_starts, (seqs + 1,), torch.int32)
     k_starts = _index("k_starts", k_starts, (seqs + 1,), torch.int32)
     if out is None:
-        out = torch.empty((total_q, heads, value), dtype=q.dtype, device=device)
+        out = q.new_empty((total_q, heads, value))
     elif tuple(out.shape) != (total_q, heads, value) or out.dtype != q.dtype or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous [total_q, heads, value] tensor")
-    lse = torch.empty((total_q, heads), dtype=torch.float32, device=device) if return_lse else None
+    lse = q.new_empty((total_q, heads), dtype=torch.float32) if return_lse else None
     with _lib.on_device(device):
         _lib.check(_lib.lib().exlr8_latent_prompt_attention(
             q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), k_rope.data_ptr(),

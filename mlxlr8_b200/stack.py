@@ -66,16 +66,15 @@ def residual_rms_norm_q8(x, weight, eps: float = 1e-5, residual=None, group: int
         raise ValueError("group must be 32, 64, 128 or the row's width, and divide it")
     code = _lib.act_code(x)
     x = x.contiguous()
-    rows = x.numel() // hidden
-    w = weight.to(x.dtype).contiguous()
-    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty(x.shape[:-1] + (hidden // group,), dtype=torch.float32, device=device)
+    w, res = _lib.like(weight, x.dtype), _lib.like(residual, x.dtype)
+    codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scales = x.new_empty(x.shape[:-1] + (hidden // group,), dtype=torch.float32)
     h = torch.empty_like(x) if return_sum else None
-    res = residual.to(x.dtype).contiguous() if residual is not None else None
     with _lib.on_device(device):
-        _lib.check(_lib.lib().exlr8_residual_rms_norm_q8(x.data_ptr(), _lib.ptr(res), w.data_ptr(), code, rows, hidden,
-                                                         group, float(eps), _lib.ptr(h), codes.data_ptr(),
-                                                         scales.data_ptr(), _lib.stream_handle(device)))
+        _lib.check(_lib.lib().exlr8_residual_rms_norm_q8(x.data_ptr(), _lib.ptr(res), w.data_ptr(), code,
+                                                         x.numel() // hidden, hidden, group, eps, _lib.ptr(h),
+                                                         codes.data_ptr(), scales.data_ptr(),
+                                                         _lib.stream_handle(device)))
     return (h, codes, scales) if return_sum else (codes, scales)
 
 
