@@ -32,122 +32,114 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// Eight channels as float32 and back.
+// Eight channels as stored: four words of two 16-bit values, or eight floats.
 template <int kAct>
-__device__ __forceinline__ void load8(const void* p, int64_t at, float (&v)[8]) {
-  if constexpr (kAct == kF32) {
-    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-    const float4 a = src[0], b = src[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+struct Eight {
+  uint32_t v[kAct == kF32 ? 8 : 4];
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + at * (kAct == kF32 ? 4 : 2));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (kAct == kBF16) {
-        v[2 * i] = __uint_as_float(u[i] << 16);
-        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      }
+    for (int i = 0; i < (kAct == kF32 ? 2 : 1); ++i) {
+      const uint4 u = src[i];
+      v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
     }
   }
-}
-
-template <int kAct>
-__device__ __forceinline__ void store8(void* p, int64_t at, const float (&v)[8]) {
-  if constexpr (kAct == kF32) {
-    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
-    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint32_t u[4];
+  __device__ __forceinline__ void store(void* p, int64_t at) const {
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(p) + at * (kAct == kF32 ? 4 : 2));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (kAct == kBF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-      else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-    }
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+    for (int i = 0; i < (kAct == kF32 ? 2 : 1); ++i) dst[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint32_t& u : v) u = 0;
+  }
+  // The sum, rounded once to the type.
+  __device__ __forceinline__ void add(const Eight& o) {
+#pragma unroll
+    for (int i = 0; i < (kAct == kF32 ? 8 : 4); ++i) {
+      if (kAct == kF32) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(o.v[i]));
+      else if (kAct == kF16) asm("add.rn.f16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(v[i]), "r"(o.v[i]));
+      else asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(v[i]), "r"(o.v[i]));
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if (kAct == kF32) return __uint_as_float(v[i]);
+    const uint32_t u = v[i / 2];
+    if (kAct == kBF16) return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? u >> 16 : u & 0xffffu)));
+  }
+};
 
 // One row per CTA, kVecs vectors of eight channels a thread, all kept in
 // registers between the sum of squares and the codes: each input is read
 // once.  A group is 4, 8 or 16 lanes of one vector index, or (kWhole) the row.
+// The code of y = h inv w is that of h w over its own maximum, so inv enters the
+// scale alone.
 template <int kAct, int kVecs, bool kWhole>
-__global__ void __launch_bounds__(1024) residual_rms_q8_kernel(const void* __restrict__ x,
-                                                              const void* __restrict__ residual,
-                                                              const void* __restrict__ w, int hidden, int group,
-                                                              float eps, void* __restrict__ h_out,
-                                                              uint8_t* __restrict__ codes,
-                                                              float* __restrict__ scales) {
-  __shared__ float red[32];
+__global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024)
+    residual_rms_q8_kernel(const void* __restrict__ x, const void* __restrict__ residual, const void* __restrict__ w,
+                           int hidden, int group, float eps, void* __restrict__ h_out, uint8_t* __restrict__ codes,
+                           float* __restrict__ scales) {
+  __shared__ float red[2][32];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, vecs = hidden / 8;
   const int64_t base = static_cast<int64_t>(blockIdx.x) * hidden;
-  float h[kVecs][8];
+  Eight<kAct> h[kVecs], r[kVecs], f[kVecs];
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int v = i * blockDim.x + threadIdx.x;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[i][e] = 0.0f;
-    if (v < vecs) load8<kAct>(x, base + 8 * v, h[i]);
-  }
-  if (residual) {
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int v = i * blockDim.x + threadIdx.x;
-      float r[8] = {};
-      if (v < vecs) load8<kAct>(residual, base + 8 * v, r);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[i][e] = round_to(kAct, h[i][e] + r[e]);
+    if (v < vecs) {
+      h[i].load(x, base + 8 * v);
+      if (residual) r[i].load(residual, base + 8 * v);
+      f[i].load(w, 8 * v);
+    } else {
+      h[i].zero();
+      r[i].zero();
+      f[i].zero();
     }
   }
   float acc = 0.0f;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int v = i * blockDim.x + threadIdx.x;
-    if (h_out && v < vecs) store8<kAct>(h_out, base + 8 * v, h[i]);
+    if (residual) h[i].add(r[i]);
+    if (h_out && v < vecs) h[i].store(h_out, base + 8 * v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc = fmaf(h[i][e], h[i][e], acc);
+    for (int e = 0; e < 8; ++e) acc = fmaf(h[i].at(e), h[i].at(e), acc);
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-  if (lane == 0) red[threadIdx.x >> 5] = acc;
-  __syncthreads();
-  acc = lane < warps ? red[lane] : 0.0f;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-  const float inv = 1.0f / sqrtf(acc / static_cast<float>(hidden) + eps);
-  float top[kVecs];
+  float y[kVecs][8], top[kVecs];
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int v = i * blockDim.x + threadIdx.x;
     top[i] = 0.0f;
-    float f[8];
-    if (v < vecs) {
-      load8<kAct>(w, 8 * v, f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        h[i][e] = h[i][e] * inv * f[e];
-        top[i] = max_nan(top[i], fabsf(h[i][e]));
-      }
+    for (int e = 0; e < 8; ++e) {
+      y[i][e] = h[i].at(e) * f[i].at(e);
+      top[i] = max_nan(top[i], fabsf(y[i][e]));
     }
-    if (!kWhole)
-      for (int off = group >> 4; off > 0; off >>= 1) top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+    if (!kWhole) {
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1)
+        if (off <= group >> 4) top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], off));
+    }
   }
   if (kWhole) {
 #pragma unroll
     for (int i = 1; i < kVecs; ++i) top[0] = max_nan(top[0], top[i]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top[0] = max_nan(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
-    __syncthreads();
-    if (lane == 0) red[threadIdx.x >> 5] = top[0];
-    __syncthreads();
-    top[0] = lane < warps ? red[lane] : 0.0f;
+    if (lane == 0) red[1][threadIdx.x >> 5] = top[0];
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+  if (lane == 0) red[0][threadIdx.x >> 5] = acc;
+  __syncthreads();
+  acc = lane < warps ? red[0][lane] : 0.0f;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+  const float inv = 1.0f / sqrtf(acc / static_cast<float>(hidden) + eps);
+  if (kWhole) {
+    top[0] = lane < warps ? red[1][lane] : 0.0f;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top[0] = max_nan(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
   }
@@ -157,18 +149,21 @@ __global__ void __launch_bounds__(1024) residual_rms_q8_kernel(const void* __res
     const int v = i * blockDim.x + threadIdx.x;
     if (v >= vecs) continue;
     const float t = kWhole ? top[0] : top[i];
-    const bool finite = t < __int_as_float(0x7f800000);
-    const float mul = finite && t > 0.0f ? 448.0f / t : 0.0f;
+    // inv is 0 in a row with an infinity, NaN in one with a NaN.
+    const float scale = t * inv / 448.0f;
+    const bool finite = t < __int_as_float(0x7f800000) && scale < __int_as_float(0x7f800000);
+    const float mul = scale > 0.0f && finite ? 448.0f / t : 0.0f;
     uint32_t two[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      uint16_t r;
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(h[i][2 * e + 1] * mul), "f"(h[i][2 * e] * mul));
-      two[e] = finite ? r : 0u;
+      uint16_t c;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(y[i][2 * e + 1] * mul), "f"(y[i][2 * e] * mul));
+      two[e] = c;
     }
-    *reinterpret_cast<uint2*>(codes + base + 8 * v) = make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16);
+    const uint2 out = finite ? make_uint2(two[0] | two[1] << 16, two[2] | two[3] << 16) : make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(codes + base + 8 * v) = out;
     if (kWhole ? v == 0 : threadIdx.x % lanes == 0)
-      scales[kWhole ? blockIdx.x : base / group + v / lanes] = finite ? t / 448.0f : __int_as_float(0x7fc00000);
+      scales[kWhole ? blockIdx.x : base / group + v / lanes] = finite ? scale : __int_as_float(0x7fc00000);
   }
 }
 
@@ -249,7 +244,7 @@ cudaError_t launch(const void* x, const void* residual, const void* w, int64_t r
     return launch_vectors<kAct, 1>(x, residual, w, rows, hidden, group, eps, h_out, codes, scales, s);
   if (vectors && vecs <= (few ? 2048 : 512))
     return launch_vectors<kAct, 2>(x, residual, w, rows, hidden, group, eps, h_out, codes, scales, s);
-  if (vectors && vecs <= (few ? 4096 : 1024))
+  if (vectors && !few && vecs <= 2048)
     return launch_vectors<kAct, 4>(x, residual, w, rows, hidden, group, eps, h_out, codes, scales, s);
   return launch_pdl(residual_rms_q8_any_kernel<kAct>, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, s, x,
                     residual, w, hidden, group, eps, h_out, codes, scales);

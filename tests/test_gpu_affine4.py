@@ -59,6 +59,7 @@ def _check(x, codes, scales, biases, x_scales=None, out_dtype=None, out=None):
     (1, 6144, 576, 64, True), (1, 512, 1000, 128, False), (2, 32, 1, 32, True), (3, 96, 33, 32, True),
     (8, 2080, 130, 32, False), (9, 1024, 64, 128, True), (16, 1152, 257, 64, True), (17, 640, 48, 128, False),
     (33, 256, 31, 64, True), (1, 128, 5, 128, True), (5, 64, 16, 64, False), (4, 16384, 70, 128, True),
+    (8, 8192, 4000, 32, True), (16, 12288, 300, 32, False), (3, 6144, 5000, 64, True),
 ])
 def test_float_activations(dtype, rows, inner, outer, group, biases):
     import torch
