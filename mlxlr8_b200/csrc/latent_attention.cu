@@ -6,9 +6,9 @@
 // tokens.
 //
 // The rows (query, head) of a sequence are the narrow side, so both products
-// are taken transposed, with 128 tokens or 128 latent channels on the tensor
+// are taken transposed, with 64 tokens or 128 latent channels on the tensor
 // core's M side and kN = 16, 32 or 64 rows on its N side:
-//   S^T [128 tokens][kN]  = C Q^T       cache tile as loaded (channels contiguous)
+//   S^T [64 tokens][kN]   = C Q^T       cache tile as loaded (channels contiguous)
 //   P^T = 2^(c S^T + base)              one thread per token, float32, to shared memory
 //   O^T [rank][kN]       += C^T P^T     the same tile, taken with its tokens contracted
 // A cache tile is read from memory once and feeds both products.  base = 6 -
@@ -19,19 +19,22 @@
 // Weights stay below 2^14 and float16 ones keep full precision down to 2^-20
 // of the largest.  Sums are float32, of the unrounded weights.
 //
-// Work is the flat list of (sequence, row tile, 128 tokens), cut evenly over
+// Work is the flat list of (sequence, row tile, 64 tokens), cut evenly over
 // the CTAs (one per SM) whatever the lengths; a sequence cut in two or more
 // leaves float32 parts in the workspace, which a second kernel joins.
 //
-// Warp 0 loads (TMA; one box per page or 16 to 128 of its tokens), warp 1
-// issues the matrix instructions, warps 2-5 and 6-9 each take half of the
-// rows for all 128 tokens.  The latent is loaded as pairs of 64-channel
-// blocks (one M = 128 of the second product) into a ring; a pair is given back
-// as soon as its product is done.  Where shared memory has no room for the
-// rotary block it shares P's buffer: the scores are done with it before P is
-// written.  Token rows that belong to no token are zeroed in the tile, since
-// 0 x NaN would reach the sum.  Waits are bounded; one that runs out leaves NaN
-// in the rows that it concerns.
+// Warp 0 loads (TMA; one box per page or 16 to 64 of its tokens), warps 1 and 2
+// issue the two products, so that the scores of the next tile are formed while
+// this one's weights are; warps 4-7 and 8-11 each take half of the rows for the
+// 64 tokens.  Tiles of 64 tokens, not 128, because the queries (72 KB at 64
+// rows of 576) leave room for 1.7 tiles of 64 but not for two of 128: with one
+// tile of 128 nothing overlapped and a tile's chain of load, scores, weights
+// and product was the bound (167 us for 64 sequences of up to 12000 tokens).  The
+// latent is loaded as pairs of 64-channel blocks (one M = 128 of the second
+// product) into a ring; a pair is given back as soon as its product is done.
+// Token rows that belong to no token are zeroed in the tile, since 0 x NaN would
+// reach the sum.  Waits are bounded; one that runs out leaves NaN in the rows
+// that it concerns.
 
 #include <cuda.h>
 
@@ -45,15 +48,16 @@ namespace exlr8 {
 
 namespace {
 
-constexpr int kThreads = 320;
-constexpr int kTile = 128;  // tokens
+constexpr int kThreads = 384;
+constexpr int kTile = 64;  // tokens
 constexpr float kLift = 6.0f;
 constexpr float kLag = 8.0f;
-constexpr uint32_t kBlock = kTile * 128;  // 128 tokens x 64 channels
+constexpr uint32_t kBlock = kTile * 128;  // 64 tokens x 64 channels
 constexpr uint32_t kPair = 2 * kBlock;
-constexpr int kMaxPairs = 8;        // ring slots
+constexpr int kMaxStages = 4;       // tiles in the ring
+constexpr int kMaxPairs = 4 * kMaxStages;
 constexpr int kMinTiles = 2;        // tiles a CTA takes at least, where there are as many
-constexpr uint32_t kSmem = 229888;  // dynamic shared memory, with 1 KB for its alignment
+constexpr uint32_t kSmem = 232448;  // all of a CTA's shared memory
 
 // ---- the flat list of tiles -----------------------------------------------------
 
@@ -145,12 +149,12 @@ struct Cut {
 // ---- the main kernel -------------------------------------------------------------
 
 struct Layout {
-  uint32_t q, p, rope, ring;  // byte offsets in shared memory
-  int pairs, ropes;           // ring slots; rotary buffers (0: it shares P's)
+  uint32_t q, p, rope, ring, shared;  // byte offsets in shared memory; P is two deep
+  int stages, ropes;                  // whole tiles in the ring; rotary buffers, 1 or 2
 };
 
 struct Shared {
-  uint64_t q_full, q_empty, s_full, p_ready, o_done;
+  uint64_t q_full, q_empty, o_done, s_full[2], s_empty[2], p_ready[2], p_done[2];
   uint64_t full[kMaxPairs], empty[kMaxPairs], rope_full[2], rope_empty[2];
   uint32_t tmem;
   Walk walk;
@@ -161,15 +165,15 @@ struct Shared {
   int limit[64];
 };
 
-// A place in the ring and the parity of its round.  (Slots are counted, not
-// divided: a division per pair made the issuing warp the bound.)
+// A tile of the ring and the parity of its round.  (Counted, not divided, and
+// of whole tiles, so that the issuing warps add constants to one base a tile:
+// with a division, and later a broadcast, per pair they were the bound.)
 struct Place {
-  int slot = 0;
+  int stage = 0;
   uint32_t round = 0;
-  __device__ __forceinline__ void advance(int by, int slots) {
-    slot += by;
-    if (slot >= slots) {
-      slot -= slots;
+  __device__ __forceinline__ void advance(int stages) {
+    if (++stage == stages) {
+      stage = 0;
       round ^= 1;
     }
   }
@@ -182,12 +186,6 @@ struct Maps {
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
-__device__ __forceinline__ float warp_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 
@@ -223,17 +221,16 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&v
   else tc_st8(taddr, v);
 }
 
-// parts: [2 * CTAs][kN][rank] float32, then [2 * CTAs][kN] pairs (log2 of the
-// unit of O and the sum, sum).
+// parts: [2 * CTAs][kN][rank] float32, sums: [2 * CTAs][kN] pairs (log2 of the
+// unit of O and the sum, the sum).
 template <int kAct, int kN>
 __global__ void __launch_bounds__(kThreads, 1)
     latent_attention_kernel(const __grid_constant__ Maps maps, const LatentAttentionArgs a, const Work w, const Layout lay,
                             int box, uint32_t columns, float* __restrict__ parts, float2* __restrict__ sums,
                             Cut* __restrict__ cuts) {
   pdl_launch_dependents();
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ Shared sh;
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];  // (nothing static lies before it)
+  Shared& sh = *reinterpret_cast<Shared*>(smem + lay.shared);
   const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int blocks = a.rank / 64, tile_pairs = a.rank / 128;
   if (warp == 0) {
@@ -261,8 +258,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 2 && lane == 0) {
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
-    mbar_init(&sh.s_full, 1);
-    mbar_init(&sh.p_ready, 256);
     mbar_init(&sh.o_done, 1);
     for (int i = 0; i < kMaxPairs; ++i) {
       mbar_init(&sh.full[i], 1);
@@ -271,6 +266,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.rope_full[i], 1);
       mbar_init(&sh.rope_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.s_empty[i], 256);
+      mbar_init(&sh.p_ready[i], 256);
+      mbar_init(&sh.p_done[i], 1);
     }
     mbar_fence_init();
   } else if (warp > 2) {
@@ -291,8 +290,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   Walk walk = sh.walk;
   const uint32_t tmem = sh.tmem, t_scores = tmem + tile_pairs * kN;
-  const int ropes = lay.ropes > 0 ? lay.ropes : 1;
-  const uint32_t rope_at = lay.ropes > 0 ? lay.rope : lay.p;
   bool ok = true;
 
   if (warp == 0) {
@@ -317,106 +314,122 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row >= 0)) * box * 128;
         for (int i = 0; ok && i < tile_pairs; ++i, ++loaded) {
-          uint64_t* full = &sh.full[place.slot];
-          ok = mbar_wait(&sh.empty[place.slot], place.round ^ 1);  // (passes in the first round)
+          const int slot = place.stage * tile_pairs + i;
+          uint64_t* full = &sh.full[slot];
+          ok = mbar_wait(&sh.empty[slot], place.round ^ 1);  // (passes in the first round)
           if (!ok) break;
           if (lane == 0) mbar_arrive_expect_tx(full, 2 * bytes);
           __syncwarp();
           if (row >= 0) {
-            uint8_t* dst = smem + lay.ring + place.slot * kPair + lane * box * 128;
+            uint8_t* dst = smem + lay.ring + slot * kPair + lane * box * 128;
             tma_load_2d(dst, &maps.cache, 128 * i, row, full);
             tma_load_2d(dst + kBlock, &maps.cache, 128 * i + 64, row, full);
           }
-          place.advance(1, lay.pairs);
         }
         if (!ok) break;
-        const int r = u & (ropes - 1);
-        ok = mbar_wait(&sh.rope_empty[r], ((u >> (ropes - 1)) & 1) ^ 1);
+        place.advance(lay.stages);
+        const int r = u & (lay.ropes - 1);
+        ok = mbar_wait(&sh.rope_empty[r], ((u >> (lay.ropes - 1)) & 1) ^ 1);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sh.rope_full[r], bytes);
         __syncwarp();
-        if (row >= 0) tma_load_2d(smem + rope_at + r * kBlock + lane * box * 128, &maps.cache, a.rank, row, &sh.rope_full[r]);
+        if (row >= 0) tma_load_2d(smem + lay.rope + r * kBlock + lane * box * 128, &maps.cache, a.rank, row, &sh.rope_full[r]);
       }
     }
     // Copies still in flight land before the CTA's memory is given back.
     if (segment > 0) mbar_wait(&sh.q_full, (segment - 1) & 1);
-    for (int i = max(0, loaded - lay.pairs); i < loaded; ++i) mbar_wait(&sh.full[i % lay.pairs], (i / lay.pairs) & 1);
-    for (int i = max(0, u - ropes); i < u; ++i) mbar_wait(&sh.rope_full[i & (ropes - 1)], (i >> (ropes - 1)) & 1);
-  } else if (warp == 1) {
-    const uint32_t score_desc = half_idesc(kAct == kBF16, kN, a.scale < 0.0f, false, false);
-    const uint32_t value_desc = half_idesc(kAct == kBF16, kN, false, true, true);
-    const uint32_t td = uniform(tmem), ts = td + tile_pairs * kN;
-    const uint32_t sq = uniform(desc_lo_sw128(smem_u32(smem + lay.q))),
-                   sp = uniform(desc_lo_rows128(smem_u32(smem + lay.p), kBlock)),
+    const int slots = lay.stages * tile_pairs;
+    for (int i = max(0, loaded - slots); i < loaded; ++i) mbar_wait(&sh.full[i % slots], (i / slots) & 1);
+    for (int i = max(0, u - lay.ropes); i < u; ++i)
+      mbar_wait(&sh.rope_full[i & (lay.ropes - 1)], (i >> (lay.ropes - 1)) & 1);
+  } else if (warp == 1) {  // scores
+    const uint32_t desc = half_idesc(kAct == kBF16, kN, a.scale < 0.0f, false, false, kTile);
+    const uint32_t ts = uniform(t_scores), sq = uniform(desc_lo_sw128(smem_u32(smem + lay.q))),
                    sc = uniform(desc_lo_sw128(smem_u32(smem + lay.ring))),
-                   sv = uniform(desc_lo_rows128(smem_u32(smem + lay.ring), kBlock)),
-                   sr = uniform(desc_lo_sw128(smem_u32(smem + rope_at)));
+                   sr = uniform(desc_lo_sw128(smem_u32(smem + lay.rope)));
     int u = 0;
-    Place first;  // of the tile
+    Place place;
     for (int segment = 0; ok && uniform(walk.next(w)); ++segment) {
       const int begin = uniform(walk.begin), end = uniform(walk.end);
       ok = warp_wait(&sh.q_full, segment & 1);
-      for (int t = begin; ok && t < end; ++t, ++u, first.advance(tile_pairs, lay.pairs)) {
-        Place place = first;
-        for (int i = 0; ok && i < tile_pairs; ++i, place.advance(1, lay.pairs)) {
-          ok = warp_wait(&sh.full[place.slot], place.round);
-          if (!ok) break;
+      for (int t = begin; ok && t < end; ++t, ++u) {
+        const int r = u & 1;
+        const uint32_t to = uniform(ts + r * kN);
+        ok = warp_wait(&sh.s_empty[r], ((u >> 1) & 1) ^ 1);  // (passes in the first round)
+        const uint32_t ct = uniform(sc + place.stage * (tile_pairs * (kPair >> 4)));
+#pragma unroll
+        for (int i = 0; i < kLatentMaxRank / 128; ++i) {
+          if (i >= tile_pairs || !ok) continue;
+          ok = warp_wait(&sh.full[place.stage * tile_pairs + i], place.round);
+          if (!ok) continue;
           tc_fence_after();
-          const uint32_t ct = uniform(sc + place.slot * (kPair >> 4)), qt = uniform(sq + i * (2 * kN * 128 >> 4));
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              tc_mma_f16(ts, desc_of(ct + (((k / 4) * kBlock + (k % 4) * 32) >> 4)),
-                         desc_of(qt + (((k / 4) * kN * 128 + (k % 4) * 32) >> 4)), score_desc, k > 0 || i > 0);
+              tc_mma_f16(to, desc_of(ct + ((i * kPair + (k / 4) * kBlock + (k % 4) * 32) >> 4)),
+                         desc_of(sq + (((2 * i + k / 4) * kN * 128 + (k % 4) * 32) >> 4)), desc, k > 0 || i > 0);
           }
           __syncwarp();
         }
-        const int r = u & (ropes - 1);
-        if (ok) ok = warp_wait(&sh.rope_full[r], (u >> (ropes - 1)) & 1);
+        place.advance(lay.stages);
+        const int rope = u & (lay.ropes - 1);
+        if (ok) ok = warp_wait(&sh.rope_full[rope], (u >> (lay.ropes - 1)) & 1);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t rt = uniform(sr + r * (kBlock >> 4)), qr = uniform(sq + blocks * (kN * 128 >> 4));
+        const uint32_t rt = uniform(sr + rope * (kBlock >> 4)), qr = sq + blocks * (kN * 128 >> 4);
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16(ts, desc_of(rt + (k * 32 >> 4)), desc_of(qr + (k * 32 >> 4)), score_desc, 1);
-          tc_commit(&sh.s_full);
-          if (lay.ropes > 0) tc_commit(&sh.rope_empty[r]);
+          for (int k = 0; k < 4; ++k) tc_mma_f16(to, desc_of(rt + (k * 32 >> 4)), desc_of(qr + (k * 32 >> 4)), desc, 1);
+          tc_commit(&sh.s_full[r]);
+          tc_commit(&sh.rope_empty[rope]);
           if (t + 1 == end) tc_commit(&sh.q_empty);
-        }
-        __syncwarp();
-        ok = warp_wait(&sh.p_ready, u & 1);
-        if (!ok) break;
-        tc_fence_after();
-        place = first;
-        for (int i = 0; i < tile_pairs; ++i, place.advance(1, lay.pairs)) {
-          const uint32_t ct = uniform(sv + place.slot * (kPair >> 4)), to = uniform(td + i * kN);
-          const uint32_t more = t > begin;
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              tc_mma_f16(to, desc_of(ct + (k * 2048 >> 4)), desc_of(sp + (k * 2048 >> 4)), value_desc,
-                         k > 0 ? 1 : more);
-            tc_commit(&sh.empty[place.slot]);
-          }
-          __syncwarp();
-        }
-        if (elect_one()) {
-          if (lay.ropes == 0) tc_commit(&sh.rope_empty[r]);
-          if (t + 1 == end) tc_commit(&sh.o_done);
         }
         __syncwarp();
       }
     }
-  } else {
+  } else if (warp == 2) {  // products with the weights
+    const uint32_t desc = half_idesc(kAct == kBF16, kN, false, true, true);
+    const uint32_t td = uniform(tmem), sp = uniform(desc_lo_rows128(smem_u32(smem + lay.p), kBlock)),
+                   sv = uniform(desc_lo_rows128(smem_u32(smem + lay.ring), kBlock));
+    int u = 0;
+    Place place;
+    while (ok && uniform(walk.next(w))) {
+      const int begin = uniform(walk.begin), end = uniform(walk.end);
+      for (int t = begin; ok && t < end; ++t, ++u) {
+        ok = warp_wait(&sh.p_ready[u & 1], (u >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t pt = uniform(sp + (u & 1) * (kBlock >> 4));
+        const uint32_t ct = uniform(sv + place.stage * (tile_pairs * (kPair >> 4)));
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < kLatentMaxRank / 128; ++i) {
+            if (i >= tile_pairs) continue;
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+              tc_mma_f16(td + i * kN, desc_of(ct + ((i * kPair + k * 2048) >> 4)), desc_of(pt + (k * 2048 >> 4)), desc,
+                         k > 0 || t > begin);
+            tc_commit(&sh.empty[place.stage * tile_pairs + i]);
+          }
+          tc_commit(&sh.p_done[u & 1]);
+          if (t + 1 == end) tc_commit(&sh.o_done);
+        }
+        __syncwarp();
+        place.advance(lay.stages);
+      }
+    }
+  } else if (warp >= 4) {
     constexpr int kCols = kN / 2;
-    const int half = (warp - 2) / 4, quad = warp & 3, bar = 1 + half;
-    const int token_row = quad * 32 + lane, col0 = half * kCols;
+    // Tensor memory has a quarter's 16 tokens in lanes 0 to 15; lanes 16 to 31
+    // take half of their rows over, so that lane i has token i % 16 and kOwn rows.
+    constexpr int kOwn = kCols / 2;
+    const int half = (warp - 4) / 4, quad = warp & 3, bar = 1 + half;
+    const int token_row = quad * 16 + (lane & 15), col0 = half * kCols, own0 = col0 + (lane >> 4) * kOwn;
     const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
     const float c = fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f;
     const int rows = a.queries * a.heads;
     int u = 0;
-    Place first;
+    Place place;
     for (int segment = 0; walk.next(w); ++segment) {
       // One warp of each half keeps its rows' maxima and limits.
       if (quad == 0 && lane < kCols) {
@@ -427,50 +440,63 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       group_sync(bar);
       const int least = walk.tokens - a.queries + 1 + walk.rt * kN / a.heads;
-      float l[kCols];
+      float l[kOwn];
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) l[i] = 0.0f;
-      for (int t = walk.begin; t < walk.end; ++t, ++u, first.advance(tile_pairs, lay.pairs)) {
-        const int token = t * kTile + token_row;
+      for (int i = 0; i < kOwn; ++i) l[i] = 0.0f;
+      for (int t = walk.begin; t < walk.end; ++t, ++u, place.advance(lay.stages)) {
+        const int token = t * kTile + token_row, r = u & 1;
         bool held = token < walk.tokens;
         if (held) {
           const int page = a.block_table[walk.b * a.table_width + token / a.page_size];
           held = page >= 0 && page < a.pages;
         }
-        if (ok) ok = mbar_wait(&sh.s_full, u & 1);
+        if (ok) ok = mbar_wait(&sh.s_full[r], (u >> 1) & 1);
         tc_fence_after();
-        uint32_t s[kCols];
-        load_columns<kCols>(t_scores + lanes + col0, s);
+        uint32_t all[kCols];
+        load_columns<kCols>(t_scores + lanes + r * kN + col0, all);
         tc_wait_ld();
-        tc_settle<kCols>(s);
-        if (!held && ok) {
-          for (int i = half * blocks / 2; i < (half + 1) * blocks / 2; ++i) {
-            uint4* line = reinterpret_cast<uint4*>(smem + lay.ring + (first.slot + i / 2) % lay.pairs * kPair +
-                                                   (i & 1) * kBlock + token_row * 128);
+        tc_settle<kCols>(all);
+        tc_fence_before();
+        mbar_arrive(&sh.s_empty[r]);
+        float s[kOwn];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) line[e] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < kOwn; ++i) {
+          const uint32_t other = __shfl_sync(0xffffffffu, all[kOwn + i], lane & 15);
+          s[i] = __uint_as_float(lane < 16 ? all[i] : other);
+        }
+        // P's buffer is free once the products of the tile before the last are done.
+        if (ok && u > 1) ok = mbar_wait(&sh.p_done[r], ((u >> 1) - 1) & 1);
+        if (!held && ok) {
+          // the two lanes of a token zero half of this half's blocks each
+          uint8_t* tile = smem + lay.ring + place.stage * tile_pairs * kPair + token_row * 128;
+          for (int i = half * blocks / 2; i < (half + 1) * blocks / 2; ++i) {
+            uint4* line = reinterpret_cast<uint4*>(tile + i * kBlock) + (lane >> 4) * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) line[e] = make_uint4(0, 0, 0, 0);
           }
         }
         if (__any_sync(0xffffffffu, !held || token >= least)) {
 #pragma unroll
-          for (int i = 0; i < kCols; ++i)
-            if (!held || token >= sh.limit[col0 + i]) s[i] = 0xff800000u;
+          for (int i = 0; i < kOwn; ++i)
+            if (!held || token >= sh.limit[own0 + i]) s[i] = -INFINITY;
         }
+        float base[kOwn];
         float grown = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kCols; i += 4) {
-          const float4 base = *reinterpret_cast<const float4*>(&sh.base[col0 + i]);
-          grown = fmaxf(grown, fmaxf(fmaf(__uint_as_float(s[i]), c, base.x), fmaf(__uint_as_float(s[i + 1]), c, base.y)));
-          grown = fmaxf(grown, fmaxf(fmaf(__uint_as_float(s[i + 2]), c, base.z), fmaf(__uint_as_float(s[i + 3]), c, base.w)));
+        for (int i = 0; i < kOwn; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(&sh.base[own0 + i]);
+          base[i] = v.x, base[i + 1] = v.y, base[i + 2] = v.z, base[i + 3] = v.w;
         }
-        if (group_any(bar, grown > kLift + kLag)) {
-          float mine = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < kCols; ++i) {
-            const float top = warp_max(__uint_as_float(s[i]));
-            if (lane == i) mine = top;
+        for (int i = 0; i < kOwn; ++i) grown = fmaxf(grown, fmaf(s[i], c, base[i]));
+        if (group_any(bar, grown > kLift + kLag)) {
+#pragma unroll
+          for (int i = 0; i < kOwn; ++i) {
+            float top = s[i];
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            if ((lane & 15) == i) sh.top[quad][own0 + i] = top;
           }
-          if (lane < kCols) sh.top[quad][col0 + lane] = mine;
           group_sync(bar);
           if (quad == 0 && lane < kCols) {
             const int i = col0 + lane;
@@ -482,16 +508,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           group_sync(bar);
 #pragma unroll
-          for (int i = 0; i < kCols; i += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(&sh.factor[col0 + i]);
-            l[i] *= f.x;
-            l[i + 1] *= f.y;
-            l[i + 2] *= f.z;
-            l[i + 3] *= f.w;
+          for (int i = 0; i < kOwn; ++i) {
+            l[i] *= sh.factor[own0 + i];
+            base[i] = sh.base[own0 + i];
           }
-          // The products of the tiles before are complete: this tile's scores
-          // were committed after them.
           if (t > walk.begin) {
+            if (ok) ok = mbar_wait(&sh.p_done[r ^ 1], ((u - 1) >> 1) & 1);  // the products of the tile before
+            tc_fence_after();
 #pragma unroll 1
             for (int k = 0; k < tile_pairs; ++k) {
               uint32_t o[kCols];
@@ -505,38 +528,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_wait_st();
           }
         }
-        uint8_t* line = smem + lay.p + token_row * 128;
+        uint32_t p[kOwn / 2];
 #pragma unroll
-        for (int i = 0; i < kCols; i += 8) {
-          uint32_t p[4];
+        for (int i = 0; i < kOwn; i += 2) {
+          // a row without a maximum has only hidden tokens: -inf + inf would be NaN
+          const float p0 = exp2_fast(fmaf(s[i], c, base[i] == INFINITY ? 0.0f : base[i]));
+          const float p1 = exp2_fast(fmaf(s[i + 1], c, base[i + 1] == INFINITY ? 0.0f : base[i + 1]));
+          l[i] += p0;
+          l[i + 1] += p1;
+          p[i / 2] = pack<kAct>(p0, p1);
+        }
+        // Row `token` of P, 16-byte pieces swizzled by the token.
+        uint8_t* line = smem + lay.p + r * kBlock + token_row * 128;
+        if constexpr (kOwn >= 8) {
 #pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            const float4 base = *reinterpret_cast<const float4*>(&sh.base[col0 + i + e]);
-            // a row without a maximum has only hidden tokens: -inf + inf would be NaN
-            const float p0 = exp2_fast(fmaf(__uint_as_float(s[i + e]), c, base.x == INFINITY ? 0.0f : base.x));
-            const float p1 = exp2_fast(fmaf(__uint_as_float(s[i + e + 1]), c, base.y == INFINITY ? 0.0f : base.y));
-            const float p2 = exp2_fast(fmaf(__uint_as_float(s[i + e + 2]), c, base.z == INFINITY ? 0.0f : base.z));
-            const float p3 = exp2_fast(fmaf(__uint_as_float(s[i + e + 3]), c, base.w == INFINITY ? 0.0f : base.w));
-            l[i + e] += p0;
-            l[i + e + 1] += p1;
-            l[i + e + 2] += p2;
-            l[i + e + 3] += p3;
-            p[e / 2] = pack<kAct>(p0, p1);
-            p[e / 2 + 1] = pack<kAct>(p2, p3);
-          }
-          const int chunk = (half * kCols + i) / 8;
-          *reinterpret_cast<uint4*>(line + ((chunk ^ (token_row & 7)) * 16)) = make_uint4(p[0], p[1], p[2], p[3]);
+          for (int i = 0; i < kOwn; i += 8)
+            *reinterpret_cast<uint4*>(line + ((((own0 + i) / 8) ^ (token_row & 7)) * 16)) =
+                make_uint4(p[i / 2], p[i / 2 + 1], p[i / 2 + 2], p[i / 2 + 3]);
+        } else {
+          *reinterpret_cast<uint2*>(line + (((own0 / 8) ^ (token_row & 7)) * 16) + (own0 & 4) * 2) = make_uint2(p[0], p[1]);
         }
         fence_async_smem();
         tc_fence_before();
-        mbar_arrive(&sh.p_ready);
+        mbar_arrive(&sh.p_ready[r]);
       }
       // The segment's sums over the tokens, then its output.
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) {
+      for (int i = 0; i < kOwn; ++i) {
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
-        if (lane == i) sh.top[quad][col0 + i] = l[i];
+        for (int off = 8; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+        if ((lane & 15) == i) sh.top[quad][own0 + i] = l[i];
       }
       group_sync(bar);
       const bool whole = walk.begin == 0 && walk.end == walk.tiles;
@@ -562,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < kCols; ++i) o[i] = 0x7fc00000u;
         }
-        const int channel = 128 * k + token_row;
+        const int channel = 128 * k + quad * 32 + lane;
         if (!whole) {
           float* dst = parts + (slot * kN + col0) * a.rank + channel;
 #pragma unroll
@@ -685,21 +706,21 @@ int sm_count() {
   return sms;
 }
 
+// Two tiles in the ring let the next one land and be scored while this one is
+// weighed; with 1.75 (two rotary buffers at 64 rows of rank 512) every tile
+// waited for its last pair (64 sequences of up to 12000 tokens: 202 us, not 178).
 Layout layout(int rank, int kn) {
-  const uint32_t room = kSmem - 1024, q = (rank / 64 + 1) * kn * 128;
-  const int tile_pairs = rank / 128;
   Layout l{};
   l.q = 0;
-  l.p = q;  // a multiple of 1 KB: kn * 128 is one of 2 KB
-  l.rope = l.p + kBlock;
-  // Rotary buffers of their own where the ring still holds a pair more than a
-  // tile; without them the rotary block waits for P's buffer.
-  for (l.ropes = 2; l.ropes >= 0; --l.ropes) {
+  l.p = (rank / 64 + 1) * kn * 128;  // a multiple of 1 KB: kn * 128 is one of 2 KB
+  l.rope = l.p + 2 * kBlock;
+  for (l.ropes = 2;; --l.ropes) {
     l.ring = l.rope + l.ropes * kBlock;
-    l.pairs = static_cast<int>((room - l.ring) / kPair);
-    if (l.pairs > kMaxPairs) l.pairs = kMaxPairs;
-    if (l.pairs > tile_pairs || l.ropes == 0) break;
+    l.stages = static_cast<int>((kSmem - sizeof(Shared) - l.ring) / (rank / 128 * kPair));
+    if (l.stages >= 2 || l.ropes == 1) break;
   }
+  if (l.stages > kMaxStages) l.stages = kMaxStages;
+  l.shared = l.ring + l.stages * (rank / 128) * kPair;
   return l;
 }
 
@@ -713,7 +734,7 @@ cudaError_t launch(const LatentAttentionArgs& a, cudaStream_t s) {
   float* parts = static_cast<float*>(a.workspace);
   float2* sums = reinterpret_cast<float2*>(parts + 2ll * ctas * kN * a.rank);
   Cut* cuts = reinterpret_cast<Cut*>(sums + 2ll * ctas * kN);
-  // The largest power of two (16 to 128) that divides a page: no box crosses one.
+  // The largest power of two (16 to 64) that divides a page: no box crosses one.
   int box = 16;
   while (box < kTile && a.page_size % (2 * box) == 0) box *= 2;
   Maps maps;
@@ -728,13 +749,14 @@ cudaError_t launch(const LatentAttentionArgs& a, cudaStream_t s) {
                        box, CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
   uint32_t columns = 32;
-  while (columns < static_cast<uint32_t>(kN * (a.rank / 128 + 1))) columns *= 2;
+  while (columns < static_cast<uint32_t>(kN * (a.rank / 128 + 2))) columns *= 2;
   auto kernel = latent_attention_kernel<kAct, kN>;
   static std::atomic<uint64_t> ready{0};
   cudaError_t err = allow_shared_memory(kernel, kSmem, ready);
   if (err != cudaSuccess) return err;
-  err = launch_pdl(kernel, dim3(ctas), dim3(kThreads), kSmem, s, maps, a, w, layout(a.rank, kN), box, columns, parts,
-                   sums, cuts);
+  const Layout lay = layout(a.rank, kN);
+  err = launch_pdl(kernel, dim3(ctas), dim3(kThreads), lay.shared + sizeof(Shared), s, maps, a, w, lay, box, columns,
+                   parts, sums, cuts);
   if (err != cudaSuccess || ctas < 2) return err;
   return launch_pdl(latent_join_kernel<kAct>, dim3(ctas - 1, kJoinShare), dim3(kJoinThreads), 0, s, a, w, kN,
                     static_cast<const float*>(parts), static_cast<const float2*>(sums),

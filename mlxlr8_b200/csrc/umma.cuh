@@ -58,13 +58,15 @@ __device__ __forceinline__ void tc_mma_f16(uint32_t d, uint64_t a, uint64_t b, u
       : "memory");
 }
 
-// kind::f16 descriptor, M = 128, float32 accumulator: A and B both float16 or
-// both bfloat16, `negate_a` multiplies A by -1, `b_rows` takes B with its N
-// side contiguous (rows of the contracted dimension).
-__host__ __device__ __forceinline__ uint32_t half_idesc(bool bf16, int n, bool negate_a, bool a_rows, bool b_rows) {
+// kind::f16 descriptor, float32 accumulator: A and B both float16 or both
+// bfloat16, `negate_a` multiplies A by -1, `a_rows` and `b_rows` take the operand
+// with its M or N side contiguous (rows of the contracted dimension).  m is 128
+// or 64; the 64 rows of D then lie in lanes 0 to 15 of each warp's 32.
+__host__ __device__ __forceinline__ uint32_t half_idesc(bool bf16, int n, bool negate_a, bool a_rows, bool b_rows,
+                                                        int m = 128) {
   const uint32_t fmt = bf16 ? 1u : 0u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (negate_a ? 1u << 13 : 0u) | (a_rows ? 1u << 15 : 0u) |
-         (b_rows ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+         (b_rows ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
 // 128-byte swizzle with the M or N side contiguous: rows of 64 16-bit values
