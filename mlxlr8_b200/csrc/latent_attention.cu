@@ -112,7 +112,17 @@ __device__ __forceinline__ int64_t sharers(int64_t total, int ctas) {
   const int64_t n = (total + kMinTiles - 1) / kMinTiles;
   return n < ctas ? n : ctas;
 }
-__device__ __forceinline__ int64_t first_tile(int64_t i, int64_t total, int64_t n) { return i * total / n; }
+__device__ __forceinline__ int64_t first_tile(int64_t i, int64_t total, int64_t n) {
+  // (a 64-bit division takes longer than the lists that need one are common)
+  if (total < (1 << 20)) return static_cast<uint32_t>(i) * static_cast<uint32_t>(total) / static_cast<uint32_t>(n);
+  return i * total / n;
+}
+
+// The CTA of flat tile x: the last whose first tile is not behind it.
+__device__ __forceinline__ int64_t owner_of(int64_t x, int64_t total, int64_t n) {
+  if (total < (1 << 20)) return (static_cast<uint32_t>(x + 1) * static_cast<uint32_t>(n) - 1) / static_cast<uint32_t>(total);
+  return ((x + 1) * n - 1) / total;
+}
 
 // A CTA's walk over its share: one segment per (sequence, row tile).
 struct Walk {
@@ -608,18 +618,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ---- joining the parts ---------------------------------------------------------------
 
-constexpr int kJoinGroups = 4;  // rows a CTA takes at a time, or threads that share a channel's parts
-constexpr int kJoinThreads = 128 * kJoinGroups;
+constexpr int kJoinWarps = 16;
 constexpr int kJoinShare = 4;   // CTAs per cut
 
 // A sequence is cut where a CTA's share begins inside it, and cut n of c cuts
-// joins every c-th row of it: blockIdx.x + 1 is that CTA, blockIdx.y one of
-// the four that divide its rows again.
+// joins every c-th row of it: blockIdx.x + 1 is that CTA, blockIdx.y one of the
+// four that divide its rows again.  A warp takes a row, 16 channels a lane;
+// with fewer rows than warps, the warps share a row's parts.
 template <int kAct>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(32 * kJoinWarps)
     latent_join_kernel(const LatentAttentionArgs a, const Work w, int kn, const float* __restrict__ parts,
                        const float2* __restrict__ sums, const Cut* __restrict__ cuts) {
-  __shared__ float4 s_o[kJoinGroups][128];
+  __shared__ float4 s_o[kJoinWarps][kLatentMaxRank / 4];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t cta = blockIdx.x + 1;
@@ -628,73 +638,85 @@ __global__ void __launch_bounds__(kJoinThreads)
   // The sequence's CTAs: `first` has its first tile, `last` its last.  A part
   // lies in its CTA's first slot where the share begins with the sequence,
   // else in the second.
-  const int64_t first = ((cut.start + 1) * cut.sharers - 1) / cut.total;
-  const int64_t last = ((cut.start + cut.tiles) * cut.sharers - 1) / cut.total;
-  const int64_t slot0 = 2 * first + (first_tile(first, cut.total, cut.sharers) < cut.start ? 1 : 0);
-  auto slot_of = [&](int64_t k) { return k == first ? slot0 : 2 * k; };
-  const int rows = w.queries * w.heads;
-  const int thread = threadIdx.x & 127, group = threadIdx.x >> 7, lane = threadIdx.x & 31;
-  const int workers = static_cast<int>(last - first) * kJoinShare;
-  const int worker = static_cast<int>(cta - first - 1) * kJoinShare + blockIdx.y;
-  // Few rows a worker: the groups share a row's parts, else a row each.
-  const bool shared = kn < workers * kJoinGroups;
-  for (int i0 = worker; i0 < kn; i0 += workers * (shared ? 1 : kJoinGroups)) {
-    const int i = shared ? i0 : i0 + group * workers;
+  const int first = static_cast<int>(owner_of(cut.start, cut.total, cut.sharers));
+  const int last = static_cast<int>(owner_of(cut.start + cut.tiles - 1, cut.total, cut.sharers));
+  const int slot0 = 2 * first + (first_tile(first, cut.total, cut.sharers) < cut.start ? 1 : 0);
+  auto slot_of = [&](int k) { return k == first ? slot0 : 2 * k; };
+  const int rows = w.queries * w.heads, count = last - first + 1, vectors = a.rank / 128;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int workers = (count - 1) * kJoinShare;
+  const int worker = (static_cast<int>(cta) - first - 1) * kJoinShare + blockIdx.y;
+  const bool shared = kn <= workers;
+  for (int i0 = worker; i0 < kn; i0 += workers * (shared ? 1 : kJoinWarps)) {
+    const int i = shared ? i0 : i0 + warp * workers;
     const int row = cut.rt * kn + i;
     const bool there = i < kn && row < rows;
     // The largest unit and the sum, by every warp for itself.
     float top = -INFINITY, sum = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float4 o[kLatentMaxRank / 128] = {};
     if (there) {
-      for (int64_t k = first + lane; k <= last; k += 32) {
-        const float2 v = sums[slot_of(k) * kn + i];
+      for (int k = lane; k < count; k += 32) {
+        const float2 v = sums[slot_of(first + k) * kn + i];
         if (v.y != 0.0f) top = fmaxf(top, v.x);
       }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      for (int64_t k = first + lane; k <= last; k += 32) {
-        const float2 v = sums[slot_of(k) * kn + i];
+      for (int k = lane; k < count; k += 32) {
+        const float2 v = sums[slot_of(first + k) * kn + i];
         if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
       }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      if (4 * thread < a.rank) {
-#pragma unroll 8
-        for (int64_t k = first + (shared ? group : 0); k <= last; k += shared ? kJoinGroups : 1) {
-          const int64_t at = slot_of(k) * kn + i;
-          const float2 v = sums[at];
-          const float4 part = *reinterpret_cast<const float4*>(parts + at * a.rank + 4 * thread);
-          const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
-          o.x = fmaf(part.x, f, o.x);
-          o.y = fmaf(part.y, f, o.y);
-          o.z = fmaf(part.z, f, o.z);
-          o.w = fmaf(part.w, f, o.w);
+#pragma unroll 4
+      for (int k = shared ? warp : 0; k < count; k += shared ? kJoinWarps : 1) {
+        const int at = slot_of(first + k) * kn + i;
+        const float2 v = sums[at];
+        const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
+        const float4* part = reinterpret_cast<const float4*>(parts + static_cast<int64_t>(at) * a.rank) + lane;
+#pragma unroll
+        for (int e = 0; e < kLatentMaxRank / 128; ++e) {
+          if (e >= vectors) break;
+          const float4 p = part[32 * e];
+          o[e].x = fmaf(p.x, f, o[e].x);
+          o[e].y = fmaf(p.y, f, o[e].y);
+          o[e].z = fmaf(p.z, f, o[e].z);
+          o[e].w = fmaf(p.w, f, o[e].w);
         }
       }
     }
     if (shared) {
-      s_o[group][thread] = o;
-      __syncthreads();
-      if (group == 0) {
 #pragma unroll
-        for (int g = 1; g < kJoinGroups; ++g) {
-          const float4 v = s_o[g][thread];
-          o.x += v.x;
-          o.y += v.y;
-          o.z += v.z;
-          o.w += v.w;
+      for (int e = 0; e < kLatentMaxRank / 128; ++e)
+        if (e < vectors) s_o[warp][32 * e + lane] = o[e];
+      __syncthreads();
+      // warp e adds up channels 128 e to 128 e + 127
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (warp < vectors) {
+#pragma unroll
+        for (int g = 0; g < kJoinWarps; ++g) {
+          const float4 p = s_o[g][32 * warp + lane];
+          v.x += p.x;
+          v.y += p.y;
+          v.z += p.z;
+          v.w += p.w;
         }
       }
       __syncthreads();
-      if (group != 0) continue;
+      if (warp >= vectors) continue;
+      o[0] = v;
     }
     if (!there) continue;
     const int64_t at = cut.sequence * rows + row;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (a.lse && thread == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-    if (4 * thread < a.rank)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * a.rank + 4 * thread) =
-          make_uint2(pack<kAct>(o.x * inv, o.y * inv), pack<kAct>(o.z * inv, o.w * inv));
+    if (a.lse && lane == 0 && (!shared || warp == 0))
+      a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * a.rank) + lane;
+#pragma unroll
+    for (int e = 0; e < kLatentMaxRank / 128; ++e) {
+      if (e >= (shared ? 1 : vectors)) break;
+      dst[32 * (shared ? warp : e)] =
+          make_uint2(pack<kAct>(o[e].x * inv, o[e].y * inv), pack<kAct>(o[e].z * inv, o[e].w * inv));
+    }
   }
 }
 
@@ -758,7 +780,7 @@ cudaError_t launch(const LatentAttentionArgs& a, cudaStream_t s) {
   err = launch_pdl(kernel, dim3(ctas), dim3(kThreads), lay.shared + sizeof(Shared), s, maps, a, w, lay, box, columns,
                    parts, sums, cuts);
   if (err != cudaSuccess || ctas < 2) return err;
-  return launch_pdl(latent_join_kernel<kAct>, dim3(ctas - 1, kJoinShare), dim3(kJoinThreads), 0, s, a, w, kN,
+  return launch_pdl(latent_join_kernel<kAct>, dim3(ctas - 1, kJoinShare), dim3(32 * kJoinWarps), 0, s, a, w, kN,
                     static_cast<const float*>(parts), static_cast<const float2*>(sums),
                     static_cast<const Cut*>(cuts));
 }

@@ -19,6 +19,12 @@
 // is why two tiles share a CTA (and why each K and V tile is read from L2
 // once for 256 queries).
 //
+// The two query tiles leave room for 1.6 tiles of keys and values (at 192 key
+// channels), so K and V tiles share one ring of blocks of 64 channels, in the
+// order of their use: the next V lands while this one is multiplied, the next
+// but one K as soon as it is done.  (Two places for K and one for V left the
+// tensor pipe waiting for V in every tile: 757 us for 8192 queries of 32 heads.)
+//
 // Warp 0 loads (TMA), warp 1 issues the matrix instructions, warps 2-5 and
 // 6-9 are the softmax of query tiles 0 and 1.  Value channels beyond 128 are
 // a second CTA's (the scores are formed again there).  Rows of the last key
@@ -42,21 +48,21 @@ constexpr int kThreads = 320;
 constexpr int kTileQ = 128;
 constexpr float kLift = 6.0f;       // weights are 2^6 of their share of the maximum
 constexpr float kLag = 8.0f;        // log2 by which a maximum may lag
-constexpr uint32_t kRing = 229376;  // 224 KB of operand tiles
+constexpr uint32_t kSmem = 229376;  // 224 KB of operand tiles
 
 template <int kBlocks>  // 64-channel blocks of a key: 2, 3 or 4
 struct Tiles {
   static constexpr int kKeys = kBlocks == 4 ? 64 : 128;
-  static constexpr uint32_t kQ = kBlocks * 16384;         // one query tile
-  static constexpr uint32_t kK = kBlocks * kKeys * 128;   // one key tile
-  static constexpr uint32_t kV = 2 * kKeys * 128;         // one value tile
-  static constexpr int kKStages = 2;
-  static constexpr int kVStages = kBlocks == 3 ? 1 : 2;
-  static_assert(2 * kQ + kKStages * kK + kVStages * kV <= kRing, "operand tiles exceed shared memory");
+  static constexpr uint32_t kQ = kBlocks * 16384;    // one query tile
+  static constexpr uint32_t kBlock = kKeys * 128;    // 64 channels of a key or value tile
+  static constexpr int kRing = (kSmem - 2 * kQ) / kBlock;
+  static_assert(kRing >= kBlocks + 4, "a key tile and two value tiles");
 };
 
+constexpr int kUnits = 8;  // key and value tiles that the barriers tell apart; the ring holds five at most
+
 struct Shared {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t q_full, full[kUnits], empty[kUnits];
   uint64_t s_full[2], p_ready[2], o_done[2];
   uint32_t tmem;
   int seq, tile;
@@ -95,8 +101,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* const k_ring = smem + 2 * T::kQ;
-  uint8_t* const v_ring = k_ring + T::kKStages * T::kK;
+  uint8_t* const ring = smem + 2 * T::kQ;
   const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int columns = a.heads * value_parts;
   const int head = blockIdx.x % columns / value_parts, part = blockIdx.x % value_parts;
@@ -135,11 +140,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       sh.seq = found;
       sh.tile = tile;
       mbar_init(&sh.q_full, 1);
+      for (int i = 0; i < kUnits; ++i) {
+        mbar_init(&sh.full[i], 1);
+        mbar_init(&sh.empty[i], 1);
+      }
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&sh.k_full[i], 1);
-        mbar_init(&sh.k_empty[i], 1);
-        mbar_init(&sh.v_full[i], 1);
-        mbar_init(&sh.v_empty[i], 1);
         mbar_init(&sh.s_full[i], 1);
         mbar_init(&sh.p_ready[i], kTileQ);
         mbar_init(&sh.o_done[i], 1);
@@ -178,99 +183,129 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = 0; b < kBlocks; ++b)
           load_tile(smem + q * T::kQ + b * 16384, &maps.q, maps.q_swap, 64 * b, head, q0 + first + q * kTileQ,
                     &sh.q_full);
-      int j = 0;
-      for (; j < all && ok; ++j) {
-        const int ks = j % T::kKStages, vs = j % T::kVStages;
-        if (j >= T::kKStages) ok = mbar_wait(&sh.k_empty[ks], (j / T::kKStages - 1) & 1);
-        if (!ok) break;
-        uint8_t* kt = k_ring + ks * T::kK;
-        mbar_arrive_expect_tx(&sh.k_full[ks], T::kK);
-        for (int b = 0; b < kBlocks - 1; ++b)
-          load_tile(kt + b * kKeys * 128, &maps.k, maps.k_swap, 64 * b, head, k0 + j * kKeys, &sh.k_full[ks]);
-        tma_load_2d(kt + (kBlocks - 1) * kKeys * 128, &maps.r, 0, k0 + j * kKeys, &sh.k_full[ks]);
-        if (j >= T::kVStages) ok = mbar_wait(&sh.v_empty[vs], (j / T::kVStages - 1) & 1);
-        if (!ok) {
-          mbar_wait(&sh.k_full[ks], (j / T::kKStages) & 1);
-          break;
+      // Unit 2 j is key tile j, unit 2 j + 1 value tile j.  `used` blocks have been
+      // given out since the start, `freed` given back.
+      int unit = 0, gone = 0, used = 0, freed = 0, at = 0;
+      for (; unit < 2 * all && ok; ++unit) {
+        const int j = unit >> 1, n = unit & 1 ? vb : kBlocks;
+        while (ok && used + n - freed > T::kRing) {
+          ok = mbar_wait(&sh.empty[gone % kUnits], (gone / kUnits) & 1);
+          freed += gone & 1 ? vb : kBlocks;
+          ++gone;
         }
-        uint8_t* vt = v_ring + vs * T::kV;
-        mbar_arrive_expect_tx(&sh.v_full[vs], vb * kKeys * 128);
-        for (int b = 0; b < vb; ++b)
-          load_tile(vt + b * kKeys * 128, &maps.v, maps.v_swap, 128 * part + 64 * b, head, k0 + j * kKeys,
-                    &sh.v_full[vs]);
+        if (!ok) break;
+        uint64_t* full = &sh.full[unit % kUnits];
+        mbar_arrive_expect_tx(full, n * T::kBlock);
+        for (int b = 0; b < n; ++b) {
+          uint8_t* dst = ring + at * T::kBlock;
+          if (unit & 1) load_tile(dst, &maps.v, maps.v_swap, 128 * part + 64 * b, head, k0 + j * kKeys, full);
+          else if (b < kBlocks - 1) load_tile(dst, &maps.k, maps.k_swap, 64 * b, head, k0 + j * kKeys, full);
+          else tma_load_2d(dst, &maps.r, 0, k0 + j * kKeys, full);
+          if (++at == T::kRing) at = 0;
+        }
+        used += n;
       }
       // Copies still in flight land before the CTA's memory is given back.
       mbar_wait(&sh.q_full, 0);
-      for (int u = max(0, j - 2); u < j; ++u) mbar_wait(&sh.k_full[u % T::kKStages], (u / T::kKStages) & 1);
-      for (int u = max(0, j - T::kVStages); u < j; ++u) mbar_wait(&sh.v_full[u % T::kVStages], (u / T::kVStages) & 1);
+      for (int u = max(0, unit - kUnits); u < unit; ++u) mbar_wait(&sh.full[u % kUnits], (u / kUnits) & 1);
     }
   } else if (warp == 1) {
     const uint32_t score_desc = half_idesc(kAct == kBF16, kKeys, a.scale < 0.0f, false, false);
     const uint32_t value_desc = half_idesc(kAct == kBF16, 64 * vb, false, false, true);
+    const uint32_t half_desc = half_idesc(kAct == kBF16, 64, false, false, true);
     const uint32_t td = uniform(tmem), sq = uniform(desc_lo_sw128(smem_u32(smem))),
-                   sk = uniform(desc_lo_sw128(smem_u32(k_ring))),
-                   sv = uniform(desc_lo_rows128(smem_u32(v_ring), kKeys * 128));
+                   sk = uniform(desc_lo_sw128(smem_u32(ring))),
+                   sv = uniform(desc_lo_rows128(smem_u32(ring), T::kBlock));
     const int n0 = uniform(tiles[0]), n1 = uniform(tiles[1]), steps = max(n0, n1);
     bool ok = steps == 0 || warp_wait(&sh.q_full, 0);
-    // S_q of key tile j.
-    auto scores = [&](int q, int j) {
-      const uint32_t qt = sq + q * (T::kQ >> 4), kt = uniform(sk + (j % T::kKStages) * (T::kK >> 4));
+    int at = 0;  // the block after the last tile's
+    // The blocks of the next tile, as low words of their descriptors.
+    auto blocks = [&](uint32_t base, int n, uint32_t* lo) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        if (b >= n) break;
+        lo[b] = uniform(base + at * (T::kBlock >> 4));
+        if (++at == T::kRing) at = 0;
+      }
+    };
+    // S_q of a key tile.
+    auto scores = [&](int q, const uint32_t* kt) {
+      const uint32_t qt = sq + q * (T::kQ >> 4);
       if (elect_one()) {
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16(td + q * 128, desc_of(qt + ((b * 16384 + kk * 32) >> 4)),
-                       desc_of(kt + ((b * kKeys * 128 + kk * 32) >> 4)), score_desc, (b | kk) != 0);
+            tc_mma_f16(td + q * 128, desc_of(qt + ((b * 16384 + kk * 32) >> 4)), desc_of(kt[b] + (kk * 32 >> 4)),
+                       score_desc, (b | kk) != 0);
         tc_commit(&sh.s_full[q]);
       }
       __syncwarp();
     };
-    if (ok && steps > 0) ok = warp_wait(&sh.k_full[0], 0);
+    uint32_t kt[4], vt[4];
+    if (ok && steps > 0) ok = warp_wait(&sh.full[0], 0);
     if (ok && steps > 0) {
       tc_fence_after();
-      if (n0 > 0) scores(0, 0);
-      if (n1 > 0) scores(1, 0);
-      if (elect_one()) tc_commit(&sh.k_empty[0]);
+      blocks(sk, kBlocks, kt);
+      if (n0 > 0) scores(0, kt);
+      if (n1 > 0) scores(1, kt);
+      if (elect_one()) tc_commit(&sh.empty[0]);
+      __syncwarp();
     }
     for (int j = 0; j < steps && ok; ++j) {
-      const int vs = j % T::kVStages;
-      ok = warp_wait(&sh.v_full[vs], (j / T::kVStages) & 1);
+      const int unit = 2 * j + 1;
+      ok = warp_wait(&sh.full[unit % kUnits], (unit / kUnits) & 1);
       if (!ok) break;
+      const int first_block = at;
+      blocks(sv, vb, vt);
       const int valid = uniform(keys) - j * kKeys;
       if (valid < kKeys) {  // rows behind the sequence's last key
-        for (int i = lane; i < (kKeys - valid) * 8; i += 32)
-          for (int b = 0; b < vb; ++b)
-            reinterpret_cast<uint4*>(v_ring + vs * T::kV + (b * kKeys + valid) * 128)[i] = make_uint4(0, 0, 0, 0);
+        for (int b = 0; b < vb; ++b) {
+          uint8_t* tile = ring + (first_block + b < T::kRing ? first_block + b : first_block + b - T::kRing) * T::kBlock;
+          for (int i = lane; i < (kKeys - valid) * 8; i += 32)
+            reinterpret_cast<uint4*>(tile + valid * 128)[i] = make_uint4(0, 0, 0, 0);
+        }
         fence_async_smem();
         __syncwarp();
       }
-      bool next = j + 1 >= steps;  // key tile j + 1 has arrived
+      const bool joined = vb == 1 || first_block + 1 < T::kRing;  // the value blocks lie in a row
+      const bool more = j + 1 < steps;
+      bool next = !more;  // key tile j + 1 has arrived
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int n = q ? n1 : n0;
         if (!ok || j >= n) continue;
         ok = warp_wait(&sh.p_ready[q], j & 1);
-        if (ok && !next) {
-          ok = warp_wait(&sh.k_full[(j + 1) % T::kKStages], ((j + 1) / T::kKStages) & 1);
-          next = true;
-        }
         if (!ok) continue;
         tc_fence_after();
-        const uint32_t vt = uniform(sv + vs * (T::kV >> 4));
         if (elect_one()) {
+          if (joined) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)
-            tc_mma_f16_ts(td + 256 + q * 128, td + q * 128 + kk * 8, desc_of(vt + (kk * 2048 >> 4)), value_desc,
-                          kk > 0 || j > 0);
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              tc_mma_f16_ts(td + 256 + q * 128, td + q * 128 + kk * 8, desc_of(vt[0] + (kk * 2048 >> 4)), value_desc,
+                            kk > 0 || j > 0);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+#pragma unroll
+              for (int b = 0; b < 2; ++b)
+                tc_mma_f16_ts(td + 256 + q * 128 + 64 * b, td + q * 128 + kk * 8, desc_of(vt[b] + (kk * 2048 >> 4)),
+                              half_desc, kk > 0 || j > 0);
+          }
           if (j + 1 >= n) tc_commit(&sh.o_done[q]);
         }
         __syncwarp();
-        if (j + 1 < n) scores(q, j + 1);
+        if (!next) {
+          ok = warp_wait(&sh.full[(unit + 1) % kUnits], ((unit + 1) / kUnits) & 1);
+          tc_fence_after();
+          blocks(sk, kBlocks, kt);
+          next = true;
+        }
+        if (ok && j + 1 < n) scores(q, kt);
       }
       if (ok && elect_one()) {
-        tc_commit(&sh.v_empty[vs]);
-        if (j + 1 < steps) tc_commit(&sh.k_empty[(j + 1) % T::kKStages]);
+        tc_commit(&sh.empty[unit % kUnits]);
+        if (more) tc_commit(&sh.empty[(unit + 1) % kUnits]);
       }
       __syncwarp();
     }
@@ -410,11 +445,11 @@ cudaError_t launch(const LatentPromptArgs& a, cudaStream_t s) {
     return cudaErrorInvalidValue;
   auto kernel = latent_prompt_kernel<kAct, kBlocks>;
   static std::atomic<uint64_t> ready{0};
-  cudaError_t err = allow_shared_memory(kernel, kRing + 1024, ready);
+  cudaError_t err = allow_shared_memory(kernel, kSmem + 1024, ready);
   if (err != cudaSuccess) return err;
   const int parts = (a.value + 127) / 128;
   const int64_t tiles = (a.total_q + 255) / 256 + a.seqs;
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * a.heads * parts)), dim3(kThreads), kRing + 1024, s, maps,
+  return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * a.heads * parts)), dim3(kThreads), kSmem + 1024, s, maps,
                     a, parts);
 }
 
