@@ -12,7 +12,8 @@
 // with c = |scale| log2(e) (a negative scale negates Q in the instruction),
 // m a running maximum and l = sum P the float32 sum of the unrounded weights.
 // m is raised only when a row's maximum has grown by more than 2^8 (then O and
-// l are multiplied once), so P stays below 2^14 and float16 weights keep their
+// l are multiplied once and the tile is weighed again), so a tile is weighed
+// without a pass for its maximum first, and P stays below 2^14 and float16 weights keep their
 // full precision down to 2^-20 of the largest.  Tensor memory is full: S_0,
 // S_1, O_0, O_1 of 128 columns each, P_q over S_q.  While the threads of one
 // query tile form its weights the tensor pipe works for the other one, which
@@ -25,8 +26,13 @@
 // but one K as soon as it is done.  (Two places for K and one for V left the
 // tensor pipe waiting for V in every tile: 757 us for 8192 queries of 32 heads.)
 //
-// Warp 0 loads (TMA), warp 1 issues the matrix instructions, warps 2-5 and
-// 6-9 are the softmax of query tiles 0 and 1.  Value channels beyond 128 are
+// The softmax of a tile adds and multiplies two float32 at a time: issue slots,
+// not the special-function unit, bounded it (655 us to 576 us; taking a part of
+// the exponentials from a polynomial on the multiply-add pipe gained nothing).
+//
+// Warp 0 loads (TMA), warp 1 issues the matrix instructions, warps 4-7 and
+// 8-11 are the softmax of query tiles 0 and 1 and take registers that the first
+// four give up.  Value channels beyond 128 are
 // a second CTA's (the scores are formed again there).  Rows of the last key
 // tile that belong to no key of the sequence are zeroed in the V tile, since
 // 0 x NaN would reach the sum.  Waits are bounded; one that runs out leaves
@@ -44,7 +50,11 @@ namespace exlr8 {
 
 namespace {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
+// Registers a thread: 168 at launch, then 72 and 208, 128 * 72 + 256 * 208 of
+// the 384 * 168 that the block holds.
+constexpr int kFewRegisters = 72, kManyRegisters = 208;
+static_assert(128 * kFewRegisters + 256 * kManyRegisters <= 384 * 168, "more than the block holds");
 constexpr int kTileQ = 128;
 constexpr float kLift = 6.0f;       // weights are 2^6 of their share of the maximum
 constexpr float kLag = 8.0f;        // log2 by which a maximum may lag
@@ -82,6 +92,26 @@ __device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, int
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Two float32 in one register pair: sm_100 adds and multiplies both at once.
+__device__ __forceinline__ uint64_t both(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void apart(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
@@ -175,6 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
   if (warp == 0) {
     if (lane == 0 && all > 0) {
       bool ok = true;
@@ -293,6 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                               half_desc, kk > 0 || j > 0);
           }
           if (j + 1 >= n) tc_commit(&sh.o_done[q]);
+          if (q == 1 || j >= n1) tc_commit(&sh.empty[unit % kUnits]);  // the value tile's last use
         }
         __syncwarp();
         if (!next) {
@@ -303,14 +336,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok && j + 1 < n) scores(q, kt);
       }
-      if (ok && elect_one()) {
-        tc_commit(&sh.empty[unit % kUnits]);
-        if (more) tc_commit(&sh.empty[(unit + 1) % kUnits]);
-      }
+      if (ok && more && elect_one()) tc_commit(&sh.empty[(unit + 1) % kUnits]);
       __syncwarp();
     }
+  }
   } else {
-    const int q = (warp - 2) / 4, quad = warp & 3;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    const int q = (warp - 4) / 4, quad = warp & 3;
     const int row = first + q * kTileQ + quad * 32 + lane;
     const int seen = row < queries ? min(keys - queries + 1 + row, keys) : 0;
     const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
@@ -333,14 +365,51 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < kKeys; ++i)
           if (i >= left) s[i] = 0xff800000u;
       }
-      float top[4] = {m, m, m, m};
+      // The largest score of the row so far.
+      auto largest = [&]() {
+        float top[4] = {m, m, m, m};
 #pragma unroll
-      for (int i = 0; i < kKeys; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
-      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      // PV of tile j - 1 is complete: this tile's scores were committed after it.
-      if (j == 0) {
-        m = best;
-      } else if (__any_sync(0xffffffffu, (best - m) * c > kLag)) {
+        for (int i = 0; i < kKeys; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i]));
+        return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      };
+      // The weights of the tile against the present m, into tensor memory over
+      // the scores; their sum, and the largest exponent (before the lift).
+      float sum, grown;
+      auto weigh = [&]() {
+        const float base = m == -INFINITY ? 0.0f : kLift - m * c;
+        const uint64_t scale2 = both(c, c), base2 = both(base, base);
+        uint64_t part[2] = {0, 0};
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 32) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t xy =
+                fma2(both(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1])), scale2, base2);
+            float x, y, u, v;
+            apart(xy, x, y);
+            top[e & 1] = fmaxf(top[e & 1], fmaxf(x, y));
+            u = exp2_fast(x);
+            v = exp2_fast(y);
+            part[e & 1] = add2(part[e & 1], both(u, v));
+            p[e] = pack<kAct>(u, v);
+          }
+          tc_st16(ts + i / 2, p);
+        }
+        float s0, s1, s2, s3;
+        apart(part[0], s0, s1);
+        apart(part[1], s2, s3);
+        sum = (s0 + s1) + (s2 + s3);
+        grown = fmaxf(top[0], top[1]);
+      };
+      if (j == 0) m = largest();
+      weigh();
+      // Rarely a score has outgrown m: raise it, multiply what was summed, weigh
+      // the tile again.  PV of tile j - 1 is complete (this tile's scores were
+      // committed after it).
+      if (j > 0 && __any_sync(0xffffffffu, grown > kLift + kLag || (m == -INFINITY && grown > -INFINITY))) {
+        const float best = largest();
         const float keep = best > m ? exp2_fast((m - best) * c) : 1.0f;
         m = best;
         l *= keep;
@@ -354,23 +423,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
           tc_st32(to + i, o);
         }
+        weigh();
       }
-      const float base = m == -INFINITY ? 0.0f : kLift - m * c;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < kKeys; i += 32) {
-        uint32_t p[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float u = exp2_fast(fmaf(__uint_as_float(s[i + 2 * e]), c, base));
-          const float v = exp2_fast(fmaf(__uint_as_float(s[i + 2 * e + 1]), c, base));
-          sum[(2 * e) & 3] += u;
-          sum[(2 * e + 1) & 3] += v;
-          p[e] = pack<kAct>(u, v);
-        }
-        tc_st16(ts + i / 2, p);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += sum;
       tc_wait_st();
       tc_fence_before();
       mbar_arrive(&sh.p_ready[q]);
