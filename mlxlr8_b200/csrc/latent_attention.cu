@@ -621,15 +621,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kJoinWarps = 16;
 constexpr int kJoinShare = 4;   // CTAs per cut
 
-// A sequence is cut where a CTA's share begins inside it, and cut n of c cuts
-// joins every c-th row of it: blockIdx.x + 1 is that CTA, blockIdx.y one of the
-// four that divide its rows again.  A warp takes a row, 16 channels a lane;
-// with fewer rows than warps, the warps share a row's parts.
+// A sequence is cut where a CTA's share begins inside it, and its cuts divide
+// its rows among themselves: blockIdx.x + 1 is that CTA, blockIdx.y one of the
+// four that divide them again.  A warp takes a row, 16 channels a lane; with
+// more CTAs than rows, a CTA takes 128 channels of a row and its warps share
+// the parts.
 template <int kAct>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     latent_join_kernel(const LatentAttentionArgs a, const Work w, int kn, const float* __restrict__ parts,
                        const float2* __restrict__ sums, const Cut* __restrict__ cuts) {
-  __shared__ float4 s_o[kJoinWarps][kLatentMaxRank / 4];
+  __shared__ float4 s_o[kJoinWarps][32];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t cta = blockIdx.x + 1;
@@ -641,82 +642,86 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   const int first = static_cast<int>(owner_of(cut.start, cut.total, cut.sharers));
   const int last = static_cast<int>(owner_of(cut.start + cut.tiles - 1, cut.total, cut.sharers));
   const int slot0 = 2 * first + (first_tile(first, cut.total, cut.sharers) < cut.start ? 1 : 0);
-  auto slot_of = [&](int k) { return k == first ? slot0 : 2 * k; };
+  auto slot_of = [&](int k) { return k == 0 ? slot0 : 2 * (first + k); };
   const int rows = w.queries * w.heads, count = last - first + 1, vectors = a.rank / 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int workers = (count - 1) * kJoinShare;
   const int worker = (static_cast<int>(cta) - first - 1) * kJoinShare + blockIdx.y;
-  const bool shared = kn <= workers;
-  for (int i0 = worker; i0 < kn; i0 += workers * (shared ? 1 : kJoinWarps)) {
-    const int i = shared ? i0 : i0 + warp * workers;
-    const int row = cut.rt * kn + i;
-    const bool there = i < kn && row < rows;
-    // The largest unit and the sum, by every warp for itself.
-    float top = -INFINITY, sum = 0.0f;
-    float4 o[kLatentMaxRank / 128] = {};
-    if (there) {
-      for (int k = lane; k < count; k += 32) {
-        const float2 v = sums[slot_of(first + k) * kn + i];
-        if (v.y != 0.0f) top = fmaxf(top, v.x);
-      }
+  // The largest unit of a row's parts and their sum; the whole warp.
+  auto total = [&](int i, float& top, float& sum) {
+    top = -INFINITY;
+    sum = 0.0f;
+    for (int k = lane; k < count; k += 32) {
+      const float2 v = sums[slot_of(k) * kn + i];
+      if (v.y != 0.0f) top = fmaxf(top, v.x);
+    }
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      for (int k = lane; k < count; k += 32) {
-        const float2 v = sums[slot_of(first + k) * kn + i];
-        if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
-      }
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    for (int k = lane; k < count; k += 32) {
+      const float2 v = sums[slot_of(k) * kn + i];
+      if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
+    }
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  };
+  auto add = [](float4& o, const float4& p, float f) {
+    o.x = fmaf(p.x, f, o.x);
+    o.y = fmaf(p.y, f, o.y);
+    o.z = fmaf(p.z, f, o.z);
+    o.w = fmaf(p.w, f, o.w);
+  };
+  auto store = [&](int row, int vector, const float4& o, float inv) {
+    uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (cut.sequence * rows + row) * a.rank);
+    dst[32 * vector + lane] = make_uint2(pack<kAct>(o.x * inv, o.y * inv), pack<kAct>(o.z * inv, o.w * inv));
+  };
+  float top, sum;
+  if (kn > workers) {
+    for (int i = worker + warp * workers; i < kn; i += kJoinWarps * workers) {
+      const int row = cut.rt * kn + i;
+      if (row >= rows) break;
+      total(i, top, sum);
+      float4 o[kLatentMaxRank / 128] = {};
 #pragma unroll 4
-      for (int k = shared ? warp : 0; k < count; k += shared ? kJoinWarps : 1) {
-        const int at = slot_of(first + k) * kn + i;
+      for (int k = 0; k < count; ++k) {
+        const int at = slot_of(k) * kn + i;
         const float2 v = sums[at];
         const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
         const float4* part = reinterpret_cast<const float4*>(parts + static_cast<int64_t>(at) * a.rank) + lane;
 #pragma unroll
-        for (int e = 0; e < kLatentMaxRank / 128; ++e) {
-          if (e >= vectors) break;
-          const float4 p = part[32 * e];
-          o[e].x = fmaf(p.x, f, o[e].x);
-          o[e].y = fmaf(p.y, f, o[e].y);
-          o[e].z = fmaf(p.z, f, o[e].z);
-          o[e].w = fmaf(p.w, f, o[e].w);
-        }
+        for (int e = 0; e < kLatentMaxRank / 128; ++e)
+          if (e < vectors) add(o[e], part[32 * e], f);
       }
-    }
-    if (shared) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (a.lse && lane == 0)
+        a.lse[cut.sequence * rows + row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 #pragma unroll
       for (int e = 0; e < kLatentMaxRank / 128; ++e)
-        if (e < vectors) s_o[warp][32 * e + lane] = o[e];
-      __syncthreads();
-      // warp e adds up channels 128 e to 128 e + 127
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (warp < vectors) {
-#pragma unroll
-        for (int g = 0; g < kJoinWarps; ++g) {
-          const float4 p = s_o[g][32 * warp + lane];
-          v.x += p.x;
-          v.y += p.y;
-          v.z += p.z;
-          v.w += p.w;
-        }
-      }
-      __syncthreads();
-      if (warp >= vectors) continue;
-      o[0] = v;
+        if (e < vectors) store(row, e, o[e], inv);
     }
-    if (!there) continue;
-    const int64_t at = cut.sequence * rows + row;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (a.lse && lane == 0 && (!shared || warp == 0))
-      a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-    uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * a.rank) + lane;
-#pragma unroll
-    for (int e = 0; e < kLatentMaxRank / 128; ++e) {
-      if (e >= (shared ? 1 : vectors)) break;
-      dst[32 * (shared ? warp : e)] =
-          make_uint2(pack<kAct>(o[e].x * inv, o[e].y * inv), pack<kAct>(o[e].z * inv, o[e].w * inv));
+    return;
+  }
+  for (int unit = worker; unit < kn * vectors; unit += workers) {
+    const int i = unit / vectors, vector = unit % vectors, row = cut.rt * kn + i;
+    if (row >= rows) break;
+    total(i, top, sum);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int k = warp; k < count; k += kJoinWarps) {
+      const int at = slot_of(k) * kn + i;
+      const float2 v = sums[at];
+      add(o, *(reinterpret_cast<const float4*>(parts + static_cast<int64_t>(at) * a.rank) + 32 * vector + lane),
+          v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f);
     }
+    s_o[warp][lane] = o;
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int g = 1; g < kJoinWarps; ++g) add(o, s_o[g][lane], 1.0f);
+      store(row, vector, o, sum == 0.0f ? 0.0f : 1.0f / sum);
+      if (a.lse && lane == 0 && vector == 0)
+        a.lse[cut.sequence * rows + row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    }
+    __syncthreads();
   }
 }
 
