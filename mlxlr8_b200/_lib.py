@@ -226,7 +226,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_handle(device: torch.device) -> int:
     # The handle itself: a torch Stream object per call costs 2 us on the host.
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 _HERE = nullcontext()
