@@ -167,54 +167,73 @@ __global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024)
   }
 }
 
-// One CTA per row, any hidden size and alignment.
-template <int kAct>
+// One CTA per row, any hidden size and alignment.  kCached keeps h w of the row
+// in shared memory, so that the inputs are read once; rows beyond kCachedMax
+// channels read them again.
+constexpr int kCachedMax = 24 * 1024;  // two CTAs of 96 KB per SM
+
+template <int kAct, bool kCached>
 __global__ void __launch_bounds__(kThreads) residual_rms_q8_any_kernel(const void* __restrict__ x,
                                                                        const void* __restrict__ residual,
                                                                        const void* __restrict__ w, int hidden,
                                                                        int group, float eps, void* __restrict__ h_out,
                                                                        uint8_t* __restrict__ codes,
                                                                        float* __restrict__ scales) {
-  __shared__ float red[kThreads / 32];
+  extern __shared__ float cache[];
+  __shared__ float red[2][kThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t base = static_cast<int64_t>(blockIdx.x) * hidden;
-  auto value = [&](int i) {
+  auto sum_at = [&](int i) {
     const float h = load_act(x, kAct, base + i);
     return residual ? round_to(kAct, h + load_act(residual, kAct, base + i)) : h;
   };
-  float acc = 0.0f;
+  auto weighted = [&](int i) { return kCached ? cache[i] : sum_at(i) * load_act(w, kAct, i); };
+  float acc = 0.0f, row_top = 0.0f;
+#pragma unroll 4
   for (int i = threadIdx.x; i < hidden; i += kThreads) {
-    const float h = value(i);
+    const float h = sum_at(i), y = h * load_act(w, kAct, i);
+    if (kCached) cache[i] = y;
     if (h_out) store_act(h_out, kAct, base + i, h);
     acc = fmaf(h, h, acc);
+    row_top = max_nan(row_top, fabsf(y));
   }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-  if (lane == 0) red[warp] = acc;
+  for (int off = 16; off > 0; off >>= 1) {
+    acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    row_top = max_nan(row_top, __shfl_xor_sync(0xffffffffu, row_top, off));
+  }
+  if (lane == 0) {
+    red[0][warp] = acc;
+    red[1][warp] = row_top;
+  }
   __syncthreads();
-  acc = 0.0f;
-  for (int i = 0; i < kThreads / 32; ++i) acc += red[i];
+  acc = row_top = 0.0f;
+  for (int i = 0; i < kThreads / 32; ++i) {
+    acc += red[0][i];
+    row_top = max_nan(row_top, red[1][i]);
+  }
   const float inv = 1.0f / sqrtf(acc / static_cast<float>(hidden) + eps);
   const int groups = hidden / group;
-  // A warp takes whole groups; with one group a row every warp finds its
-  // maximum again.
+  // A warp takes whole groups; all threads share the one group of a row.
   for (int gi = groups == 1 ? 0 : warp; gi < groups; gi += kThreads / 32) {
-    float top = 0.0f;
-    for (int i = lane; i < group; i += 32)
-      top = max_nan(top, fabsf(value(gi * group + i) * inv * load_act(w, kAct, gi * group + i)));
+    float top = row_top;
+    if (groups > 1) {
+      top = 0.0f;
+      for (int i = lane; i < group; i += 32) top = max_nan(top, fabsf(weighted(gi * group + i)));
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const bool finite = top < __int_as_float(0x7f800000);
-    const float mul = finite && top > 0.0f ? 448.0f / top : 0.0f;
-    const int first = groups == 1 ? threadIdx.x : lane, step = groups == 1 ? kThreads : 32;
-    for (int i = first; i < group; i += step) {
-      const float y = value(gi * group + i) * inv * load_act(w, kAct, gi * group + i);
-      codes[base + gi * group + i] = finite ? to_e4m3(y * mul) : 0;
+      for (int off = 16; off > 0; off >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
     }
+    const float scale = top * inv / 448.0f;
+    const bool finite = top < __int_as_float(0x7f800000) && scale < __int_as_float(0x7f800000);
+    const float mul = scale > 0.0f && finite ? 448.0f / top : 0.0f;
+    const int first = groups == 1 ? threadIdx.x : lane, step = groups == 1 ? kThreads : 32;
+#pragma unroll 4
+    for (int i = gi * group + first; i < (gi + 1) * group; i += step)
+      codes[base + i] = finite ? to_e4m3(weighted(i) * mul) : 0;
     if (groups == 1 ? threadIdx.x == 0 : lane == 0)
-      scales[static_cast<int64_t>(blockIdx.x) * groups + gi] = finite ? top / 448.0f : __int_as_float(0x7fc00000);
+      scales[static_cast<int64_t>(blockIdx.x) * groups + gi] = finite ? scale : __int_as_float(0x7fc00000);
   }
 }
 
@@ -246,7 +265,14 @@ cudaError_t launch(const void* x, const void* residual, const void* w, int64_t r
     return launch_vectors<kAct, 2>(x, residual, w, rows, hidden, group, eps, h_out, codes, scales, s);
   if (vectors && !few && vecs <= 2048)
     return launch_vectors<kAct, 4>(x, residual, w, rows, hidden, group, eps, h_out, codes, scales, s);
-  return launch_pdl(residual_rms_q8_any_kernel<kAct>, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, s, x,
+  const dim3 grid(static_cast<unsigned>(rows));
+  if (hidden > kCachedMax)
+    return launch_pdl(residual_rms_q8_any_kernel<kAct, false>, grid, dim3(kThreads), 0, s, x, residual, w, hidden, group,
+                      eps, h_out, codes, scales);
+  static std::atomic<uint64_t> ready{0};
+  const cudaError_t err = allow_shared_memory(residual_rms_q8_any_kernel<kAct, true>, kCachedMax * 4, ready);
+  if (err != cudaSuccess) return err;
+  return launch_pdl(residual_rms_q8_any_kernel<kAct, true>, grid, dim3(kThreads), static_cast<size_t>(hidden) * 4, s, x,
                     residual, w, hidden, group, eps, h_out, codes, scales);
 }
 

@@ -47,6 +47,7 @@ def _check(x, w, residual, group, eps=1e-5):
 @pytest.mark.parametrize("rows, hidden, group", [
     (1, 6144, 128), (3, 6144, 64), (5, 256, 32), (2, 128, 128), (7, 1000, 1000), (2, 1, 1), (3, 33, 33),
     (4, 8192, 8192), (2, 20480, 128), (1, 20001, 20001), (300, 512, 64),
+    (2, 30001, 30001), (3, 33280, 128), (40, 4099, 4099),
 ])
 @pytest.mark.parametrize("with_residual", [False, True])
 def test_codes_and_scales_match_the_formula(dtype, rows, hidden, group, with_residual):
