@@ -590,7 +590,8 @@ int exlr8_residual_rms_norm_q8(const void* x, const void* residual, const void* 
                                int hidden, int group, float eps, void* h_out, uint8_t* codes, float* scales,
                                void* stream);
 
-/* ---- attention half of a decoder block ------------------------------------ */
+/* ---- attention half of a decoder block ------------------------------------
+ * No output of these calls may overlap an input. */
 
 /* Linear layer with 4-bit affine weights (the affine4 dense format of
  * exlr8/dense.py:19-67; MLX quantize(bits=4)): codes uint32 [out][in / 8], low
@@ -601,7 +602,8 @@ int exlr8_residual_rms_norm_q8(const void* x, const void* residual, const void* 
  * [rows][in / x_group] scales its codes (x_group 32, 64, 128 or in_features,
  * a divisor of in_features).  out [rows][out] in out_dtype.  x and codes
  * 16-byte aligned.  Sums are float32.  Made for decode: up to 16 rows share
- * one pass over the weights, more rows make more passes. */
+ * one pass over the weights, more rows (at most 2^19) make more passes.  An
+ * infinite channel of x gives NaN in its row, where w * x might be infinite. */
 int exlr8_affine4_linear(const void* x, int x_dtype, const float* x_scales, int x_group, int64_t rows,
                          int in_features, int out_features, const uint32_t* codes, const void* scales,
                          const void* biases, int scale_dtype, int group, void* out, int out_dtype, void* stream);
@@ -636,7 +638,9 @@ int exlr8_latent_append(const void* latent, int64_t latent_stride, const void* r
  * lengths[b] - queries + 1 + t of them, and gives zeros (lse -inf) when that
  * is none.  Rows past a length are never used, whatever they hold; table
  * entries outside [0, pages) hold no tokens; a length past the table's room
- * counts as that room.  lse (nullable) float32 [batch][queries][heads] is the
+ * counts as that room (table_width * page_size is at most 2^30).  A token that
+ * some query of the sequence sees has to be finite for all of them: a weight of
+ * zero times NaN is NaN.  lse (nullable) float32 [batch][queries][heads] is the
  * natural logarithm of the softmax's sum.  Every pointer 16-byte aligned.
  * Workspace: exlr8_latent_attention_workspace. */
 size_t exlr8_latent_attention_workspace(int64_t batch, int queries, int heads, int rank);
@@ -653,7 +657,9 @@ int exlr8_latent_attention(const void* q_latent, const void* q_rope, int64_t bat
  * Sequence s has the queries q_starts[s] .. q_starts[s + 1] and the keys
  * k_starts[s] .. k_starts[s + 1] (int32 [seqs + 1], ascending); with n queries
  * and m keys, query i sees the first m - n + 1 + i keys, and gives zeros (lse
- * -inf) when that is none.  out [total_q][heads][value] and lse (nullable,
+ * -inf) when that is none.  Keys and values that some query of the sequence
+ * sees have to be finite for all of them: a weight of zero times NaN is NaN.
+ * Starts outside the operands count as their ends.  out [total_q][heads][value] and lse (nullable,
  * float32 [total_q][heads]) are written for the rows of the sequences only.
  * 1 <= seqs <= 4096. */
 int exlr8_latent_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,

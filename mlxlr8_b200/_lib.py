@@ -260,6 +260,17 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def refuse_overlap(out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """``out`` (contiguous) may share no memory with an input."""
+    begin, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for t in inputs:
+        if t is None or t.numel() == 0:
+            continue
+        extent = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        if begin < t.data_ptr() + extent * t.element_size() and t.data_ptr() < end:
+            raise ValueError("out must not overlap an input")
+
+
 def act_code(t: torch.Tensor) -> int:
     try:
         return DTYPE_CODES[t.dtype]

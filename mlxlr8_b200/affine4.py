@@ -39,11 +39,11 @@ def affine4_linear(x, codes, scales, biases=None, *, x_scales=None, out_dtype=No
     """``x @ w.T`` for ``x [..., in]`` -> ``[..., out]``, summed in float32 and
     rounded once to ``out_dtype`` (x's; bfloat16 for E4M3 codes).
 
-    ``x_scales [..., in / g]`` (float32, ``g`` 32, 64, 128 or ``in``) belongs to
+    An infinite channel makes its row NaN.  ``x_scales [..., in / g]`` (float32, ``g`` 32, 64, 128 or ``in``) belongs to
     ``x`` of dtype float8_e4m3fn.  ``out`` (optional) receives the result."""
     device = _lib.require_cuda(x, codes, scales, biases, x_scales, out)
     in_features, out_features, group = _check_weights(codes, scales, biases)
-    if x.shape[-1] != in_features:
+    if x.dim() == 0 or x.shape[-1] != in_features:
         raise ValueError("activation width does not match in_features")
     lead = x.shape[:-1]
     x_group = in_features
@@ -64,6 +64,8 @@ def affine4_linear(x, codes, scales, biases=None, *, x_scales=None, out_dtype=No
         out = scales.new_empty(lead + (out_features,), dtype=dtype)
     elif out.shape != lead + (out_features,) or not out.is_contiguous() or out_dtype not in (None, out.dtype):
         raise ValueError("out must be a contiguous [..., out] tensor")
+    else:
+        _lib.refuse_overlap(out, x, codes, scales, biases, x_scales)
     x, codes, scales = _lib.aligned(x), _lib.aligned(codes), scales.contiguous()
     biases = biases.contiguous() if biases is not None else None
     with _lib.on_device(device):

@@ -274,11 +274,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int first = ((begin + block * kBlock) * kChunk >> group_shift) + scale_half * per;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) raw_s[e] = raw_b[e] = 0;
-    if (S::kPacked && a.scale_dtype == kF32) {
-    } else if (a.scale_dtype == kF32) {
+    if (a.scale_dtype == kF32) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
-        if (e >= per || first + e >= groups) continue;
+        if (S::kPacked || e >= per || first + e >= groups) continue;
         raw_s[e] = __ldg(static_cast<const uint32_t*>(a.scales) + scale_at + first + e);
         if (a.biases) raw_b[e] = __ldg(static_cast<const uint32_t*>(a.biases) + scale_at + first + e);
       }
@@ -301,20 +300,20 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int e = 0; e < kPer; ++e)
         if (e < per) dst[e * kRows] = raw_s[e] | raw_b[e] << 16;
     } else {
-    float2* dst = s_scale + buffer * S::kScales * kRows + scale_half * per * kRows + scale_row;
+      float2* dst = s_scale + buffer * S::kScales * kRows + scale_half * per * kRows + scale_row;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      if (e >= per) continue;
-      float v = __uint_as_float(raw_s[e]), b = __uint_as_float(raw_b[e]);
-      if (a.scale_dtype == kBF16) {
-        v = __uint_as_float(raw_s[e] << 16);
-        b = __uint_as_float(raw_b[e] << 16);
-      } else if (a.scale_dtype == kF16) {
-        v = __half2float(__ushort_as_half(static_cast<unsigned short>(raw_s[e])));
-        b = __half2float(__ushort_as_half(static_cast<unsigned short>(raw_b[e])));
+      for (int e = 0; e < kPer; ++e) {
+        if (e >= per) continue;
+        float v = __uint_as_float(raw_s[e]), b = __uint_as_float(raw_b[e]);
+        if (a.scale_dtype == kBF16) {
+          v = __uint_as_float(raw_s[e] << 16);
+          b = __uint_as_float(raw_b[e] << 16);
+        } else if (a.scale_dtype == kF16) {
+          v = __half2float(__ushort_as_half(static_cast<unsigned short>(raw_s[e])));
+          b = __half2float(__ushort_as_half(static_cast<unsigned short>(raw_b[e])));
+        }
+        dst[e * kRows] = make_float2(16.0f * v, a.biases ? b - 16.0f * v : -24.0f * v);
       }
-      dst[e * kRows] = make_float2(16.0f * v, a.biases ? b - 16.0f * v : -24.0f * v);
-    }
     }
     if (kX == kXE4M3 && threadIdx.x < S::kScales * S::kTokens)
       s_x[buffer * S::kScales * S::kTokens + threadIdx.x] = raw_x;
@@ -356,8 +355,10 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int p = 0; p < 2; ++p) {
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
-              const uint32_t av[4] = {code_pair<kHalf>(w[2 * m], 2 * p, mask, one), code_pair<kHalf>(w[2 * m + 1], 2 * p, mask, one),
-                                      code_pair<kHalf>(w[2 * m], 2 * p + 1, mask, one), code_pair<kHalf>(w[2 * m + 1], 2 * p + 1, mask, one)};
+              const uint32_t av[4] = {code_pair<kHalf>(w[2 * m], 2 * p, mask, one),
+                                      code_pair<kHalf>(w[2 * m + 1], 2 * p, mask, one),
+                                      code_pair<kHalf>(w[2 * m], 2 * p + 1, mask, one),
+                                      code_pair<kHalf>(w[2 * m + 1], 2 * p + 1, mask, one)};
 #pragma unroll
               for (int n = 0; n < kTiles; ++n)
 #pragma unroll

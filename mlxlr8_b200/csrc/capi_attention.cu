@@ -46,7 +46,7 @@ int exlr8_affine4_linear(const void* x, int x_dtype, const float* x_scales, int 
                          const void* biases, int scale_dtype, int group, void* out, int out_dtype, void* stream) {
   const bool q8 = x_dtype == EXLR8_DTYPE_E4M3;
   if ((!valid_act(x_dtype) && !q8) || !valid_act(scale_dtype) || !valid_act(out_dtype)) return EXLR8_ERR_DTYPE;
-  if (rows < 0 || rows > (1 << 20) || in_features <= 0 || in_features > (1 << 24) || out_features <= 0 ||
+  if (rows < 0 || rows > (1 << 19) || in_features <= 0 || in_features > (1 << 24) || out_features <= 0 ||
       out_features > (1 << 24))
     return EXLR8_ERR_SHAPE;
   if ((group != 32 && group != 64 && group != 128) || in_features % group) return EXLR8_ERR_SHAPE;
@@ -96,7 +96,7 @@ int exlr8_latent_attention(const void* q_latent, const void* q_rope, int64_t bat
   if (!half_type(dtype)) return EXLR8_ERR_DTYPE;
   const size_t need = exlr8_latent_attention_workspace(batch, queries, heads, rank);
   if (need == kBadSize || !pages_ok(pages, page_size) || table_width < 0 ||
-      static_cast<int64_t>(table_width) * page_size > kMaxGrid)
+      static_cast<int64_t>(table_width) * page_size > (1 << 30))
     return EXLR8_ERR_SHAPE;
   if (batch == 0) return EXLR8_OK;
   if (!q_latent || !q_rope || !lengths || !out || (table_width > 0 && !block_table) || (pages > 0 && !cache) ||

@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float unit = sh.m[i] * c - kLift;
         if (!whole) sums[slot * kN + i] = make_float2(unit, ok ? sum : NAN);
         else if (a.lse && row < rows)
-          a.lse[walk.b * rows + row] = sum == 0.0f ? -INFINITY : (unit + log2f(sum)) * 0.6931471805599453f;
+          a.lse[walk.b * rows + row] = !ok ? NAN : sum == 0.0f ? -INFINITY : (unit + log2f(sum)) * 0.6931471805599453f;
         sh.factor[i] = sum == 0.0f ? 0.0f : 1.0f / sum;
       }
       group_sync(bar);

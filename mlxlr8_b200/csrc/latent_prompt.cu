@@ -140,17 +140,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the sequences and taken from the last (its rows see the most keys).
   pdl_launch_dependents();
   pdl_wait();
+  auto start_of = [&](const int32_t* starts, int s, int64_t total) {
+    return min(max(starts[s], 0), static_cast<int>(total));
+  };
+  auto tiles_of = [&](int s) {
+    const int n = s < a.seqs ? start_of(a.q_starts, s + 1, a.total_q) - start_of(a.q_starts, s, a.total_q) : 0;
+    return (max(n, 0) + 255) / 256;
+  };
   if (warp == 0) {
     int total = 0;
-    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
-      const int s = s0 + lane;
-      int n = s < a.seqs ? (max(a.q_starts[s + 1] - a.q_starts[s], 0) + 255) / 256 : 0;
-      total += __reduce_add_sync(0xffffffffu, n);
-    }
+    for (int s0 = 0; s0 < a.seqs; s0 += 32) total += __reduce_add_sync(0xffffffffu, tiles_of(s0 + lane));
     int at = total - 1 - static_cast<int>(blockIdx.x / columns), found = -1, tile = 0;
     for (int s0 = 0; s0 < a.seqs && at >= 0 && found < 0; s0 += 32) {
-      const int s = s0 + lane;
-      const int n = s < a.seqs ? (max(a.q_starts[s + 1] - a.q_starts[s], 0) + 255) / 256 : 0;
+      const int n = tiles_of(s0 + lane);
       int end = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -184,10 +186,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (sh.seq < 0) return;
-  const int q0 = min(max(a.q_starts[sh.seq], 0), static_cast<int>(a.total_q));
-  const int queries = min(a.q_starts[sh.seq + 1], static_cast<int>(a.total_q)) - q0;
-  const int k0 = min(max(a.k_starts[sh.seq], 0), static_cast<int>(a.total_k));
-  const int keys = max(min(a.k_starts[sh.seq + 1], static_cast<int>(a.total_k)) - k0, 0);
+  const int q0 = start_of(a.q_starts, sh.seq, a.total_q);
+  const int queries = start_of(a.q_starts, sh.seq + 1, a.total_q) - q0;
+  const int k0 = start_of(a.k_starts, sh.seq, a.total_k);
+  const int keys = max(start_of(a.k_starts, sh.seq + 1, a.total_k) - k0, 0);
   const int first = sh.tile * 256;
   const int vb = min(2, a.value / 64 - 2 * part);  // 64-channel value blocks of this CTA
   // Key tiles of each query tile: its last query sees the most keys.
@@ -206,140 +208,140 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = sh.tmem;
 
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
-  if (warp == 0) {
-    if (lane == 0 && all > 0) {
-      bool ok = true;
-      mbar_arrive_expect_tx(&sh.q_full, 2 * T::kQ);
-      for (int q = 0; q < 2; ++q)
-        for (int b = 0; b < kBlocks; ++b)
-          load_tile(smem + q * T::kQ + b * 16384, &maps.q, maps.q_swap, 64 * b, head, q0 + first + q * kTileQ,
-                    &sh.q_full);
-      // Unit 2 j is key tile j, unit 2 j + 1 value tile j.  `used` blocks have been
-      // given out since the start, `freed` given back.
-      int unit = 0, gone = 0, used = 0, freed = 0, at = 0;
-      for (; unit < 2 * all && ok; ++unit) {
-        const int j = unit >> 1, n = unit & 1 ? vb : kBlocks;
-        while (ok && used + n - freed > T::kRing) {
-          ok = mbar_wait(&sh.empty[gone % kUnits], (gone / kUnits) & 1);
-          freed += gone & 1 ? vb : kBlocks;
-          ++gone;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    if (warp == 0) {
+      if (lane == 0 && all > 0) {
+        bool ok = true;
+        mbar_arrive_expect_tx(&sh.q_full, 2 * T::kQ);
+        for (int q = 0; q < 2; ++q)
+          for (int b = 0; b < kBlocks; ++b)
+            load_tile(smem + q * T::kQ + b * 16384, &maps.q, maps.q_swap, 64 * b, head, q0 + first + q * kTileQ,
+                      &sh.q_full);
+        // Unit 2 j is key tile j, unit 2 j + 1 value tile j.  `used` blocks have been
+        // given out since the start, `freed` given back.
+        int unit = 0, gone = 0, used = 0, freed = 0, at = 0;
+        for (; unit < 2 * all && ok; ++unit) {
+          const int j = unit >> 1, n = unit & 1 ? vb : kBlocks;
+          while (ok && used + n - freed > T::kRing) {
+            ok = mbar_wait(&sh.empty[gone % kUnits], (gone / kUnits) & 1);
+            freed += gone & 1 ? vb : kBlocks;
+            ++gone;
+          }
+          if (!ok) break;
+          uint64_t* full = &sh.full[unit % kUnits];
+          mbar_arrive_expect_tx(full, n * T::kBlock);
+          for (int b = 0; b < n; ++b) {
+            uint8_t* dst = ring + at * T::kBlock;
+            if (unit & 1) load_tile(dst, &maps.v, maps.v_swap, 128 * part + 64 * b, head, k0 + j * kKeys, full);
+            else if (b < kBlocks - 1) load_tile(dst, &maps.k, maps.k_swap, 64 * b, head, k0 + j * kKeys, full);
+            else tma_load_2d(dst, &maps.r, 0, k0 + j * kKeys, full);
+            if (++at == T::kRing) at = 0;
+          }
+          used += n;
         }
-        if (!ok) break;
-        uint64_t* full = &sh.full[unit % kUnits];
-        mbar_arrive_expect_tx(full, n * T::kBlock);
-        for (int b = 0; b < n; ++b) {
-          uint8_t* dst = ring + at * T::kBlock;
-          if (unit & 1) load_tile(dst, &maps.v, maps.v_swap, 128 * part + 64 * b, head, k0 + j * kKeys, full);
-          else if (b < kBlocks - 1) load_tile(dst, &maps.k, maps.k_swap, 64 * b, head, k0 + j * kKeys, full);
-          else tma_load_2d(dst, &maps.r, 0, k0 + j * kKeys, full);
+        // Copies still in flight land before the CTA's memory is given back.
+        mbar_wait(&sh.q_full, 0);
+        for (int u = max(0, unit - kUnits); u < unit; ++u) mbar_wait(&sh.full[u % kUnits], (u / kUnits) & 1);
+      }
+    } else if (warp == 1) {
+      const uint32_t score_desc = half_idesc(kAct == kBF16, kKeys, a.scale < 0.0f, false, false);
+      const uint32_t value_desc = half_idesc(kAct == kBF16, 64 * vb, false, false, true);
+      const uint32_t half_desc = half_idesc(kAct == kBF16, 64, false, false, true);
+      const uint32_t td = uniform(tmem), sq = uniform(desc_lo_sw128(smem_u32(smem))),
+                     sk = uniform(desc_lo_sw128(smem_u32(ring))),
+                     sv = uniform(desc_lo_rows128(smem_u32(ring), T::kBlock));
+      const int n0 = uniform(tiles[0]), n1 = uniform(tiles[1]), steps = max(n0, n1);
+      bool ok = steps == 0 || warp_wait(&sh.q_full, 0);
+      int at = 0;  // the block after the last tile's
+      // The blocks of the next tile, as low words of their descriptors.
+      auto blocks = [&](uint32_t base, int n, uint32_t* lo) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if (b >= n) break;
+          lo[b] = uniform(base + at * (T::kBlock >> 4));
           if (++at == T::kRing) at = 0;
         }
-        used += n;
-      }
-      // Copies still in flight land before the CTA's memory is given back.
-      mbar_wait(&sh.q_full, 0);
-      for (int u = max(0, unit - kUnits); u < unit; ++u) mbar_wait(&sh.full[u % kUnits], (u / kUnits) & 1);
-    }
-  } else if (warp == 1) {
-    const uint32_t score_desc = half_idesc(kAct == kBF16, kKeys, a.scale < 0.0f, false, false);
-    const uint32_t value_desc = half_idesc(kAct == kBF16, 64 * vb, false, false, true);
-    const uint32_t half_desc = half_idesc(kAct == kBF16, 64, false, false, true);
-    const uint32_t td = uniform(tmem), sq = uniform(desc_lo_sw128(smem_u32(smem))),
-                   sk = uniform(desc_lo_sw128(smem_u32(ring))),
-                   sv = uniform(desc_lo_rows128(smem_u32(ring), T::kBlock));
-    const int n0 = uniform(tiles[0]), n1 = uniform(tiles[1]), steps = max(n0, n1);
-    bool ok = steps == 0 || warp_wait(&sh.q_full, 0);
-    int at = 0;  // the block after the last tile's
-    // The blocks of the next tile, as low words of their descriptors.
-    auto blocks = [&](uint32_t base, int n, uint32_t* lo) {
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        if (b >= n) break;
-        lo[b] = uniform(base + at * (T::kBlock >> 4));
-        if (++at == T::kRing) at = 0;
-      }
-    };
-    // S_q of a key tile.
-    auto scores = [&](int q, const uint32_t* kt) {
-      const uint32_t qt = sq + q * (T::kQ >> 4);
-      if (elect_one()) {
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc_mma_f16(td + q * 128, desc_of(qt + ((b * 16384 + kk * 32) >> 4)), desc_of(kt[b] + (kk * 32 >> 4)),
-                       score_desc, (b | kk) != 0);
-        tc_commit(&sh.s_full[q]);
-      }
-      __syncwarp();
-    };
-    uint32_t kt[4], vt[4];
-    if (ok && steps > 0) ok = warp_wait(&sh.full[0], 0);
-    if (ok && steps > 0) {
-      tc_fence_after();
-      blocks(sk, kBlocks, kt);
-      if (n0 > 0) scores(0, kt);
-      if (n1 > 0) scores(1, kt);
-      if (elect_one()) tc_commit(&sh.empty[0]);
-      __syncwarp();
-    }
-    for (int j = 0; j < steps && ok; ++j) {
-      const int unit = 2 * j + 1;
-      ok = warp_wait(&sh.full[unit % kUnits], (unit / kUnits) & 1);
-      if (!ok) break;
-      const int first_block = at;
-      blocks(sv, vb, vt);
-      const int valid = uniform(keys) - j * kKeys;
-      if (valid < kKeys) {  // rows behind the sequence's last key
-        for (int b = 0; b < vb; ++b) {
-          uint8_t* tile = ring + (first_block + b < T::kRing ? first_block + b : first_block + b - T::kRing) * T::kBlock;
-          for (int i = lane; i < (kKeys - valid) * 8; i += 32)
-            reinterpret_cast<uint4*>(tile + valid * 128)[i] = make_uint4(0, 0, 0, 0);
-        }
-        fence_async_smem();
-        __syncwarp();
-      }
-      const bool joined = vb == 1 || first_block + 1 < T::kRing;  // the value blocks lie in a row
-      const bool more = j + 1 < steps;
-      bool next = !more;  // key tile j + 1 has arrived
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int n = q ? n1 : n0;
-        if (!ok || j >= n) continue;
-        ok = warp_wait(&sh.p_ready[q], j & 1);
-        if (!ok) continue;
-        tc_fence_after();
+      };
+      // S_q of a key tile.
+      auto scores = [&](int q, const uint32_t* kt) {
+        const uint32_t qt = sq + q * (T::kQ >> 4);
         if (elect_one()) {
-          if (joined) {
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-              tc_mma_f16_ts(td + 256 + q * 128, td + q * 128 + kk * 8, desc_of(vt[0] + (kk * 2048 >> 4)), value_desc,
-                            kk > 0 || j > 0);
-          } else {
+          for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-#pragma unroll
-              for (int b = 0; b < 2; ++b)
-                tc_mma_f16_ts(td + 256 + q * 128 + 64 * b, td + q * 128 + kk * 8, desc_of(vt[b] + (kk * 2048 >> 4)),
-                              half_desc, kk > 0 || j > 0);
-          }
-          if (j + 1 >= n) tc_commit(&sh.o_done[q]);
-          if (q == 1 || j >= n1) tc_commit(&sh.empty[unit % kUnits]);  // the value tile's last use
+            for (int kk = 0; kk < 4; ++kk)
+              tc_mma_f16(td + q * 128, desc_of(qt + ((b * 16384 + kk * 32) >> 4)), desc_of(kt[b] + (kk * 32 >> 4)),
+                         score_desc, (b | kk) != 0);
+          tc_commit(&sh.s_full[q]);
         }
         __syncwarp();
-        if (!next) {
-          ok = warp_wait(&sh.full[(unit + 1) % kUnits], ((unit + 1) / kUnits) & 1);
-          tc_fence_after();
-          blocks(sk, kBlocks, kt);
-          next = true;
-        }
-        if (ok && j + 1 < n) scores(q, kt);
+      };
+      uint32_t kt[4], vt[4];
+      if (ok && steps > 0) ok = warp_wait(&sh.full[0], 0);
+      if (ok && steps > 0) {
+        tc_fence_after();
+        blocks(sk, kBlocks, kt);
+        if (n0 > 0) scores(0, kt);
+        if (n1 > 0) scores(1, kt);
+        if (elect_one()) tc_commit(&sh.empty[0]);
+        __syncwarp();
       }
-      if (ok && more && elect_one()) tc_commit(&sh.empty[(unit + 1) % kUnits]);
-      __syncwarp();
+      for (int j = 0; j < steps && ok; ++j) {
+        const int unit = 2 * j + 1;
+        ok = warp_wait(&sh.full[unit % kUnits], (unit / kUnits) & 1);
+        if (!ok) break;
+        const int first_block = at;
+        blocks(sv, vb, vt);
+        const int valid = uniform(keys) - j * kKeys;
+        if (valid < kKeys) {  // rows behind the sequence's last key
+          for (int b = 0; b < vb; ++b) {
+            uint8_t* tile = ring + (first_block + b < T::kRing ? first_block + b : first_block + b - T::kRing) * T::kBlock;
+            for (int i = lane; i < (kKeys - valid) * 8; i += 32)
+              reinterpret_cast<uint4*>(tile + valid * 128)[i] = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+          __syncwarp();
+        }
+        const bool joined = vb == 1 || first_block + 1 < T::kRing;  // the value blocks lie in a row
+        const bool more = j + 1 < steps;
+        bool next = !more;  // key tile j + 1 has arrived
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int n = q ? n1 : n0;
+          if (!ok || j >= n) continue;
+          ok = warp_wait(&sh.p_ready[q], j & 1);
+          if (!ok) continue;
+          tc_fence_after();
+          if (elect_one()) {
+            if (joined) {
+#pragma unroll
+              for (int kk = 0; kk < kKeys / 16; ++kk)
+                tc_mma_f16_ts(td + 256 + q * 128, td + q * 128 + kk * 8, desc_of(vt[0] + (kk * 2048 >> 4)), value_desc,
+                              kk > 0 || j > 0);
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < kKeys / 16; ++kk)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                  tc_mma_f16_ts(td + 256 + q * 128 + 64 * b, td + q * 128 + kk * 8, desc_of(vt[b] + (kk * 2048 >> 4)),
+                                half_desc, kk > 0 || j > 0);
+            }
+            if (j + 1 >= n) tc_commit(&sh.o_done[q]);
+            if (q == 1 || j >= n1) tc_commit(&sh.empty[unit % kUnits]);  // the value tile's last use
+          }
+          __syncwarp();
+          if (!next) {
+            ok = warp_wait(&sh.full[(unit + 1) % kUnits], ((unit + 1) / kUnits) & 1);
+            tc_fence_after();
+            blocks(sk, kBlocks, kt);
+            next = true;
+          }
+          if (ok && j + 1 < n) scores(q, kt);
+        }
+        if (ok && more && elect_one()) tc_commit(&sh.empty[(unit + 1) % kUnits]);
+        __syncwarp();
+      }
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int q = (warp - 4) / 4, quad = warp & 3;
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool store = row < queries;
     const int64_t at = (static_cast<int64_t>(q0) + row) * a.heads + head;
     if (a.lse && part == 0 && store)
-      a.lse[at] = l > 0.0f ? (m * c - kLift + log2f(l)) * 0.6931471805599453f : (l == 0.0f ? -INFINITY : l);
+      a.lse[at] = !ok ? NAN : l > 0.0f ? (m * c - kLift + log2f(l)) * 0.6931471805599453f : (l == 0.0f ? -INFINITY : l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     for (int i = 0; i < 64 * vb; i += 32) {
       uint32_t o[32];

@@ -47,7 +47,8 @@ struct Eight {
   __device__ __forceinline__ void store(void* p, int64_t at) const {
     uint4* dst = reinterpret_cast<uint4*>(static_cast<char*>(p) + at * (kAct == kF32 ? 4 : 2));
 #pragma unroll
-    for (int i = 0; i < (kAct == kF32 ? 2 : 1); ++i) dst[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    for (int i = 0; i < (kAct == kF32 ? 2 : 1); ++i)
+      dst[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -267,8 +268,8 @@ cudaError_t launch(const void* x, const void* residual, const void* w, int64_t r
     return launch_vectors<kAct, 4>(x, residual, w, rows, hidden, group, eps, h_out, codes, scales, s);
   const dim3 grid(static_cast<unsigned>(rows));
   if (hidden > kCachedMax)
-    return launch_pdl(residual_rms_q8_any_kernel<kAct, false>, grid, dim3(kThreads), 0, s, x, residual, w, hidden, group,
-                      eps, h_out, codes, scales);
+    return launch_pdl(residual_rms_q8_any_kernel<kAct, false>, grid, dim3(kThreads), 0, s, x, residual, w, hidden,
+                      group, eps, h_out, codes, scales);
   static std::atomic<uint64_t> ready{0};
   const cudaError_t err = allow_shared_memory(residual_rms_q8_any_kernel<kAct, true>, kCachedMax * 4, ready);
   if (err != cudaSuccess) return err;

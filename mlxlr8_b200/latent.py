@@ -61,7 +61,8 @@ def latent_append(latent, rope_key, cache, slots, *, weight=None, eps: float = 1
     ``q_rope [tokens, heads, 64]`` where given, are rotated: channel pairs (2i, 2i
     + 1) when ``interleaved``, else (i, i + 32).  A slot outside the cache (-1
     for padding rows) writes nothing; so does a position outside the table,
-    whose rotated queries are NaN.  Returns the rotated queries (a new
+    whose rotated queries are NaN.  Two tokens with one slot leave either
+    entry.  Returns the rotated queries (a new
     tensor), or None."""
     device = _lib.require_cuda(latent, rope_key, cache, slots, weight, cos_sin, positions, q_rope)
     rank = _check_cache(cache)
@@ -110,7 +111,8 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
     Sequence ``b`` has ``lengths[b]`` (int32) tokens in the pages ``block_table[b]``
     (int32 [batch, width]); its last query sees all of them, an earlier one
     fewer by its distance from the last.  A query that sees none gives zeros.
-    Rows past a length are not used, whatever they hold.  With
+    Rows past a length are not used, whatever they hold; a row that is not
+    finite reaches every query of its sequence, earlier ones too.  With
     ``return_lse`` also float32 ``[batch, queries, heads]``, the logarithm of the
     softmax's sum (-inf where nothing was seen), by which results over parts
     of a context can be joined.  ``workspace`` (optional uint8 tensor) is used
@@ -135,6 +137,10 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
         out = torch.empty_like(q_latent)
     elif out.shape != q_latent.shape or out.dtype != cache.dtype or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous tensor like q_latent")
+    else:
+        _lib.refuse_overlap(out, q_latent, q_rope, cache, block_table, lengths)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
     lse = q_latent.new_empty((batch, queries, heads), dtype=torch.float32) if return_lse else None
     lib = _lib.lib()
     with _lib.on_device(device):
@@ -175,7 +181,8 @@ def latent_prompt_attention(q, k, k_rope, v, q_starts, k_starts, scale: float, *
     ``k_starts[s] : k_starts[s + 1]`` (int32 [seqs + 1], ascending); its last
     query sees all its keys, an earlier one fewer by its distance from the
     last, so a chunk with a history is one call.  A query that sees none gives
-    zeros.  Rows behind the last sequence are left as they were (in a new
+    zeros.  A key or value that is not finite reaches every query of its
+    sequence, earlier ones too.  Rows behind the last sequence are left as they were (in a new
     ``out``: undefined).  With ``return_lse`` also float32 ``[total_q, heads]``."""
     device = _lib.require_cuda(q, k, k_rope, v, q_starts, k_starts, out)
     _half("q", q)
@@ -201,6 +208,8 @@ def latent_prompt_attention(q, k, k_rope, v, q_starts, k_starts, scale: float, *
     elif tuple(out.shape) != (total_q, heads, value) or out.dtype != q.dtype or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous [total_q, heads, value] tensor")
+    else:
+        _lib.refuse_overlap(out, q, k, k_rope, v, q_starts, k_starts)
     lse = q.new_empty((total_q, heads), dtype=torch.float32) if return_lse else None
     with _lib.on_device(device):
         _lib.check(_lib.lib().exlr8_latent_prompt_attention(

@@ -57,6 +57,8 @@ def residual_rms_norm_q8(x, weight, eps: float = 1e-5, residual=None, group: int
     = max|y| / 448``.  A group of zeros has scale 0; a group with a value that
     is not finite has scale NaN and codes 0."""
     device = _lib.require_cuda(x, weight, residual)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("the norm needs a channel")
     hidden = x.shape[-1]
     if weight.shape != (hidden,):
         raise ValueError("norm weight must have one entry per hidden channel")

@@ -32,7 +32,7 @@ def _linear(x=P, x_dtype=2, xs=None, xg=0, rows=1, inner=256, outer=8, codes=P, 
 @pytest.mark.parametrize("change, status", [
     (dict(rows=0), 0), (dict(x_dtype=4), 8), (dict(sdt=3), 8), (dict(odt=3), 8), (dict(inner=0), 16),
     (dict(inner=224), 16), (dict(group=16), 16), (dict(group=256), 16), (dict(outer=0), 16), (dict(rows=-3), 16),
-    (dict(rows=(1 << 20) + 1), 16), (dict(x_dtype=3, xs=P, xg=96), 16), (dict(x_dtype=3, xs=P, xg=0), 16),
+    (dict(rows=(1 << 20) + 1), 16), (dict(rows=(1 << 19) + 1), 16), (dict(x_dtype=3, xs=P, xg=96), 16), (dict(x_dtype=3, xs=P, xg=0), 16),
     (dict(x_dtype=3, xg=128), 11), (dict(xs=P), 11), (dict(x=None), 11), (dict(codes=None), 11), (dict(out=None), 11),
     (dict(x=P + 8), 9), (dict(codes=P + 4), 9),
 ])
@@ -65,7 +65,7 @@ def _attend(ql=P, batch=1, queries=1, heads=8, rank=512, dtype=2, cache=P, pages
 @pytest.mark.parametrize("change, status", [
     (dict(batch=0), 0), (dict(dtype=0), 8), (dict(dtype=3), 8), (dict(rank=100), 16), (dict(queries=0), 16),
     (dict(heads=0), 16), (dict(page=20), 16), (dict(batch=-1), 16), (dict(batch=1 << 30), 16), (dict(width=-1), 16),
-    (dict(pages=1 << 40), 16), (dict(width=1 << 30), 16), (dict(queries=1 << 30, heads=1 << 16), 16),
+    (dict(pages=1 << 40), 16), (dict(width=1 << 30), 16), (dict(width=(1 << 26) + 1), 16), (dict(queries=1 << 30, heads=1 << 16), 16),
     (dict(ql=None), 11), (dict(table=None), 11), (dict(lengths=None), 11), (dict(cache=None), 11), (dict(out=None), 11),
     (dict(scale=float("inf")), 11), (dict(scale=float("nan")), 11), (dict(ql=P + 2), 9), (dict(cache=P + 8), 9),
 ])

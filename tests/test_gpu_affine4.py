@@ -189,6 +189,9 @@ def test_no_rows_and_refusals():
                  lambda: affine4_linear(x8, codes, scales, biases, x_scales=torch.ones(2, 16, device="cuda")),
                  lambda: affine4_linear(x.double(), codes, scales, biases),
                  lambda: affine4_linear(x, codes, scales, biases, out=torch.empty(2, 7, device="cuda")),
+                 lambda: affine4_linear(x, codes, scales, biases, out=x[:, :8].reshape(-1)[:0]),
+                 lambda: affine4_linear(x.view(-1)[:256], codes, scales, biases, out=x.view(-1)[100:108]),
+                 lambda: affine4_linear(x[0, 0], codes, scales, biases),
                  lambda: affine4_linear(x, codes, scales, biases, out_dtype=torch.int8),
                  lambda: affine4_linear(x, codes, scales.cpu(), biases),
                  lambda: Affine4Linear(codes, scales[:4])):

@@ -366,6 +366,11 @@ def test_absorbed_refusals():
                  lambda: latent_attention(ql[0], qr[0], cache, table, lengths, 1.0),
                  lambda: latent_attention(ql, qr, cache[..., :560], table, lengths, 1.0),
                  lambda: latent_attention(ql, qr, cache, table, lengths, 1.0, out=ql[..., :256]),
+                 lambda: latent_attention(ql, qr, cache, table, lengths, 1.0, out=ql),
+                 lambda: latent_attention(ql, qr, cache, table, lengths, 1.0,
+                                          out=cache.view(-1)[:8192].view(2, 1, 8, 512)),
+                 lambda: latent_attention(ql, qr, cache, table, lengths, 1.0,
+                                          workspace=torch.empty(1 << 26, 2, device="cuda", dtype=torch.uint8)[:, 0]),
                  lambda: latent_attention(ql, qr, cache, table.cpu(), lengths, 1.0)):
         with pytest.raises((ValueError, RuntimeError)):
             call()
@@ -518,7 +523,53 @@ def test_prompt_refusals():
                  lambda: latent_prompt_attention(q, k, kr, v, s[:1], s[:1], 1.0),
                  lambda: latent_prompt_attention(q.float(), k.float(), kr.float(), v.float(), s, s, 1.0),
                  lambda: latent_prompt_attention(q, k, kr, v, s, s, 1.0, out=q[..., :128]),
+                 lambda: latent_prompt_attention(q, k, kr, v, s, s, 1.0, out=v),
                  lambda: latent_prompt_attention(q, k, kr, v, s, s, float("inf")),
                  lambda: latent_prompt_attention(q, k, kr, v, s.cpu(), s, 1.0)):
         with pytest.raises((ValueError, RuntimeError)):
             call()
+
+
+def test_prompt_starts_outside_the_operands():
+    """Starts past either end count as that end; descending ones hold no query."""
+    import torch
+
+    from mlxlr8_b200.latent import latent_prompt_attention
+
+    g = torch.Generator(device="cuda").manual_seed(95)
+    q, k, kr, v = _operands(g, [300], [300], 2, 128, 128, torch.bfloat16)
+    low, high = -2 ** 31, 2 ** 31 - 1
+
+    def run(qs, ks):
+        qs, ks = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (qs, ks))
+        out = torch.full((300, 2, 128), 7.0, device="cuda").bfloat16()
+        return latent_prompt_attention(q, k, kr, v, qs, ks, 0.1, out=out)
+
+    whole = run([0, 300], [0, 300])
+    assert torch.equal(run([low, high], [low, high]), whole)
+    assert torch.equal(run([0, 300, high, low, -5, 0], [0, 300, high, low, low, 0]), whole)
+    assert bool((run([high, high], [0, 300]) == 7.0).all()) and bool((run([300, 0], [0, 300]) == 7.0).all())
+
+
+def test_absorbed_many_short_sequences():
+    """More sequences than CTAs, most of them empty or of one token."""
+    import torch
+
+    from mlxlr8_b200.latent import latent_attention
+
+    g = torch.Generator(device="cuda").manual_seed(96)
+    batch, heads, rank = 5003, 2, 128
+    cache = torch.randn(64, 16, rank + 64, generator=g, device="cuda").bfloat16()
+    ql, qr = (torch.randn(batch, 1, heads, n, generator=g, device="cuda").bfloat16() for n in (rank, 64))
+    table = torch.randint(0, 64, (batch, 2), generator=g, device="cuda", dtype=torch.int32)
+    lengths = torch.tensor([0, 1, 0, 17, 1], device="cuda", dtype=torch.int32).repeat(1001)[:batch]
+    lengths[-1] = 32
+    got = latent_attention(ql, qr, cache, table, lengths, 0.1)
+    rows = cache[table.long()].view(batch, 32, rank + 64).double()
+    s = torch.einsum("bhd,bnd->bhn", torch.cat([ql, qr], -1)[:, 0].double(), rows) * 0.1
+    mask = torch.arange(32, device="cuda") < lengths[:, None]
+    p = torch.softmax(s.masked_fill(~mask[:, None], -1e300), -1) * (lengths > 0)[:, None, None]
+    rows = rows[..., :rank]
+    half = 2.0 ** -8  # rounded weights, rounded output; scores and sums in float32 are far below
+    expected, weight = (torch.einsum("bhn,bnd->bhd", p, r) for r in (rows, rows.abs()))
+    _close(got[:, 0], expected, 1.02 * half * (weight + expected.abs()) + 2.0 ** -25)

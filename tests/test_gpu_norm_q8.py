@@ -115,6 +115,9 @@ def test_no_rows_and_refusals():
             residual_rms_norm_q8(x, w, **bad)
     with pytest.raises(ValueError, match="one entry per hidden channel"):
         residual_rms_norm_q8(x, w[:-1])
+    for none in (x[:, :0], x[0, 0]):
+        with pytest.raises(ValueError, match="needs a channel"):
+            residual_rms_norm_q8(none, w[:0])
     with pytest.raises(ValueError, match="dtype"):
         residual_rms_norm_q8(x.double(), w)
     with pytest.raises(ValueError, match="CUDA"):
