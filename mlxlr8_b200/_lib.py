@@ -205,19 +205,24 @@ def check(status: int) -> None:
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
     """All operands must live on one CUDA device; there is no CPU path."""
-    if not torch.cuda.is_available():
-        raise RuntimeError("the exlr8 B200 operators need a CUDA device (no CPU fallback)")
     first = index = None
     for t in tensors:
-        if t is None:
+        if t is None or t.get_device() == index:
             continue
         if not t.is_cuda:
+            if not torch.cuda.is_available():
+                break
             raise ValueError("exlr8 B200 operators take CUDA tensors")
-        if first is None:
-            first, index = t, t.get_device()
-        elif t.get_device() != index:
+        if first is not None:
             raise ValueError("operands are on different devices")
-    return first.device if first is not None else torch.device("cuda", torch.cuda.current_device())
+        first, index = t, t.get_device()
+    else:
+        if first is not None:
+            return first.device
+    # (asked here only: it takes as long as the checks of six operands)
+    if not torch.cuda.is_available():
+        raise RuntimeError("the exlr8 B200 operators need a CUDA device (no CPU fallback)")
+    return torch.device("cuda", torch.cuda.current_device())
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -236,7 +241,7 @@ _HERE = nullcontext()
 def on_device(device: torch.device):
     """Context in which ``device`` is current: a launch on another device's
     stream than the current one's would fail."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def host_device_pointer(t: torch.Tensor) -> int:

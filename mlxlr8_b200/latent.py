@@ -14,6 +14,7 @@ values (prompts).  ``LatentPages`` hands out pages, and
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -30,14 +31,24 @@ def _half(name, t, dtype=None):
 
 
 def _check_cache(cache):
-    if cache.dim() != 3 or cache.shape[2] - ROPE not in (128, 256, 384, 512):
+    """(pages, page size, rank) of a cache."""
+    shape = cache.shape
+    if len(shape) != 3 or shape[2] - ROPE not in (128, 256, 384, 512):
         raise ValueError("the cache is [pages, page_size, rank + 64] with rank 128, 256, 384 or 512")
-    if cache.shape[1] == 0 or cache.shape[1] % 16:
+    pages, size, width = shape
+    if size == 0 or size % 16:
         raise ValueError("the page size must be a multiple of 16")
     if not cache.is_contiguous():
         raise ValueError("the cache must be contiguous")
     _half("the cache", cache)
-    return cache.shape[2] - ROPE
+    return pages, size, width - ROPE
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(device_index, queries, heads, rank):
+    """Of one call, whatever its batch."""
+    with torch.cuda.device(device_index):
+        return _lib.lib().exlr8_latent_attention_workspace(1, queries, heads, rank)
 
 
 def _index(name, t, shape, dtype):
@@ -65,39 +76,41 @@ def latent_append(latent, rope_key, cache, slots, *, weight=None, eps: float = 1
     entry.  Returns the rotated queries (a new
     tensor), or None."""
     device = _lib.require_cuda(latent, rope_key, cache, slots, weight, cos_sin, positions, q_rope)
-    rank = _check_cache(cache)
-    if latent.dim() != 2 or latent.shape[1] != rank or tuple(rope_key.shape) != (latent.shape[0], ROPE):
-        raise ValueError("latent must be [tokens, rank] and rope_key [tokens, 64]")
-    tokens = latent.shape[0]
-    _half("latent", latent, cache.dtype)
-    _half("rope_key", rope_key, cache.dtype)
+    pages, page_size, rank = _check_cache(cache)
+    dtype = cache.dtype
+    tokens = slots.numel()
+    if latent.shape != (tokens, rank) or rope_key.shape != (tokens, ROPE):
+        raise ValueError("latent must be [tokens, rank] and rope_key [tokens, 64], with a slot a token")
+    _half("latent", latent, dtype)
+    _half("rope_key", rope_key, dtype)
     slots = _index("slots", slots, (tokens,), torch.int64)
     if weight is not None:
-        if tuple(weight.shape) != (rank,):
+        if weight.shape != (rank,):
             raise ValueError("the latent norm's weight must have one entry per latent channel")
-        weight = _lib.like(weight, cache.dtype)
+        weight = _lib.like(weight, dtype)
     if (cos_sin is None) != (positions is None):
         raise ValueError("cos_sin and positions go together")
     if cos_sin is not None:
-        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 3 or tuple(cos_sin.shape[1:]) != (ROPE // 2, 2):
+        if cos_sin.dtype != torch.float32 or cos_sin.shape != (len(cos_sin), ROPE // 2, 2):
             raise ValueError("cos_sin must be float32 [positions, 32, 2]")
         cos_sin = _lib.aligned(cos_sin)
         positions = _index("positions", positions, (tokens,), torch.int32)
     latent, rope_key = _rows(latent), _rows(rope_key)
     q_out, heads, q_strides = None, 0, (0, 0)
     if q_rope is not None:
-        if q_rope.dim() != 3 or q_rope.shape[0] != tokens or q_rope.shape[1] == 0 or q_rope.shape[2] != ROPE:
+        heads = q_rope.shape[1] if q_rope.dim() == 3 else 0
+        if heads == 0 or q_rope.shape != (tokens, heads, ROPE):
             raise ValueError("q_rope must be [tokens, heads, 64]")
-        _half("q_rope", q_rope, cache.dtype)
-        q_rope, heads = _rows(q_rope), q_rope.shape[1]
+        _half("q_rope", q_rope, dtype)
+        q_rope = _rows(q_rope)
         q_strides = q_rope.stride()[:2]
-        q_out = cache.new_empty((tokens, heads, ROPE))
+        q_out = torch.empty_like(q_rope, memory_format=torch.contiguous_format)
     with _lib.on_device(device):
         _lib.check(_lib.lib().exlr8_latent_append(
             latent.data_ptr(), latent.stride(0), rope_key.data_ptr(), rope_key.stride(0), tokens, rank,
             _lib.act_code(cache), _lib.ptr(weight), float(eps), _lib.ptr(cos_sin),
             0 if cos_sin is None else cos_sin.shape[0], _lib.ptr(positions), int(interleaved), slots.data_ptr(),
-            cache.data_ptr(), cache.shape[0], cache.shape[1], _lib.ptr(q_rope), *q_strides, heads, _lib.ptr(q_out),
+            cache.data_ptr(), pages, page_size, _lib.ptr(q_rope), *q_strides, heads, _lib.ptr(q_out),
             _lib.stream_handle(device)))
     return q_out
 
@@ -118,17 +131,18 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
     of a context can be joined.  ``workspace`` (optional uint8 tensor) is used
     when it is large enough; calls that overlap need one each."""
     device = _lib.require_cuda(q_latent, q_rope, cache, block_table, lengths, out, workspace)
-    rank = _check_cache(cache)
-    if q_latent.dim() != 4 or q_latent.shape[3] != rank or q_rope.shape != q_latent.shape[:3] + (ROPE,):
+    pages, page_size, rank = _check_cache(cache)
+    batch, queries, heads, width = q_latent.shape if q_latent.dim() == 4 else (0, 0, 0, 0)
+    if width != rank or q_rope.shape != (batch, queries, heads, ROPE):
         raise ValueError("q_latent must be [batch, queries, heads, rank] and q_rope [batch, queries, heads, 64]")
     _half("q_latent", q_latent, cache.dtype)
     _half("q_rope", q_rope, cache.dtype)
-    batch, queries, heads, _ = q_latent.shape
     if queries == 0 or heads == 0:
         raise ValueError("latent attention needs a query and a head")
     if block_table.dim() != 2:
         raise ValueError("block_table must be int32 [batch, pages]")
-    block_table = _index("block_table", block_table, (batch, block_table.shape[1]), torch.int32)
+    table_width = block_table.shape[1]
+    block_table = _index("block_table", block_table, (batch, table_width), torch.int32)
     lengths = _index("lengths", lengths, (batch,), torch.int32)
     q_latent, q_rope = _lib.aligned(q_latent), _lib.aligned(q_rope)
     if cache.data_ptr() % 16:
@@ -142,18 +156,16 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("the workspace must be contiguous")
     lse = q_latent.new_empty((batch, queries, heads), dtype=torch.float32) if return_lse else None
-    lib = _lib.lib()
+    need = _workspace_bytes(device.index, queries, heads, rank)
+    if need >= 1 << 62:
+        raise ValueError("operand sizes or strides are outside what the operator takes")
+    if workspace is None or workspace.nbytes < need:
+        workspace = q_latent.new_empty(need, dtype=torch.uint8)
     with _lib.on_device(device):
-        need = lib.exlr8_latent_attention_workspace(batch, queries, heads, rank)
-        if need >= 1 << 62:
-            raise ValueError("operand sizes or strides are outside what the operator takes")
-        if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = _lib.workspace(need, device)
-        _lib.check(lib.exlr8_latent_attention(
+        _lib.check(_lib.lib().exlr8_latent_attention(
             q_latent.data_ptr(), q_rope.data_ptr(), batch, queries, heads, rank, _lib.act_code(cache), cache.data_ptr(),
-            cache.shape[0], cache.shape[1], block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
-            float(scale), out.data_ptr(), _lib.ptr(lse), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _lib.stream_handle(device)))
+            pages, page_size, block_table.data_ptr(), table_width, lengths.data_ptr(), float(scale), out.data_ptr(),
+            _lib.ptr(lse), workspace.data_ptr(), workspace.nbytes, _lib.stream_handle(device)))
     return (out, lse) if return_lse else out
 
 
@@ -189,11 +201,12 @@ def latent_prompt_attention(q, k, k_rope, v, q_starts, k_starts, scale: float, *
     q, k, v = (_heads_first(name, t, q.dtype) for name, t in (("q", q), ("k", k), ("v", v)))
     _half("k_rope", k_rope, q.dtype)
     total_q, heads, width = q.shape
-    total_k, nope, value = k.shape[0], k.shape[2], v.shape[2]
+    total_k, _, nope = k.shape
+    value = v.shape[2]
     if nope not in (64, 128, 192) or value not in (64, 128, 192, 256):
         raise ValueError("keys have 64, 128 or 192 channels beside the rotary ones, values 64, 128, 192 or 256")
-    if width != nope + ROPE or heads == 0 or tuple(k.shape[:2]) != (total_k, heads) \
-            or tuple(v.shape[:2]) != (total_k, heads) or tuple(k_rope.shape) != (total_k, ROPE):
+    if width != nope + ROPE or heads == 0 or k.shape != (total_k, heads, nope) \
+            or v.shape != (total_k, heads, value) or k_rope.shape != (total_k, ROPE):
         raise ValueError("q, k, k_rope and v do not match")
     if k_rope.stride(1) != 1 or k_rope.stride(0) % 8 or (k_rope.stride(0) == 0 and total_k > 1) \
             or k_rope.data_ptr() % 16:
@@ -205,7 +218,7 @@ def latent_prompt_attention(q, k, k_rope, v, q_starts, k_starts, scale: float, *
     k_starts = _index("k_starts", k_starts, (seqs + 1,), torch.int32)
     if out is None:
         out = q.new_empty((total_q, heads, value))
-    elif tuple(out.shape) != (total_q, heads, value) or out.dtype != q.dtype or not out.is_contiguous() \
+    elif out.shape != (total_q, heads, value) or out.dtype != q.dtype or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous [total_q, heads, value] tensor")
     else:
@@ -302,8 +315,8 @@ class LatentSelfAttention:
 
     def __init__(self, input_norm, query_latent, query_rope, key, key_norm, output, cache, heads, scale, cos_sin,
                  eps: float = 1e-5, group: int = 128, interleaved: bool = True):
-        self.rank = _check_cache(cache)
-        if heads < 1 or tuple(key_norm.shape) != (self.rank,):
+        self.rank = _check_cache(cache)[2]
+        if heads < 1 or key_norm.shape != (self.rank,):
             raise ValueError("the latent norm's weight must have one entry per latent channel")
         self.input_norm, self.key_norm = input_norm, key_norm.to(cache.dtype)
         self.query_latent, self.query_rope, self.key, self.output = query_latent, query_rope, key, output

@@ -57,12 +57,13 @@ def residual_rms_norm_q8(x, weight, eps: float = 1e-5, residual=None, group: int
     = max|y| / 448``.  A group of zeros has scale 0; a group with a value that
     is not finite has scale NaN and codes 0."""
     device = _lib.require_cuda(x, weight, residual)
-    if x.dim() == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("the norm needs a channel")
-    hidden = x.shape[-1]
+    hidden = shape[-1]
     if weight.shape != (hidden,):
         raise ValueError("norm weight must have one entry per hidden channel")
-    if residual is not None and residual.shape != x.shape:
+    if residual is not None and residual.shape != shape:
         raise ValueError("the residual must have the shape of x")
     if group != hidden and (group not in (32, 64, 128) or hidden % group):
         raise ValueError("group must be 32, 64, 128 or the row's width, and divide it")
@@ -70,7 +71,7 @@ def residual_rms_norm_q8(x, weight, eps: float = 1e-5, residual=None, group: int
     x = x.contiguous()
     w, res = _lib.like(weight, x.dtype), _lib.like(residual, x.dtype)
     codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-    scales = x.new_empty(x.shape[:-1] + (hidden // group,), dtype=torch.float32)
+    scales = x.new_empty((*shape[:-1], hidden // group), dtype=torch.float32)
     h = torch.empty_like(x) if return_sum else None
     with _lib.on_device(device):
         _lib.check(_lib.lib().exlr8_residual_rms_norm_q8(x.data_ptr(), _lib.ptr(res), w.data_ptr(), code,
