@@ -231,8 +231,9 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&v
   else tc_st8(taddr, v);
 }
 
-// parts: [2 * CTAs][kN][rank] float32, sums: [2 * CTAs][kN] pairs (log2 of the
-// unit of O and the sum, the sum).
+// A CTA leaves two parts at most: slot i holds that of CTA i's first segment,
+// slot CTAs + i that of its last.  parts: [2 * CTAs][kN][rank] float32, sums:
+// [kN][2 * CTAs] pairs (log2 of the unit of O and the sum, the sum).
 template <int kAct, int kN>
 __global__ void __launch_bounds__(kThreads, 1)
     latent_attention_kernel(const __grid_constant__ Maps maps, const LatentAttentionArgs a, const Work w, const Layout lay,
@@ -571,12 +572,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       group_sync(bar);
       const bool whole = walk.begin == 0 && walk.end == walk.tiles;
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (segment > 0);
+      const int64_t slot = blockIdx.x + (segment > 0 ? gridDim.x : 0);
       if (quad == 0 && lane < kCols) {
         const int i = col0 + lane, row = walk.rt * kN + i;
         const float sum = (sh.top[0][i] + sh.top[1][i]) + (sh.top[2][i] + sh.top[3][i]);
         const float unit = sh.m[i] * c - kLift;
-        if (!whole) sums[slot * kN + i] = make_float2(unit, ok ? sum : NAN);
+        if (!whole) sums[i * 2 * gridDim.x + slot] = make_float2(unit, ok ? sum : NAN);
         else if (a.lse && row < rows)
           a.lse[walk.b * rows + row] = !ok ? NAN : sum == 0.0f ? -INFINITY : (unit + log2f(sum)) * 0.6931471805599453f;
         sh.factor[i] = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -641,8 +642,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   // else in the second.
   const int first = static_cast<int>(owner_of(cut.start, cut.total, cut.sharers));
   const int last = static_cast<int>(owner_of(cut.start + cut.tiles - 1, cut.total, cut.sharers));
-  const int slot0 = 2 * first + (first_tile(first, cut.total, cut.sharers) < cut.start ? 1 : 0);
-  auto slot_of = [&](int k) { return k == 0 ? slot0 : 2 * (first + k); };
+  const int ctas = gridDim.x + 1;
+  const int slot0 = first + (first_tile(first, cut.total, cut.sharers) < cut.start ? ctas : 0);
+  auto slot_of = [&](int k) { return k == 0 ? slot0 : first + k; };
   const int rows = w.queries * w.heads, count = last - first + 1, vectors = a.rank / 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int workers = (count - 1) * kJoinShare;
@@ -652,13 +654,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     top = -INFINITY;
     sum = 0.0f;
     for (int k = lane; k < count; k += 32) {
-      const float2 v = sums[slot_of(k) * kn + i];
+      const float2 v = sums[i * 2 * ctas + slot_of(k)];
       if (v.y != 0.0f) top = fmaxf(top, v.x);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     for (int k = lane; k < count; k += 32) {
-      const float2 v = sums[slot_of(k) * kn + i];
+      const float2 v = sums[i * 2 * ctas + slot_of(k)];
       if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
     }
 #pragma unroll
@@ -684,7 +686,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 #pragma unroll 4
       for (int k = 0; k < count; ++k) {
         const int at = slot_of(k) * kn + i;
-        const float2 v = sums[at];
+        const float2 v = sums[i * 2 * ctas + slot_of(k)];
         const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
         const float4* part = reinterpret_cast<const float4*>(parts + static_cast<int64_t>(at) * a.rank) + lane;
 #pragma unroll
@@ -708,7 +710,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
 #pragma unroll 8
     for (int k = warp; k < count; k += kJoinWarps) {
       const int at = slot_of(k) * kn + i;
-      const float2 v = sums[at];
+      const float2 v = sums[i * 2 * ctas + slot_of(k)];
       add(o, *(reinterpret_cast<const float4*>(parts + static_cast<int64_t>(at) * a.rank) + 32 * vector + lane),
           v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f);
     }
