@@ -231,6 +231,26 @@ __device__ __forceinline__ void store_columns(uint32_t taddr, const uint32_t (&v
   else tc_st8(taddr, v);
 }
 
+// Value `own` of the 16 lanes of a half warp folded together, own = lane % 16 /
+// (16 / kN): every step halves the values a lane holds.
+template <int kN, class F>
+__device__ __forceinline__ float fold(const float (&v)[kN], int lane, F f) {
+  float t[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) t[i] = v[i];
+#pragma unroll
+  for (int m = kN / 2, off = 8; off > 0; m /= 2, off /= 2) {
+    const bool up = lane & off;
+    if (m == 0) t[0] = f(t[0], __shfl_xor_sync(0xffffffffu, t[0], off));
+#pragma unroll
+    for (int i = 0; i < m; ++i) {
+      const float other = __shfl_xor_sync(0xffffffffu, up ? t[i] : t[i + m], off);
+      t[i] = f(up ? t[i + m] : t[i], other);
+    }
+  }
+  return t[0];
+}
+
 // A CTA leaves two parts at most: slot i holds that of CTA i's first segment,
 // slot CTAs + i that of its last.  parts: [2 * CTAs][kN][rank] float32, sums:
 // [kN][2 * CTAs] pairs (log2 of the unit of O and the sum, the sum).
@@ -433,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kCols = kN / 2;
     // Tensor memory has a quarter's 16 tokens in lanes 0 to 15; lanes 16 to 31
     // take half of their rows over, so that lane i has token i % 16 and kOwn rows.
-    constexpr int kOwn = kCols / 2;
+    constexpr int kOwn = kCols / 2, kShare = 16 / kOwn;
     const int half = (warp - 4) / 4, quad = warp & 3, bar = 1 + half;
     const int token_row = quad * 16 + (lane & 15), col0 = half * kCols, own0 = col0 + (lane >> 4) * kOwn;
     const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
@@ -479,11 +499,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && u > 1) ok = mbar_wait(&sh.p_done[r], ((u >> 1) - 1) & 1);
         if (!held && ok) {
           // the two lanes of a token zero half of this half's blocks each
+          // (in an order that spreads a warp's tokens over the banks)
           uint8_t* tile = smem + lay.ring + place.stage * tile_pairs * kPair + token_row * 128;
           for (int i = half * blocks / 2; i < (half + 1) * blocks / 2; ++i) {
             uint4* line = reinterpret_cast<uint4*>(tile + i * kBlock) + (lane >> 4) * 4;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) line[e] = make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < 4; ++e) line[e ^ (token_row & 3)] = make_uint4(0, 0, 0, 0);
           }
         }
         if (__any_sync(0xffffffffu, !held || token >= least)) {
@@ -501,13 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kOwn; ++i) grown = fmaxf(grown, fmaf(s[i], c, base[i]));
         if (group_any(bar, grown > kLift + kLag)) {
-#pragma unroll
-          for (int i = 0; i < kOwn; ++i) {
-            float top = s[i];
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            if ((lane & 15) == i) sh.top[quad][own0 + i] = top;
-          }
+          const float best = fold(s, lane, [](float a, float b) { return fmaxf(a, b); });
+          if (lane % kShare == 0) sh.top[quad][own0 + lane % 16 / kShare] = best;
           group_sync(bar);
           if (quad == 0 && lane < kCols) {
             const int i = col0 + lane;
@@ -564,12 +580,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&sh.p_ready[r]);
       }
       // The segment's sums over the tokens, then its output.
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
-        if ((lane & 15) == i) sh.top[quad][own0 + i] = l[i];
-      }
+      const float row_sum = fold(l, lane, [](float a, float b) { return a + b; });
+      if (lane % kShare == 0) sh.top[quad][own0 + lane % 16 / kShare] = row_sum;
       group_sync(bar);
       const bool whole = walk.begin == 0 && walk.end == walk.tiles;
       const int64_t slot = blockIdx.x + (segment > 0 ? gridDim.x : 0);
@@ -600,12 +612,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < kCols; ++i, dst += a.rank) *dst = __uint_as_float(o[i]);
         } else {
-          const int row = walk.rt * kN + col0;
-          const int64_t first = (walk.b * rows + row) * a.rank + channel;
+          // Four lanes trade their channels of four rows, so that each stores four
+          // channels of one (single channels took 8000 cycles at 64 x 512).
+          const int row = walk.rt * kN + col0 + (lane & 3);
+          uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (walk.b * rows + row) * a.rank +
+                                                (channel & ~3));
 #pragma unroll
-          for (int i = 0; i < kCols; ++i)
-            if (row + i < rows)
-              store_act(a.out, kAct, first + static_cast<int64_t>(i) * a.rank, __uint_as_float(o[i]) * sh.factor[col0 + i]);
+          for (int i = 0; i < kCols; i += 4, dst += a.rank) {
+            const float4 f = *reinterpret_cast<const float4*>(&sh.factor[col0 + i]);
+            const uint32_t two[2] = {pack<kAct>(__uint_as_float(o[i]) * f.x, __uint_as_float(o[i + 1]) * f.y),
+                                     pack<kAct>(__uint_as_float(o[i + 2]) * f.z, __uint_as_float(o[i + 3]) * f.w)};
+            uint32_t w[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // channels c, c + 1 of row 2 e + lane % 2
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, two[e], 1);
+              w[e] = lane & 1 ? __byte_perm(other, two[e], 0x7632) : __byte_perm(two[e], other, 0x5410);
+            }
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 2 ? w[0] : w[1], 2);
+            if (row + i < rows) *dst = lane & 2 ? make_uint2(other, w[1]) : make_uint2(w[0], other);
+          }
         }
       }
       group_sync(bar);  // the shared rows are free for the next segment
