@@ -56,7 +56,6 @@ constexpr uint32_t kBlock = kTile * 128;  // 64 tokens x 64 channels
 constexpr uint32_t kPair = 2 * kBlock;
 constexpr int kMaxStages = 4;       // tiles in the ring
 constexpr int kMaxPairs = 4 * kMaxStages;
-constexpr int kMinTiles = 2;        // tiles a CTA takes at least, where there are as many
 constexpr uint32_t kSmem = 232448;  // all of a CTA's shared memory
 
 // ---- the flat list of tiles -----------------------------------------------------
@@ -73,13 +72,26 @@ __device__ __forceinline__ int tokens_of(const Work& w, int64_t b) {
 }
 __device__ __forceinline__ int tiles_of(const Work& w, int64_t b) { return (tokens_of(w, b) + kTile - 1) / kTile; }
 
-// Tiles of all sequences; the calling warp takes part as a whole.
-__device__ int64_t total_tiles(const Work& w, int lane) {
-  int64_t n = 0;
-  for (int64_t b = lane; b < w.batch; b += 32) n += tiles_of(w, b);
+// Tiles of all sequences, and the CTAs that share them; the calling warp takes
+// part as a whole.  A CTA takes two tiles at least, where one each would cut
+// sequences in more than half as many places as there are CTAs (the parts are
+// what a short call spends its time on: 9 sequences of up to 1167 tokens and 64
+// rows, 25 us with two and 29 with one; 5 of up to 700 and 60 rows, 23 and 19).
+__device__ void total_tiles(const Work& w, int ctas, int lane, int64_t* total, int64_t* sharers) {
+  int64_t n = 0, sequences = 0;
+  for (int64_t b = lane; b < w.batch; b += 32) {
+    const int tiles = tiles_of(w, b);
+    n += tiles;
+    sequences += tiles > 0;
+  }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-  return n * w.row_tiles;
+  for (int off = 16; off > 0; off >>= 1) {
+    n += __shfl_xor_sync(0xffffffffu, n, off);
+    sequences += __shfl_xor_sync(0xffffffffu, sequences, off);
+  }
+  *total = n * w.row_tiles;
+  const int64_t least = (n - sequences) * w.row_tiles > ctas / 2 ? 2 : 1, most = (*total + least - 1) / least;
+  *sharers = most < ctas ? most : ctas;
 }
 
 // The sequence of flat tile `at` (at < total), and the tiles before it.
@@ -107,11 +119,7 @@ __device__ void find_sequence(const Work& w, int64_t at, int lane, int64_t* sequ
   *before = base;
 }
 
-// CTAs that share `total` tiles, and the first tile of one of them.
-__device__ __forceinline__ int64_t sharers(int64_t total, int ctas) {
-  const int64_t n = (total + kMinTiles - 1) / kMinTiles;
-  return n < ctas ? n : ctas;
-}
+// The first tile of CTA i of n that share `total`.
 __device__ __forceinline__ int64_t first_tile(int64_t i, int64_t total, int64_t n) {
   // (a 64-bit division takes longer than the lists that need one are common)
   if (total < (1 << 20)) return static_cast<uint32_t>(i) * static_cast<uint32_t>(total) / static_cast<uint32_t>(n);
@@ -266,8 +274,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int blocks = a.rank / 64, tile_pairs = a.rank / 128;
   if (warp == 0) {
     pdl_wait();
-    const int64_t total = total_tiles(w, lane);
-    const int64_t n = sharers(total, gridDim.x);
+    int64_t total, n;
+    total_tiles(w, gridDim.x, lane, &total, &n);
     Walk walk{};
     if (blockIdx.x < n) {
       const int64_t at = first_tile(blockIdx.x, total, n);
@@ -287,6 +295,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     tmem_alloc(&sh.tmem, columns);
   } else if (warp == 2 && lane == 0) {
+    prefetch_tensor_map(&maps.q);
+    prefetch_tensor_map(&maps.r);
+    prefetch_tensor_map(&maps.cache);
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
     mbar_init(&sh.o_done, 1);
@@ -432,13 +443,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t pt = uniform(sp + (u & 1) * (kBlock >> 4));
         const uint32_t ct = uniform(sv + place.stage * (tile_pairs * (kPair >> 4)));
+        const int steps = uniform((walk.tokens - t * kTile + 15) / 16);  // 16 tokens each
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < kLatentMaxRank / 128; ++i) {
             if (i >= tile_pairs) continue;
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              tc_mma_f16(td + i * kN, desc_of(ct + ((i * kPair + k * 2048) >> 4)), desc_of(pt + (k * 2048 >> 4)), desc,
+              if (k < steps) tc_mma_f16(td + i * kN, desc_of(ct + ((i * kPair + k * 2048) >> 4)), desc_of(pt + (k * 2048 >> 4)), desc,
                          k > 0 || t > begin);
             tc_commit(&sh.empty[place.stage * tile_pairs + i]);
           }
@@ -497,14 +509,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // P's buffer is free once the products of the tile before the last are done.
         if (ok && u > 1) ok = mbar_wait(&sh.p_done[r], ((u >> 1) - 1) & 1);
-        if (!held && ok) {
-          // the two lanes of a token zero half of this half's blocks each
-          // (in an order that spreads a warp's tokens over the banks)
+        if (!held && ok && token < (walk.tokens + 15) / 16 * 16) {
+          // The two lanes of a token zero half of this half's blocks each, in an
+          // order that spreads a warp's tokens over the banks.
           uint8_t* tile = smem + lay.ring + place.stage * tile_pairs * kPair + token_row * 128;
           for (int i = half * blocks / 2; i < (half + 1) * blocks / 2; ++i) {
-            uint4* line = reinterpret_cast<uint4*>(tile + i * kBlock) + (lane >> 4) * 4;
+            uint4* line = reinterpret_cast<uint4*>(tile + i * kBlock);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) line[e ^ (token_row & 3)] = make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < 4; ++e) line[((lane >> 4) * 4 + e) ^ (token_row & 7)] = make_uint4(0, 0, 0, 0);
           }
         }
         if (__any_sync(0xffffffffu, !held || token >= least)) {
@@ -646,20 +658,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 constexpr int kJoinWarps = 16;
 constexpr int kJoinShare = 4;   // CTAs per cut
+constexpr int kJoinHeld = 5;    // parts of a row a lane weighs
+constexpr int kMaxCtas = 32 * kJoinHeld;
 
 // A sequence is cut where a CTA's share begins inside it, and its cuts divide
-// its rows among themselves: blockIdx.x + 1 is that CTA, blockIdx.y one of the
+// its rows among themselves: blockIdx.y + 1 is that CTA, blockIdx.x one of the
 // four that divide them again.  A warp takes a row, 16 channels a lane; with
 // more CTAs than rows, a CTA takes 128 channels of a row and its warps share
-// the parts.
+// the parts.  (A row's cuts are neighbours in the grid, so that those with work
+// are resident at once.)
 template <int kAct>
 __global__ void __launch_bounds__(32 * kJoinWarps)
     latent_join_kernel(const LatentAttentionArgs a, const Work w, int kn, const float* __restrict__ parts,
                        const float2* __restrict__ sums, const Cut* __restrict__ cuts) {
   __shared__ float4 s_o[kJoinWarps][32];
+  __shared__ float s_f[kJoinWarps][32 * kJoinHeld];
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t cta = blockIdx.x + 1;
+  const int64_t cta = blockIdx.y + 1;
   const Cut cut = cuts[cta];
   if (cta >= cut.sharers || first_tile(cta, cut.total, cut.sharers) <= cut.start) return;
   // The sequence's CTAs: `first` has its first tile, `last` its last.  A part
@@ -667,29 +683,39 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   // else in the second.
   const int first = static_cast<int>(owner_of(cut.start, cut.total, cut.sharers));
   const int last = static_cast<int>(owner_of(cut.start + cut.tiles - 1, cut.total, cut.sharers));
-  const int ctas = gridDim.x + 1;
+  const int ctas = gridDim.y + 1;
   const int slot0 = first + (first_tile(first, cut.total, cut.sharers) < cut.start ? ctas : 0);
   auto slot_of = [&](int k) { return k == 0 ? slot0 : first + k; };
   const int rows = w.queries * w.heads, count = last - first + 1, vectors = a.rank / 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int workers = (count - 1) * kJoinShare;
-  const int worker = (static_cast<int>(cta) - first - 1) * kJoinShare + blockIdx.y;
-  // The largest unit of a row's parts and their sum; the whole warp.
-  auto total = [&](int i, float& top, float& sum) {
+  const int worker = (static_cast<int>(cta) - first - 1) * kJoinShare + blockIdx.x;
+  // The largest unit of a row's parts, their sum, and what each part counts
+  // (in s_f[warp]); the whole warp.
+  auto weigh = [&](int i, float& top, float& sum) {
+    float2 v[kJoinHeld];
     top = -INFINITY;
     sum = 0.0f;
-    for (int k = lane; k < count; k += 32) {
-      const float2 v = sums[i * 2 * ctas + slot_of(k)];
-      if (v.y != 0.0f) top = fmaxf(top, v.x);
+#pragma unroll
+    for (int e = 0; e < kJoinHeld; ++e) {
+      const int k = lane + 32 * e;
+      v[e] = k < count ? sums[i * 2 * ctas + slot_of(k)] : make_float2(0.0f, 0.0f);
     }
 #pragma unroll
+    for (int e = 0; e < kJoinHeld; ++e)
+      if (v[e].y != 0.0f) top = fmaxf(top, v[e].x);
+#pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    for (int k = lane; k < count; k += 32) {
-      const float2 v = sums[i * 2 * ctas + slot_of(k)];
-      if (v.y != 0.0f) sum += v.y * exp2_fast(v.x - top);
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < kJoinHeld; ++e) {
+      const float f = v[e].y != 0.0f ? exp2_fast(v[e].x - top) : 0.0f;
+      sum = fmaf(v[e].y, f, sum);
+      s_f[warp][lane + 32 * e] = f;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    __syncwarp();
   };
   auto add = [](float4& o, const float4& p, float f) {
     o.x = fmaf(p.x, f, o.x);
@@ -706,13 +732,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
     for (int i = worker + warp * workers; i < kn; i += kJoinWarps * workers) {
       const int row = cut.rt * kn + i;
       if (row >= rows) break;
-      total(i, top, sum);
+      weigh(i, top, sum);
       float4 o[kLatentMaxRank / 128] = {};
 #pragma unroll 4
       for (int k = 0; k < count; ++k) {
         const int at = slot_of(k) * kn + i;
-        const float2 v = sums[i * 2 * ctas + slot_of(k)];
-        const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
+        const float f = s_f[warp][k];
         const float4* part = reinterpret_cast<const float4*>(parts + static_cast<int64_t>(at) * a.rank) + lane;
 #pragma unroll
         for (int e = 0; e < kLatentMaxRank / 128; ++e)
@@ -730,14 +755,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps)
   for (int unit = worker; unit < kn * vectors; unit += workers) {
     const int i = unit / vectors, vector = unit % vectors, row = cut.rt * kn + i;
     if (row >= rows) break;
-    total(i, top, sum);
+    weigh(i, top, sum);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
     for (int k = warp; k < count; k += kJoinWarps) {
       const int at = slot_of(k) * kn + i;
-      const float2 v = sums[i * 2 * ctas + slot_of(k)];
       add(o, *(reinterpret_cast<const float4*>(parts + static_cast<int64_t>(at) * a.rank) + 32 * vector + lane),
-          v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f);
+          s_f[warp][k]);
     }
     s_o[warp][lane] = o;
     __syncthreads();
@@ -757,7 +781,7 @@ int rows_per_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 int sm_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
+  return sms < kMaxCtas ? sms : kMaxCtas;
 }
 
 // Two tiles in the ring let the next one land and be scored while this one is
@@ -812,7 +836,7 @@ cudaError_t launch(const LatentAttentionArgs& a, cudaStream_t s) {
   err = launch_pdl(kernel, dim3(ctas), dim3(kThreads), lay.shared + sizeof(Shared), s, maps, a, w, lay, box, columns,
                    parts, sums, cuts);
   if (err != cudaSuccess || ctas < 2) return err;
-  return launch_pdl(latent_join_kernel<kAct>, dim3(ctas - 1, kJoinShare), dim3(32 * kJoinWarps), 0, s, a, w, kN,
+  return launch_pdl(latent_join_kernel<kAct>, dim3(kJoinShare, ctas - 1), dim3(32 * kJoinWarps), 0, s, a, w, kN,
                     static_cast<const float*>(parts), static_cast<const float2*>(sums),
                     static_cast<const Cut*>(cuts));
 }
