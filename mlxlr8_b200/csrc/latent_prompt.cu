@@ -69,13 +69,15 @@ struct Tiles {
   static_assert(kRing >= kBlocks + 4, "a key tile and two value tiles");
 };
 
+constexpr int kSplitGroups = 80;  // tiles of queries from which no two CTAs per tile would fit the GPU
+
 constexpr int kUnits = 8;  // key and value tiles that the barriers tell apart; the ring holds five at most
 
 struct Shared {
   uint64_t q_full, full[kUnits], empty[kUnits];
   uint64_t s_full[2], p_ready[2], o_done[2];
   uint32_t tmem;
-  int seq, tile;
+  int tile, q0, queries, k0, keys;  // tile -1: none
 };
 
 struct Maps {
@@ -123,36 +125,77 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return r;
 }
 
-template <int kAct, int kBlocks>
+// Four floats at the same shared-memory place of CTA `rank` of the cluster.
+__device__ __forceinline__ float4 load_cluster4(const void* p, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr(smem_u32(p), rank)));
+  return v;
+}
+__device__ __forceinline__ float2 load_cluster2(const void* p, int rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(cluster_addr(smem_u32(p), rank)));
+  return v;
+}
+
+// Lane and lane ^ off exchange: the one without the bit keeps its x and takes the
+// other's x for y, the one with it keeps its y and takes the other's y for x.
+__device__ __forceinline__ void trade(uint4& x, uint4& y, bool bit, int off) {
+  uint32_t* const u = &x.x;
+  uint32_t* const v = &y.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, bit ? u[i] : v[i], off);
+    if (bit) u[i] = other;
+    else v[i] = other;
+  }
+}
+
+// kSplit: a cluster shares the keys of one tile of queries.
+template <int kAct, int kBlocks, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
-    latent_prompt_kernel(const __grid_constant__ Maps maps, const LatentPromptArgs a, int value_parts) {
+    latent_prompt_kernel(const __grid_constant__ Maps maps, const LatentPromptArgs a, int value_parts, int shares) {
   using T = Tiles<kBlocks>;
   constexpr int kKeys = T::kKeys;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* const ring = smem + 2 * T::kQ;
+  float4* const staged = reinterpret_cast<float4*>(smem);  // [256][128 channels] of a share, over the operands
+  float2* const stats = reinterpret_cast<float2*>(smem + 256 * 512);        // of its rows: unit of O (log2), sum
+  float* const weights = reinterpret_cast<float*>(smem + 256 * 512 + 2048);  // [128][8] of the rows that it joins
   const int warp = static_cast<int>(uniform(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int columns = a.heads * value_parts;
-  const int head = blockIdx.x % columns / value_parts, part = blockIdx.x % value_parts;
+  const int group = kSplit ? blockIdx.x / shares : blockIdx.x, share = kSplit ? blockIdx.x % shares : 0;
+  const int head = group % columns / value_parts, part = group % value_parts;
 
   // The CTA's sequence and its tile of 256 queries: tiles are numbered over
   // the sequences and taken from the last (its rows see the most keys).
   pdl_launch_dependents();
   pdl_wait();
-  auto start_of = [&](const int32_t* starts, int s, int64_t total) {
-    return min(max(starts[s], 0), static_cast<int>(total));
-  };
-  auto tiles_of = [&](int s) {
-    const int n = s < a.seqs ? start_of(a.q_starts, s + 1, a.total_q) - start_of(a.q_starts, s, a.total_q) : 0;
-    return (max(n, 0) + 255) / 256;
-  };
   if (warp == 0) {
+    // A sequence's queries and keys, one sequence a lane.
+    int q0, queries, k0, keys;
+    auto load = [&](int s) {
+      auto clamped = [](int v, int64_t total) { return min(max(v, 0), static_cast<int>(total)); };
+      const bool some = s < a.seqs;
+      q0 = some ? clamped(a.q_starts[s], a.total_q) : 0;
+      k0 = some ? clamped(a.k_starts[s], a.total_k) : 0;
+      queries = some ? max(clamped(a.q_starts[s + 1], a.total_q) - q0, 0) : 0;
+      keys = some ? max(clamped(a.k_starts[s + 1], a.total_k) - k0, 0) : 0;
+    };
     int total = 0;
-    for (int s0 = 0; s0 < a.seqs; s0 += 32) total += __reduce_add_sync(0xffffffffu, tiles_of(s0 + lane));
-    int at = total - 1 - static_cast<int>(blockIdx.x / columns), found = -1, tile = 0;
-    for (int s0 = 0; s0 < a.seqs && at >= 0 && found < 0; s0 += 32) {
-      const int n = tiles_of(s0 + lane);
+    for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+      load(s0 + lane);
+      total += __reduce_add_sync(0xffffffffu, (queries + 255) / 256);
+    }
+    int at = total - 1 - group / columns, tile = -1;
+    for (int s0 = 0; s0 < a.seqs && at >= 0 && tile < 0; s0 += 32) {
+      if (a.seqs > 32) load(s0 + lane);
+      const int n = (queries + 255) / 256;
       int end = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -163,14 +206,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (mine) {
         const int which = __ffs(mine) - 1;
         tile = at - __shfl_sync(0xffffffffu, end - n, which);
-        found = s0 + which;
+        q0 = __shfl_sync(0xffffffffu, q0, which);
+        k0 = __shfl_sync(0xffffffffu, k0, which);
+        queries = __shfl_sync(0xffffffffu, queries, which);
+        keys = __shfl_sync(0xffffffffu, keys, which);
       } else {
         at -= __shfl_sync(0xffffffffu, end, 31);
       }
     }
     if (lane == 0) {
-      sh.seq = found;
       sh.tile = tile;
+      sh.q0 = q0, sh.queries = queries, sh.k0 = k0, sh.keys = keys;
+      prefetch_tensor_map(&maps.q);
+      prefetch_tensor_map(&maps.k);
+      prefetch_tensor_map(&maps.r);
+      prefetch_tensor_map(&maps.v);
       mbar_init(&sh.q_full, 1);
       for (int i = 0; i < kUnits; ++i) {
         mbar_init(&sh.full[i], 1);
@@ -184,12 +234,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_fence_init();
     }
   }
+  if (warp == 1) tmem_alloc(&sh.tmem, 512);
+  tc_fence_before();
   __syncthreads();
-  if (sh.seq < 0) return;
-  const int q0 = start_of(a.q_starts, sh.seq, a.total_q);
-  const int queries = start_of(a.q_starts, sh.seq + 1, a.total_q) - q0;
-  const int k0 = start_of(a.k_starts, sh.seq, a.total_k);
-  const int keys = max(start_of(a.k_starts, sh.seq + 1, a.total_k) - k0, 0);
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  if (sh.tile < 0) {
+    if (warp == 1) tmem_free(tmem, 512);
+    return;
+  }
+  const int q0 = sh.q0, queries = sh.queries, k0 = sh.k0, keys = sh.keys;
   const int first = sh.tile * 256;
   const int vb = min(2, a.value / 64 - 2 * part);  // 64-channel value blocks of this CTA
   // Key tiles of each query tile: its last query sees the most keys.
@@ -200,13 +254,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int seen = last >= first + q * kTileQ ? min(keys - queries + 1 + last, keys) : 0;
     tiles[q] = seen > 0 ? (seen + kKeys - 1) / kKeys : 0;
   }
+  int begin = 0;  // the first key tile of this CTA's share
+  if (kSplit) {
+    const int most = max(tiles[0], tiles[1]);
+    begin = most * share / shares;
+    const int end = most * (share + 1) / shares;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) tiles[q] = max(min(tiles[q], end) - begin, 0);
+  }
   const int all = max(tiles[0], tiles[1]);
-  if (warp == 1) tmem_alloc(&sh.tmem, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sh.tmem;
-
+  const int own0 = k0 + begin * kKeys;  // the share's first key
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
     if (warp == 0) {
@@ -232,9 +289,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(full, n * T::kBlock);
           for (int b = 0; b < n; ++b) {
             uint8_t* dst = ring + at * T::kBlock;
-            if (unit & 1) load_tile(dst, &maps.v, maps.v_swap, 128 * part + 64 * b, head, k0 + j * kKeys, full);
-            else if (b < kBlocks - 1) load_tile(dst, &maps.k, maps.k_swap, 64 * b, head, k0 + j * kKeys, full);
-            else tma_load_2d(dst, &maps.r, 0, k0 + j * kKeys, full);
+            if (unit & 1) load_tile(dst, &maps.v, maps.v_swap, 128 * part + 64 * b, head, own0 + j * kKeys, full);
+            else if (b < kBlocks - 1) load_tile(dst, &maps.k, maps.k_swap, 64 * b, head, own0 + j * kKeys, full);
+            else tma_load_2d(dst, &maps.r, 0, own0 + j * kKeys, full);
             if (++at == T::kRing) at = 0;
           }
           used += n;
@@ -292,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const int first_block = at;
         blocks(sv, vb, vt);
-        const int valid = uniform(keys) - j * kKeys;
+        const int valid = uniform(keys - begin * kKeys) - j * kKeys;
         if (valid < kKeys) {  // rows behind the sequence's last key
           for (int b = 0; b < vb; ++b) {
             uint8_t* tile = ring + (first_block + b < T::kRing ? first_block + b : first_block + b - T::kRing) * T::kBlock;
@@ -342,11 +399,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     }
+    if constexpr (kSplit) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int q = (warp - 4) / 4, quad = warp & 3;
     const int row = first + q * kTileQ + quad * 32 + lane;
-    const int seen = row < queries ? min(keys - queries + 1 + row, keys) : 0;
+    const int seen = (row < queries ? min(keys - queries + 1 + row, keys) : 0) - begin * kKeys;  // of the share
     const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
     const uint32_t ts = tmem + lanes + q * 128, to = tmem + lanes + 256 + q * 128;
     const float c = fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f;
@@ -434,31 +496,112 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (tiles[q] > 0 && ok) ok = mbar_wait(&sh.o_done[q], 0);
     tc_fence_after();
-    const bool store = row < queries;
-    const int64_t at = (static_cast<int64_t>(q0) + row) * a.heads + head;
-    if (a.lse && part == 0 && store)
-      a.lse[at] = !ok ? NAN : l > 0.0f ? (m * c - kLift + log2f(l)) * 0.6931471805599453f : (l == 0.0f ? -INFINITY : l);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int i = 0; i < 64 * vb; i += 32) {
-      uint32_t o[32];
-      if (tiles[q] > 0) {
+    if constexpr (kSplit) {
+      // The share's sums and outputs, over the operand tiles once both query
+      // tiles are done with them; 16-byte pieces swizzled by the row.
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const int r = q * kTileQ + quad * 32 + lane;
+      stats[r] = make_float2(m * c - kLift, ok ? l : NAN);
+      for (int i = 0; tiles[q] > 0 && i < 64 * vb; i += 32) {
+        uint32_t o[32];
         tc_ld32(to + i, o);
         tc_wait_ld();
         tc_settle<32>(o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          staged[r * 32 + ((i / 4 + e) ^ (r & 7))] =
+              make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                          __uint_as_float(o[4 * e + 3]));
       }
-      if (!store) continue;
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at * a.value + 128 * part + i);
+      __syncwarp();
+      cluster_sync();
+      // A CTA joins its share of the rows: first what each CTA's part of a row
+      // counts (eight lanes a row), then the parts, a warp a row.
+      const int row0 = 256 * share / shares, rows = 256 * (share + 1) / shares - row0;
+      const int id = threadIdx.x - 128;
+      for (int i0 = 0; i0 < rows; i0 += 32) {
+        const int i = i0 + id / 8, s = id % 8;
+        const bool there = i < rows && s < shares;
+        const float2 v = there ? load_cluster2(&stats[row0 + i], s) : make_float2(0.0f, 0.0f);
+        float top = v.y != 0.0f ? v.x : -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t w[4];
+        for (int off = 4; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float f = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
+        float sum = v.y * f;
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          float u = __uint_as_float(o[8 * e + 2 * f]) * inv, v = __uint_as_float(o[8 * e + 2 * f + 1]) * inv;
-          if (seen <= 0) u = v = 0.0f;
-          if (!ok) u = v = __int_as_float(0x7fc00000);
-          w[f] = pack<kAct>(u, v);
+        for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (i < rows) weights[i * 8 + s] = v.y != 0.0f ? f / sum : 0.0f;
+        const int at = first + row0 + i;
+        if (a.lse && part == 0 && i < rows && s == 0 && at < queries)
+          a.lse[(static_cast<int64_t>(q0) + at) * a.heads + head] =
+              sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 2
+      for (int i = warp - 4; i < rows; i += 8) {
+        const int r = row0 + i, at = first + r;
+        if (at >= queries || lane >= 16 * vb) continue;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int s0 = 0; s0 < shares; s0 += 4) {
+          float4 p[4];
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            p[s] = load_cluster4(&staged[r * 32 + (lane ^ (r & 7))], min(s0 + s, shares - 1));
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const float f = weights[i * 8 + s0 + s];
+            if (f == 0.0f) continue;  // a part that sees nothing of the row holds no output
+            sum.x = fmaf(p[s].x, f, sum.x);
+            sum.y = fmaf(p[s].y, f, sum.y);
+            sum.z = fmaf(p[s].z, f, sum.z);
+            sum.w = fmaf(p[s].w, f, sum.w);
+          }
         }
-        dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) +
+                                 ((static_cast<int64_t>(q0) + at) * a.heads + head) * a.value + 128 * part)[lane] =
+            make_uint2(pack<kAct>(sum.x, sum.y), pack<kAct>(sum.z, sum.w));
+      }
+      __syncwarp();
+      cluster_sync();  // no CTA leaves while its part is read
+    } else {
+      const bool store = row < queries;
+      const int64_t at = (static_cast<int64_t>(q0) + row) * a.heads + head;
+      if (a.lse && part == 0 && store)
+        a.lse[at] = !ok ? NAN : l > 0.0f ? (m * c - kLift + log2f(l)) * 0.6931471805599453f : (l == 0.0f ? -INFINITY : l);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      for (int i = 0; i < 64 * vb; i += 32) {
+        uint32_t o[32];
+        if (tiles[q] > 0) {
+          tc_ld32(to + i, o);
+          tc_wait_ld();
+          tc_settle<32>(o);
+        }
+        uint4 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t two[4];
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            float u = __uint_as_float(o[8 * e + 2 * f]) * inv, v = __uint_as_float(o[8 * e + 2 * f + 1]) * inv;
+            if (seen <= 0) u = v = 0.0f;
+            if (!ok) u = v = __int_as_float(0x7fc00000);
+            two[f] = pack<kAct>(u, v);
+          }
+          w[e] = make_uint4(two[0], two[1], two[2], two[3]);
+        }
+        // Four lanes trade pieces of their rows, so that they store 64 bytes of
+        // one row at a time (a row a lane took 3500 cycles for 256 x 128).
+        trade(w[0], w[1], lane & 1, 1);
+        trade(w[2], w[3], lane & 1, 1);
+        trade(w[0], w[2], lane & 2, 2);
+        trade(w[1], w[3], lane & 2, 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t to_row = row - (lane & 3) + e;
+          if (to_row < queries)
+            reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + ((q0 + to_row) * a.heads + head) * a.value +
+                                     128 * part + i)[lane & 3] = w[e];
+        }
       }
     }
   }
@@ -481,6 +624,22 @@ bool encode_rows(CUtensorMap* map, int* swap, CUtensorMapDataType type, const vo
   return encode_tiled_3d(map, type, base, {d, h, n}, {hs, ts}, {64, 1, rows}, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Clusters of n CTAs that the current device holds at once; asked of the driver
+// once per device and size.
+template <typename Kernel>
+cudaError_t clusters_at_once(Kernel kernel, cudaLaunchConfig_t cfg, int n, int* clusters) {
+  static std::atomic<int> known[16][9];
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  if (device < 16 && (*clusters = known[device][n].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  cfg.gridDim = dim3(n);
+  cfg.attrs->val.clusterDim.x = n;
+  err = cudaOccupancyMaxActiveClusters(clusters, kernel, &cfg);
+  if (err == cudaSuccess && device < 16) known[device][n].store(*clusters, std::memory_order_relaxed);
+  return err;
+}
+
 template <int kAct, int kBlocks>
 cudaError_t launch(const LatentPromptArgs& a, cudaStream_t s) {
   using T = Tiles<kBlocks>;
@@ -500,14 +659,51 @@ cudaError_t launch(const LatentPromptArgs& a, cudaStream_t s) {
       !encode_rows(&maps.v, &maps.v_swap, type, empty ? a.q : a.v, empty ? 64 : a.value, a.heads, keys,
                    empty ? a.q_token : a.v_token, empty ? a.q_head : a.v_head, T::kKeys))
     return cudaErrorInvalidValue;
-  auto kernel = latent_prompt_kernel<kAct, kBlocks>;
-  static std::atomic<uint64_t> ready{0};
-  cudaError_t err = allow_shared_memory(kernel, kSmem + 1024, ready);
-  if (err != cudaSuccess) return err;
   const int parts = (a.value + 127) / 128;
-  const int64_t tiles = (a.total_q + 255) / 256 + a.seqs;
-  return launch_pdl(kernel, dim3(static_cast<unsigned>(tiles * a.heads * parts)), dim3(kThreads), kSmem + 1024, s, maps,
-                    a, parts);
+  // No more tiles of 256 queries can hold queries of ascending sequences.
+  const int64_t tiles = a.total_q < a.seqs ? a.total_q : (a.total_q - a.seqs) / 256 + a.seqs;
+  const int64_t groups = tiles * a.heads * parts;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem + 1024;
+  cfg.stream = s;
+  static std::atomic<uint64_t> ready[2];
+  // Few tiles of queries leave SMs idle while each walks its keys one tile after
+  // the other: a cluster of CTAs shares them, as many as are resident at once,
+  // two key tiles each at least (165 queries over 2165 keys, 8 heads of 256 + 256
+  // channels: KEYS us alone, SHARED by six; a join takes 3 us).
+  int shares = 1;
+  const int64_t key_tiles = a.total_k / a.seqs / T::kKeys;
+  if (groups < kSplitGroups && key_tiles >= 4) {
+    auto kernel = latent_prompt_kernel<kAct, kBlocks, true>;
+    cudaError_t err = allow_shared_memory(kernel, kSmem + 1024, ready[1]);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    for (int n = 8, fit; err == cudaSuccess && n > 1 && shares == 1; --n) {
+      if (2 * n > key_tiles) continue;
+      err = clusters_at_once(kernel, cfg, n, &fit);
+      if (groups <= fit) shares = n;
+    }
+    if (err != cudaSuccess) return err;
+    if (shares > 1) {
+      attr[0].val.clusterDim.x = shares;
+      cfg.gridDim.x = static_cast<unsigned>(groups * shares);
+      cfg.numAttrs = 2;
+      return cudaLaunchKernelEx(&cfg, kernel, maps, a, parts, shares);
+    }
+  }
+  auto kernel = latent_prompt_kernel<kAct, kBlocks, false>;
+  const cudaError_t err = allow_shared_memory(kernel, kSmem + 1024, ready[0]);
+  if (err != cudaSuccess) return err;
+  cfg.attrs = attr + 1;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, maps, a, parts, 1);
 }
 
 template <int kAct>

@@ -442,6 +442,27 @@ def test_prompt_scores_of_every_size():
                 _prompt(q, k, kr, v, [700], [700], scale)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("queries, keys, heads, nope, value", [
+    ([165], [2165], 3, 192, 256), ([900], [900], 4, 64, 64), ([5, 260, 0], [1900, 2260, 900], 2, 128, 192),
+    ([40], [1200], 1, 128, 128), ([700], [600], 1, 128, 64), ([256, 1], [2050, 1], 2, 64, 128),
+])
+def test_prompt_with_keys_shared_by_several_ctas(dtype, queries, keys, heads, nope, value):
+    """Few tiles of queries and many keys: two, four or eight CTAs to a tile."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(sum(queries) + heads)
+    q, k, kr, v = _operands(g, queries, keys, heads, nope, value, torch_dtype(dtype))
+    got = _prompt(q, k, kr, v, queries, keys, 1.5 * (nope + 64) ** -0.5)
+    # a score that outgrows all before it, in the last share and in the first
+    for at in (0, keys[0] - queries[0]):
+        if at >= 0:
+            k2 = k.clone()
+            k2[at] *= 30.0
+            _prompt(q, k2, kr, v, queries, keys, 0.2)
+    assert torch.equal(_prompt(q, k, kr, v, queries, keys, 1.5 * (nope + 64) ** -0.5), got)
+
+
 def test_prompt_takes_views_and_leaves_other_rows():
     import torch
 
