@@ -5,15 +5,20 @@
 // Decoding reads every code once for a handful of rows, so the kernel is
 // built to stream.  A CTA takes 128 weight rows in stages of 128 channels (the
 // rows' 64 bytes and the channels of x, tensor-map boxes), and two CTAs per SM
-// keep their rings full; eight warps multiply with mma.sync m16n8k16 (weights on the M side, up to 8 rows of x on the N side; the
-// products need a few percent of even the warp-level tensor rate, so tcgen05
-// would gain nothing, and its operands would have to be unpacked through
-// shared memory).  What bounds such a kernel after the loads is the integer
-// pipe that unpacks the codes, so a code is only moved, with one shift and one
-// three-input logic operation per pair, into the upper mantissa bits of 1.0:
-// v = 1 + q / 16, exact in bfloat16 and float16.  Then, for every unit u of one
+// keep their rings full; eight warps multiply with mma.sync m16n8k16 (weights
+// on the M side, up to 8 rows of x on the N side; the products need a few
+// percent of even the warp-level tensor rate, so tcgen05 would gain nothing,
+// and its operands would have to be unpacked through shared memory).  What
+// bounds such a kernel after the loads is the integer pipe that unpacks the
+// codes, so a code is only masked where it lies.  With float16 products (float16
+// x and E4M3 x, which float16 holds exactly) it is the subnormal q 2^-24 or, four
+// bits up, q 2^-20: exact, two accumulators.  bfloat16 products would leave
+// such sums below float32's normal range, so there a shift and a three-input
+// logic operation a pair make it v = 1 + q / 16.  Then, for every unit u of one
 // weight scale (and one scale of x),
-//   y = sum_u 16 s_u * (sum_{k in u} v_k x_k) + (b_u - 16 s_u) * (sum_{k in u} x_k)
+//   float16:   y = sum_u s_u * (sum_{k in u} q_k x_k) + b_u * (sum_{k in u} x_k)
+//   bfloat16:  y = sum_u 16 s_u * (sum_{k in u} v_k x_k)
+//                  + (b_u - 16 s_u) * (sum_{k in u} x_k)
 // (b = -8 s without biases).  Products are exact and sums float32; v lies in
 // [1, 2), so what cancels is no more than three times the sum of |q - 8| x.  The
 // second sum is a product with ones, which lands it in the accumulator's
@@ -23,18 +28,24 @@
 // quad takes word 4 j + t of a row's 16, so that place j is 32 channels: units
 // of 32, 64 and 128 are whole places.  The swizzles (64 bytes for the codes, 128
 // for x) make both reads free of bank conflicts but for a factor of two on x.
-// Float32 x is cut into three bfloat16 pieces that sum to it; E4M3 codes are
-// exact in float16 and their scales multiply the unit's sum.  Groups of warps
-// that cover the 128 rows take stages in turn, each group in places of its own
-// (a group that waited on another's place could be a round ahead of it, and a
-// barrier's parity does not tell two rounds apart); a thread of the group
-// refills a place when the group has left it.  The scales come through shared
-// memory too, four stages at a time, converted once and laid out a block ahead
-// in three buffers, so that no warp waits for more than the others' last block:
-// read by every lane from global memory, each load touched eight lines, and
-// groups of 32 took four times as long as groups of 128.  A cluster of up to eight CTAs
-// shares the channels of one row tile where the row tiles alone would not fill
-// the SMs evenly; sums are added in a fixed order: the same bits every run.
+// Float32 x is cut into three bfloat16 pieces that sum to it; scales of E4M3
+// codes multiply the unit's sum.  Groups of warps that cover the 128 rows take
+// stages in turn, each group in places of its own (a group that waited on
+// another's place could be a round ahead of it, and a barrier's parity does not
+// tell two rounds apart); a thread of the group refills a place when the group
+// has left it.  The scales come through shared memory too, four stages at a
+// time, converted once and laid out a block ahead in three buffers, so that no
+// warp waits for more than the others' last block: read by every lane from
+// global memory, each load touched eight lines, and groups of 32 took four
+// times as long as groups of 128.  (Eight stages at a time: 8 x 6144 x 36864 3%
+// faster, 1 x 16384 x 6144 5% slower.)  A cluster of up to eight CTAs shares the
+// channels of one row tile where the row tiles alone would not fill the SMs
+// evenly; sums are added in a fixed order: the same bits every run.
+//
+// On the device: 1 row of 16384 x 6144 (50 MB) 23.3 us, 2.3 TB/s; 8 E4M3 rows of
+// 6144 x 36864 (113 MB) 30.4 us, 3.9 TB/s; 1 row of 6144 x 576 6.6 us.  The
+// schedulers issue in 54% of the cycles with 3.6 warps each, the integer pipe
+// is half busy: latency between the two, and the uneven last round of CTAs.
 
 #include <cuda.h>
 
@@ -69,12 +80,15 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Codes i and i + 4 of a word as 1 + q / 16 in two 16-bit floats: q at mantissa
-// bits 3 to 6 of bfloat16, 6 to 9 of float16.  The mask and the ones come in
-// registers: as constants they made two instructions of (v & mask) | ones.
+// Codes i and i + 4 of a word in two 16-bit floats.  bfloat16: 1 + q / 16, q at
+// mantissa bits 3 to 6.  float16: the code alone, a subnormal q 2^-24 (even i) or
+// q 2^-20 (odd i) where it lies, after one shift for i of 2 and 3.  The mask and
+// the ones come in registers: as constants they made two instructions of (v &
+// mask) | ones.
 template <bool kHalf>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, uint32_t mask, uint32_t ones) {
-  const int up = (kHalf ? 6 : 3) - 4 * i;
+  if (kHalf) return (i < 2 ? w : w >> 8) & (i & 1 ? 0x00F000F0u : 0x000F000Fu);
+  const int up = 3 - 4 * i;
   const uint32_t v = up >= 0 ? w << up : w >> -up;
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(ones));
@@ -135,6 +149,12 @@ __device__ __forceinline__ Pieces<kX> load_pieces(const uint8_t* x, int token, i
     interleave(p.v[0], c.x, c.y, c.z, c.w);
   }
   return p;
+}
+
+// What the two sums of a unit count, from the scale and the bias.
+template <bool kHalf>
+__device__ __forceinline__ float2 scale_pair(float s, float b) {
+  return kHalf ? make_float2(16777216.0f * s, b) : make_float2(16.0f * s, fmaf(-16.0f, s, b));
 }
 
 // A float at the same shared-memory place of CTA `rank` of the cluster.
@@ -241,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                   static_cast<int>(row0), &full[slot]);
   };
   uint32_t mask, one;
-  asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(kHalf ? 0x03C003C0 : 0x00780078));
+  asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(0x00780078));
   asm volatile("mov.b32 %0, %1;" : "=r"(one) : "n"(kHalf ? 0x3C003C00 : 0x3F803F80));
   const bool loader = warp % S::kWarps == 0 && lane == 0;
   // Stage i belongs to group i % kGroups; its n-th stage to that group's place n % kDepth.
@@ -312,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           v = __half2float(__ushort_as_half(static_cast<unsigned short>(raw_s[e])));
           b = __half2float(__ushort_as_half(static_cast<unsigned short>(raw_b[e])));
         }
-        dst[e * kRows] = make_float2(16.0f * v, a.biases ? b - 16.0f * v : -24.0f * v);
+        dst[e * kRows] = scale_pair<kHalf>(v, a.biases ? b : -8.0f * v);
       }
     }
     if (kX == kXE4M3 && threadIdx.x < S::kScales * S::kTokens)
@@ -342,7 +362,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         if (kUnits > 1 && (begin + i) * kChunk + u * kUnit >= in) break;
-        float acc[kTiles][kM][4] = {}, ones[kTiles][4] = {};
+        // [0]: the sums of codes i = 0 and 2, [1]: of 1 and 3 (float16), else of all.
+        float acc[kHalf ? 2 : 1][kTiles][kM][4] = {}, ones[kTiles][4] = {};
 #pragma unroll
         for (int j = u * kPlaces; j < (u + 1) * kPlaces; ++j) {
           uint32_t w[2 * kM];
@@ -355,15 +376,16 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int p = 0; p < 2; ++p) {
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
-              const uint32_t av[4] = {code_pair<kHalf>(w[2 * m], 2 * p, mask, one),
-                                      code_pair<kHalf>(w[2 * m + 1], 2 * p, mask, one),
-                                      code_pair<kHalf>(w[2 * m], 2 * p + 1, mask, one),
-                                      code_pair<kHalf>(w[2 * m + 1], 2 * p + 1, mask, one)};
+              const int i0 = kHalf ? p : 2 * p, i1 = kHalf ? p + 2 : 2 * p + 1;
+              const uint32_t av[4] = {code_pair<kHalf>(w[2 * m], i0, mask, one),
+                                      code_pair<kHalf>(w[2 * m + 1], i0, mask, one),
+                                      code_pair<kHalf>(w[2 * m], i1, mask, one),
+                                      code_pair<kHalf>(w[2 * m + 1], i1, mask, one)};
 #pragma unroll
               for (int n = 0; n < kTiles; ++n)
 #pragma unroll
                 for (int set = 0; set < kSets; ++set)
-                  mma(acc[n][m], av, x[n].v[set][2 * p], x[n].v[set][2 * p + 1], kHalf);
+                  mma(acc[kHalf ? p : 0][n][m], av, x[n].v[set][i0], x[n].v[set][i1], kHalf);
             }
             const uint32_t av[4] = {one, one, one, one};
 #pragma unroll
@@ -398,8 +420,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               v = a.scale_dtype == kBF16 ? make_float2(__uint_as_float(raw << 16), __uint_as_float(raw & 0xffff0000u))
                                          : __half22float2(*reinterpret_cast<const __half2*>(&raw));
             }
-            v.x *= 16.0f;
-            v.y = a.biases ? v.y - v.x : -1.5f * v.x;
+            v = scale_pair<kHalf>(v.x, a.biases ? v.y : -8.0f * v.x);
           } else {
             v = scale[8 * r];
           }
@@ -408,7 +429,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int f = 0; f < 2; ++f) {
               float& o = out[n][r / 2][2 * (r & 1) + f];
-              const float y = fmaf(ones[n][f], v.y, acc[n][r / 2][2 * (r & 1) + f] * v.x);
+              float sum = acc[0][n][r / 2][2 * (r & 1) + f];
+              if (kHalf) sum = fmaf(acc[kHalf][n][r / 2][2 * (r & 1) + f], 0.0625f, sum);
+              const float y = fmaf(ones[n][f], v.y, sum * v.x);
               o = kX == kXE4M3 ? fmaf(y, xs[n][f], o) : o + y;
             }
         }
