@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ---- joining the parts ---------------------------------------------------------------
 
-constexpr int kJoinWarps = 16;
+constexpr int kJoinWarps = 8;
 constexpr int kJoinShare = 4;   // CTAs per cut
 constexpr int kJoinHeld = 5;    // parts of a row a lane weighs
 constexpr int kMaxCtas = 32 * kJoinHeld;
@@ -668,7 +668,7 @@ constexpr int kMaxCtas = 32 * kJoinHeld;
 // the parts.  (A row's cuts are neighbours in the grid, so that those with work
 // are resident at once.)
 template <int kAct>
-__global__ void __launch_bounds__(32 * kJoinWarps)
+__global__ void __launch_bounds__(32 * kJoinWarps, 4)
     latent_join_kernel(const LatentAttentionArgs a, const Work w, int kn, const float* __restrict__ parts,
                        const float2* __restrict__ sums, const Cut* __restrict__ cuts) {
   __shared__ float4 s_o[kJoinWarps][32];
