@@ -157,11 +157,12 @@ struct Walk {
   }
 };
 
-// What a CTA leaves for the join: the (sequence, row tile) of its first tile,
-// where that begins, and the cut of the list.
+// What a CTA that begins inside a (sequence, row tile) leaves for the join: the
+// CTAs that share it, `first` to first + count - 1, and the slot of the part of
+// the first; count is 0 where the CTA begins with one.
 struct Cut {
-  int64_t start, total, sharers, sequence;
-  int rt, tiles;
+  int64_t sequence;
+  int rt, first, count, slot;
 };
 
 // ---- the main kernel -------------------------------------------------------------
@@ -176,6 +177,7 @@ struct Shared {
   uint64_t full[kMaxPairs], empty[kMaxPairs], rope_full[2], rope_empty[2];
   uint32_t tmem;
   Walk walk;
+  int64_t at, total, sharers;  // the share's first tile; of all CTAs
   __align__(16) float base[64];
   __align__(16) float factor[64];
   float m[64];
@@ -287,9 +289,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       walk.tiles = (walk.tokens + kTile - 1) / kTile;
       walk.rt = static_cast<int>((at - before) / walk.tiles);
       walk.tile = static_cast<int>((at - before) % walk.tiles);
-      if (lane == 0) cuts[blockIdx.x] = Cut{at - walk.tile, total, n, sequence, walk.rt, walk.tiles};
-    } else if (lane == 0) {
-      cuts[blockIdx.x] = Cut{};
+      if (lane == 0) {
+        sh.at = at;
+        sh.total = total;
+        sh.sharers = n;
+      }
     }
     if (lane == 0) sh.walk = walk;
   } else if (warp == 1) {
@@ -460,6 +464,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         place.advance(lay.stages);
       }
+    }
+  } else if (warp == 3) {  // what the join needs to know
+    if (lane == 0) {
+      Cut cut{walk.b, walk.rt, 0, 0, 0};
+      if (walk.tile > 0) {
+        const int64_t start = sh.at - walk.tile;
+        cut.first = static_cast<int>(owner_of(start, sh.total, sh.sharers));
+        cut.count = static_cast<int>(owner_of(start + walk.tiles - 1, sh.total, sh.sharers)) - cut.first + 1;
+        cut.slot = cut.first + (first_tile(cut.first, sh.total, sh.sharers) < start ? gridDim.x : 0);
+      }
+      cuts[blockIdx.x] = cut;
     }
   } else if (warp >= 4) {
     constexpr int kCols = kN / 2;
@@ -677,16 +692,12 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 4)
   pdl_wait();
   const int64_t cta = blockIdx.y + 1;
   const Cut cut = cuts[cta];
-  if (cta >= cut.sharers || first_tile(cta, cut.total, cut.sharers) <= cut.start) return;
-  // The sequence's CTAs: `first` has its first tile, `last` its last.  A part
-  // lies in its CTA's first slot where the share begins with the sequence,
-  // else in the second.
-  const int first = static_cast<int>(owner_of(cut.start, cut.total, cut.sharers));
-  const int last = static_cast<int>(owner_of(cut.start + cut.tiles - 1, cut.total, cut.sharers));
-  const int ctas = gridDim.y + 1;
-  const int slot0 = first + (first_tile(first, cut.total, cut.sharers) < cut.start ? ctas : 0);
-  auto slot_of = [&](int k) { return k == 0 ? slot0 : first + k; };
-  const int rows = w.queries * w.heads, count = last - first + 1, vectors = a.rank / 128;
+  if (cut.count == 0) return;
+  // A part lies in its CTA's first slot where the share begins with the
+  // sequence or inside it, in the second where it ends with its beginning.
+  const int ctas = gridDim.y + 1, first = cut.first, count = cut.count;
+  auto slot_of = [&](int k) { return k == 0 ? cut.slot : first + k; };
+  const int rows = w.queries * w.heads, vectors = a.rank / 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int workers = (count - 1) * kJoinShare;
   const int worker = (static_cast<int>(cta) - first - 1) * kJoinShare + blockIdx.x;
