@@ -13,12 +13,12 @@
 // m a running maximum and l = sum P the float32 sum of the unrounded weights.
 // m is raised only when a row's maximum has grown by more than 2^8 (then O and
 // l are multiplied once and the tile is weighed again), so a tile is weighed
-// without a pass for its maximum first, and P stays below 2^14 and float16 weights keep their
-// full precision down to 2^-20 of the largest.  Tensor memory is full: S_0,
-// S_1, O_0, O_1 of 128 columns each, P_q over S_q.  While the threads of one
-// query tile form its weights the tensor pipe works for the other one, which
-// is why two tiles share a CTA (and why each K and V tile is read from L2
-// once for 256 queries).
+// without a pass for its maximum first, and P stays below 2^14 and float16
+// weights keep their full precision down to 2^-20 of the largest.  Tensor memory
+// is full: S_0, S_1, O_0, O_1 of 128 columns each, P_q over S_q.  While the
+// threads of one query tile form its weights the tensor pipe works for the other
+// one, which is why two tiles share a CTA (and why each K and V tile is read
+// from L2 once for 256 queries).
 //
 // The two query tiles leave room for 1.6 tiles of keys and values (at 192 key
 // channels), so K and V tiles share one ring of blocks of 64 channels, in the
@@ -32,11 +32,19 @@
 //
 // Warp 0 loads (TMA), warp 1 issues the matrix instructions, warps 4-7 and
 // 8-11 are the softmax of query tiles 0 and 1 and take registers that the first
-// four give up.  Value channels beyond 128 are
-// a second CTA's (the scores are formed again there).  Rows of the last key
-// tile that belong to no key of the sequence are zeroed in the V tile, since
-// 0 x NaN would reach the sum.  Waits are bounded; one that runs out leaves
-// NaN in the CTA's output.
+// four give up.  Value channels beyond 128 are a second CTA's (the scores are
+// formed again there).  Rows of the last key tile that belong to no key of the
+// sequence are zeroed in the V tile, since 0 x NaN would reach the sum.  Waits
+// are bounded; one that runs out leaves NaN in the CTA's output.
+//
+// Where the tiles of queries are few, a cluster of two to eight CTAs shares the
+// keys of one: each leaves O, m and l of its share in its shared memory, float32
+// over the operands, and joins a part of the rows from all of them, in the order
+// of the shares.
+//
+// 8192 queries of 32 heads (128 + 64 key and 128 value channels): 551 us, 1247
+// TFLOP/s, the tensor pipe bound; 5 prompts of 1300 tokens, 16 heads: 26 us, the
+// longest one's keys in turn (2000 cycles a tile).
 
 #include <cuda.h>
 
@@ -677,7 +685,8 @@ cudaError_t launch(const LatentPromptArgs& a, cudaStream_t s) {
   // Few tiles of queries leave SMs idle while each walks its keys one tile after
   // the other: a cluster of CTAs shares them, as many as are resident at once,
   // two key tiles each at least (165 queries over 2165 keys, 8 heads of 256 + 256
-  // channels: KEYS us alone, SHARED by six; a join takes 3 us).
+  // channels: 58 us alone, 29 by four, 24 by six; by eight, of which 15 fit and 16
+  // were needed, 35).
   int shares = 1;
   const int64_t key_tiles = a.total_k / a.seqs / T::kKeys;
   if (groups < kSplitGroups && key_tiles >= 4) {

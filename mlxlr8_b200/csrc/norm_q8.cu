@@ -8,6 +8,9 @@
 // code, which saturates at 448 by construction.  A group of zeros has scale 0
 // and codes 0; a group with a value that is not finite has scale NaN and
 // codes 0, so that every value it stands for is NaN.
+//
+// Bound by memory: 8192 x 6144 bfloat16 with residual and groups of 128, 354 MB,
+// 61.7 us or 5.7 TB/s; one scale a row 52.7 us; one row 2.2 us, a launch.
 
 #include "common.cuh"
 #include "launch.cuh"
@@ -170,7 +173,8 @@ __global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024)
 
 // One CTA per row, any hidden size and alignment.  kCached keeps h w of the row
 // in shared memory, so that the inputs are read once; rows beyond kCachedMax
-// channels read them again.
+// channels read them again.  Single loads: 5000 x 7999 bfloat16 88 us, 3.2 TB/s
+// (106 us with the inputs read three times).
 constexpr int kCachedMax = 24 * 1024;  // two CTAs of 96 KB per SM
 
 template <int kAct, bool kCached>
@@ -257,7 +261,7 @@ cudaError_t launch(const void* x, const void* residual, const void* w, int64_t r
   const bool vectors = hidden % 8 == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(w, 16) &&
                        aligned(h_out, 16) && aligned(codes, 8);
   // A few rows spread over as many threads as a row has vectors; many rows
-  // leave more loads to a thread and more rows to an SM.
+  // leave more loads to a thread and more rows to an SM.  296: two CTAs an SM.
   const int vecs = hidden / 8;
   const bool few = rows <= 296;
   if (vectors && vecs <= (few ? 1024 : 256))
