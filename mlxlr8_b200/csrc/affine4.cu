@@ -32,8 +32,8 @@
 // codes multiply the unit's sum.  Groups of warps that cover the 128 rows take
 // stages in turn, each group in places of its own (a group that waited on
 // another's place could be a round ahead of it, and a barrier's parity does not
-// tell two rounds apart); a thread of the group refills a place when the group
-// has left it.  The scales come through shared memory too, four stages at a
+// tell two rounds apart); the last warp to leave a place has its next stage
+// fetched.  The scales come through shared memory too, four stages at a
 // time, converted once and laid out a block ahead in three buffers, so that no
 // warp waits for more than the others' last block: read by every lane from
 // global memory, each load touched eight lines, and groups of 32 took four
@@ -42,8 +42,8 @@
 // channels of one row tile where the row tiles alone would not fill the SMs
 // evenly; sums are added in a fixed order: the same bits every run.
 //
-// On the device: 1 row of 16384 x 6144 (50 MB) 23.3 us, 2.3 TB/s; 8 E4M3 rows of
-// 6144 x 36864 (113 MB) 30.4 us, 3.9 TB/s; 1 row of 6144 x 576 6.6 us.  The
+// On the device: 1 row of 16384 x 6144 (50 MB) 23.0 us, 2.3 TB/s; 8 E4M3 rows of
+// 6144 x 36864 (113 MB) 30.2 us, 3.9 TB/s; 1 row of 6144 x 576 6.5 us.  The
 // schedulers issue in 54% of the cycles with 3.6 warps each, the integer pipe
 // is half busy: latency between the two, and the uneven last round of CTAs.
 
@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int kSets = Pieces<kX>::kSets, kM = S::kM;
   constexpr int kUnits = kChunk / kUnit, kPlaces = kUnit / 32;  // units of a stage, places of a unit
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], laid[3];
+  __shared__ uint64_t full[kMaxStages], laid[3];
+  __shared__ uint32_t left[kMaxStages];  // warps that have left a place, since the start
   __shared__ float s_sum[S::kOutputs];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kCount; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], S::kWarps);
+      left[i] = 0;
     }
     for (int i = 0; i < 3; ++i) mbar_init(&laid[i], 8);
     mbar_fence_init();
@@ -263,12 +264,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint32_t mask, one;
   asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(0x00780078));
   asm volatile("mov.b32 %0, %1;" : "=r"(one) : "n"(kHalf ? 0x3C003C00 : 0x3F803F80));
-  const bool loader = warp % S::kWarps == 0 && lane == 0;
+  // A warp is done with stage i: the last of its group fetches the place's next
+  // stage (none waits for another here).
+  bool ok = true;
+  auto leave = [&](int i, int slot) {
+    if (!ok || i + S::kCount >= stages) return;
+    uint32_t before;
+    asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;"
+                 : "=r"(before)
+                 : "r"(smem_u32(&left[slot]))
+                 : "memory");
+    if (before % S::kWarps == S::kWarps - 1) load(i + S::kCount, slot);
+  };
   // Stage i belongs to group i % kGroups; its n-th stage to that group's place n % kDepth.
   if (threadIdx.x == 0)
     for (int i = 0; i < min(stages, S::kCount); ++i) load(i, i % S::kGroups * S::kDepth + i / S::kGroups);
   __syncwarp();
-  bool ok = true;
   float out[kTiles][kM][4];
 #pragma unroll
   for (int n = 0; n < kTiles; ++n)
@@ -396,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         if (u == kUnits - 1) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&empty[slot]);  // the stage has been read
+          if (lane == 0) leave(i, slot);
         }
         const int at = (i % kBlock) * kChunk + u * kUnit;  // channel in the block
         const float2* scale = s_scale + (buffer * S::kScales + (at >> group_shift)) * kRows + r0;
@@ -435,15 +446,6 @@ __global__ void __launch_bounds__(kThreads, 2)
               o = kX == kXE4M3 ? fmaf(y, xs[n][f], o) : o + y;
             }
         }
-      }
-      if (kUnits > 1 && (begin + i + 1) * kChunk > in && (in % kChunk) <= kChunk - kUnit) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[slot]);  // a last stage that ends early
-      }
-      // The group's first thread refills the place once its warps have left it.
-      if (loader && i + S::kCount < stages && ok) {
-        ok = mbar_wait(&empty[slot], round);
-        if (ok) load(i + S::kCount, slot);
       }
       __syncwarp();
       if (++slot == (group + 1) * S::kDepth) {
