@@ -642,8 +642,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int channel = 128 * k + quad * 32 + lane;
         if (!whole) {
           float* dst = parts + (slot * kN + col0) * a.rank + channel;
+          const int count = rows - walk.rt * kN - col0;  // (the join reads no row past the last)
 #pragma unroll
-          for (int i = 0; i < kCols; ++i, dst += a.rank) *dst = __uint_as_float(o[i]);
+          for (int i = 0; i < kCols; ++i, dst += a.rank)
+            if (i < count) *dst = __uint_as_float(o[i]);
         } else {
           // Four lanes trade their channels of four rows, so that each stores four
           // channels of one (single channels took 8000 cycles at 64 x 512).
