@@ -8,7 +8,6 @@ raises if the library is missing or no CUDA device is present.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from ctypes import c_double, POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 from functools import lru_cache
 from pathlib import Path
@@ -235,13 +234,18 @@ def stream_handle(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-_HERE = nullcontext()
-
-
-def on_device(device: torch.device):
-    """Context in which ``device`` is current: a launch on another device's
-    stream than the current one's would fail."""
-    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+def call(device: torch.device, function, *args) -> None:
+    """``check(function(*args, stream))`` on the current stream of ``device``,
+    with ``device`` current: a launch on another device's stream than the
+    current one's would fail."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status)
 
 
 def host_device_pointer(t: torch.Tensor) -> int:

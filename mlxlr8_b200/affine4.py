@@ -68,12 +68,9 @@ def affine4_linear(x, codes, scales, biases=None, *, x_scales=None, out_dtype=No
         _lib.refuse_overlap(out, x, codes, scales, biases, x_scales)
     x, codes, scales = _lib.aligned(x), _lib.aligned(codes), scales.contiguous()
     biases = biases.contiguous() if biases is not None else None
-    with _lib.on_device(device):
-        _lib.check(_lib.lib().exlr8_affine4_linear(x.data_ptr(), x_code, _lib.ptr(x_scales), x_group,
-                                                   x.numel() // in_features, in_features, out_features,
-                                                   codes.data_ptr(), scales.data_ptr(), _lib.ptr(biases),
-                                                   _lib.act_code(scales), group, out.data_ptr(), _lib.act_code(out),
-                                                   _lib.stream_handle(device)))
+    _lib.call(device, _lib.lib().exlr8_affine4_linear, x.data_ptr(), x_code, _lib.ptr(x_scales), x_group,
+              x.numel() // in_features, in_features, out_features, codes.data_ptr(), scales.data_ptr(),
+              _lib.ptr(biases), _lib.act_code(scales), group, out.data_ptr(), _lib.act_code(out))
     return out
 
 

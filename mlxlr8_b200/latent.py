@@ -105,13 +105,10 @@ def latent_append(latent, rope_key, cache, slots, *, weight=None, eps: float = 1
         q_rope = _rows(q_rope)
         q_strides = q_rope.stride()[:2]
         q_out = torch.empty_like(q_rope, memory_format=torch.contiguous_format)
-    with _lib.on_device(device):
-        _lib.check(_lib.lib().exlr8_latent_append(
-            latent.data_ptr(), latent.stride(0), rope_key.data_ptr(), rope_key.stride(0), tokens, rank,
-            _lib.act_code(cache), _lib.ptr(weight), float(eps), _lib.ptr(cos_sin),
-            0 if cos_sin is None else cos_sin.shape[0], _lib.ptr(positions), int(interleaved), slots.data_ptr(),
-            cache.data_ptr(), pages, page_size, _lib.ptr(q_rope), *q_strides, heads, _lib.ptr(q_out),
-            _lib.stream_handle(device)))
+    _lib.call(device, _lib.lib().exlr8_latent_append, latent.data_ptr(), latent.stride(0), rope_key.data_ptr(),
+              rope_key.stride(0), tokens, rank, _lib.act_code(cache), _lib.ptr(weight), float(eps), _lib.ptr(cos_sin),
+              0 if cos_sin is None else cos_sin.shape[0], _lib.ptr(positions), interleaved, slots.data_ptr(),
+              cache.data_ptr(), pages, page_size, _lib.ptr(q_rope), *q_strides, heads, _lib.ptr(q_out))
     return q_out
 
 
@@ -161,11 +158,9 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
         raise ValueError("operand sizes or strides are outside what the operator takes")
     if workspace is None or workspace.nbytes < need:
         workspace = q_latent.new_empty(need, dtype=torch.uint8)
-    with _lib.on_device(device):
-        _lib.check(_lib.lib().exlr8_latent_attention(
-            q_latent.data_ptr(), q_rope.data_ptr(), batch, queries, heads, rank, _lib.act_code(cache), cache.data_ptr(),
-            pages, page_size, block_table.data_ptr(), table_width, lengths.data_ptr(), float(scale), out.data_ptr(),
-            _lib.ptr(lse), workspace.data_ptr(), workspace.nbytes, _lib.stream_handle(device)))
+    _lib.call(device, _lib.lib().exlr8_latent_attention, q_latent.data_ptr(), q_rope.data_ptr(), batch, queries, heads,
+              rank, _lib.act_code(cache), cache.data_ptr(), pages, page_size, block_table.data_ptr(), table_width,
+              lengths.data_ptr(), float(scale), out.data_ptr(), _lib.ptr(lse), workspace.data_ptr(), workspace.nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -224,12 +219,10 @@ def latent_prompt_attention(q, k, k_rope, v, q_starts, k_starts, scale: float, *
     else:
         _lib.refuse_overlap(out, q, k, k_rope, v, q_starts, k_starts)
     lse = q.new_empty((total_q, heads), dtype=torch.float32) if return_lse else None
-    with _lib.on_device(device):
-        _lib.check(_lib.lib().exlr8_latent_prompt_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), k_rope.data_ptr(),
-            k_rope.stride(0), v.data_ptr(), v.stride(0), v.stride(1), total_q, total_k, heads, nope, value,
-            _lib.act_code(q), q_starts.data_ptr(), k_starts.data_ptr(), seqs, float(scale), out.data_ptr(),
-            _lib.ptr(lse), _lib.stream_handle(device)))
+    _lib.call(device, _lib.lib().exlr8_latent_prompt_attention, q.data_ptr(), *q.stride()[:2], k.data_ptr(),
+              *k.stride()[:2], k_rope.data_ptr(), k_rope.stride(0), v.data_ptr(), *v.stride()[:2], total_q, total_k,
+              heads, nope, value, _lib.act_code(q), q_starts.data_ptr(), k_starts.data_ptr(), seqs, float(scale),
+              out.data_ptr(), _lib.ptr(lse))
     return (out, lse) if return_lse else out
 
 

@@ -73,11 +73,8 @@ def residual_rms_norm_q8(x, weight, eps: float = 1e-5, residual=None, group: int
     codes = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     scales = x.new_empty((*shape[:-1], hidden // group), dtype=torch.float32)
     h = torch.empty_like(x) if return_sum else None
-    with _lib.on_device(device):
-        _lib.check(_lib.lib().exlr8_residual_rms_norm_q8(x.data_ptr(), _lib.ptr(res), w.data_ptr(), code,
-                                                         x.numel() // hidden, hidden, group, eps, _lib.ptr(h),
-                                                         codes.data_ptr(), scales.data_ptr(),
-                                                         _lib.stream_handle(device)))
+    _lib.call(device, _lib.lib().exlr8_residual_rms_norm_q8, x.data_ptr(), _lib.ptr(res), w.data_ptr(), code,
+              x.numel() // hidden, hidden, group, float(eps), _lib.ptr(h), codes.data_ptr(), scales.data_ptr())
     return (h, codes, scales) if return_sum else (codes, scales)
 
 
