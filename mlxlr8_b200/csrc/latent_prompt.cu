@@ -42,9 +42,14 @@
 // over the operands, and joins a part of the rows from all of them, in the order
 // of the shares.
 //
-// 8192 queries of 32 heads (128 + 64 key and 128 value channels): 551 us, 1247
-// TFLOP/s, the tensor pipe bound; 5 prompts of 1300 tokens, 16 heads: 26 us, the
-// longest one's keys in turn (2000 cycles a tile).
+// A tile of at most 128 queries leaves one query tile empty: its key tiles go to
+// the two softmax groups in turn, so that the products of one run under the
+// weights of the other (82 queries of six sequences over 2000 keys each, 24
+// heads: 40 -> 28 us).
+//
+// 8192 queries of 32 heads (128 + 64 key and 128 value channels): 551 to 600 us
+// with the power that is left, 1247 to 1146 TFLOP/s, the tensor pipe bound; 5 prompts of 1300 tokens, 16 heads: 25 us, the
+// longest one's keys in turn (2900 cycles a tile for 256 queries).
 
 #include <cuda.h>
 
@@ -147,6 +152,10 @@ __device__ __forceinline__ float2 load_cluster2(const void* p, int rank) {
                : "=f"(v.x), "=f"(v.y)
                : "r"(cluster_addr(smem_u32(p), rank)));
   return v;
+}
+
+__device__ __forceinline__ float4 join(const float4& a, float f, const float4& b, float g) {
+  return make_float4(fmaf(a.x, f, b.x * g), fmaf(a.y, f, b.y * g), fmaf(a.z, f, b.z * g), fmaf(a.w, f, b.w * g));
 }
 
 // Lane and lane ^ off exchange: the one without the bit keeps its x and takes the
@@ -271,25 +280,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int q = 0; q < 2; ++q) tiles[q] = max(min(tiles[q], end) - begin, 0);
   }
   const int all = max(tiles[0], tiles[1]);
+  // One query tile alone: both softmax groups take its key tiles in turn, each
+  // with a maximum, a sum and an output of its own, joined at the end.
+  const bool lone = first + kTileQ >= queries;
   const int own0 = k0 + begin * kKeys;  // the share's first key
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
     if (warp == 0) {
       if (lane == 0 && all > 0) {
         bool ok = true;
-        mbar_arrive_expect_tx(&sh.q_full, 2 * T::kQ);
-        for (int q = 0; q < 2; ++q)
+        mbar_arrive_expect_tx(&sh.q_full, lone ? T::kQ : 2 * T::kQ);
+        for (int q = 0; q < (lone ? 1 : 2); ++q)
           for (int b = 0; b < kBlocks; ++b)
             load_tile(smem + q * T::kQ + b * 16384, &maps.q, maps.q_swap, 64 * b, head, q0 + first + q * kTileQ,
                       &sh.q_full);
-        // Unit 2 j is key tile j, unit 2 j + 1 value tile j.  `used` blocks have been
-        // given out since the start, `freed` given back.
+        // Units in the order of their use: K_0 V_0 K_1 V_1 ..., for a lone query tile
+        // K_0 K_1 V_0 K_2 V_1 ... V_n-2 V_n-1.  `used` blocks have been given out
+        // since the start, `freed` given back.
+        const int units = 2 * all;
+        auto is_value = [&](int u) { return !lone ? (u & 1) != 0 : u + 1 == units || (u > 0 && (u & 1) == 0); };
         int unit = 0, gone = 0, used = 0, freed = 0, at = 0;
-        for (; unit < 2 * all && ok; ++unit) {
-          const int j = unit >> 1, n = unit & 1 ? vb : kBlocks;
+        for (; unit < units && ok; ++unit) {
+          const bool value = is_value(unit);
+          const int n = value ? vb : kBlocks;
+          const int j = !lone ? unit / 2 : value ? (unit + 1 == units ? all : unit / 2) - 1 : (unit + 1) / 2;
           while (ok && used + n - freed > T::kRing) {
             ok = mbar_wait(&sh.empty[gone % kUnits], (gone / kUnits) & 1);
-            freed += gone & 1 ? vb : kBlocks;
+            freed += is_value(gone) ? vb : kBlocks;
             ++gone;
           }
           if (!ok) break;
@@ -297,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive_expect_tx(full, n * T::kBlock);
           for (int b = 0; b < n; ++b) {
             uint8_t* dst = ring + at * T::kBlock;
-            if (unit & 1) load_tile(dst, &maps.v, maps.v_swap, 128 * part + 64 * b, head, own0 + j * kKeys, full);
+            if (value) load_tile(dst, &maps.v, maps.v_swap, 128 * part + 64 * b, head, own0 + j * kKeys, full);
             else if (b < kBlocks - 1) load_tile(dst, &maps.k, maps.k_swap, 64 * b, head, own0 + j * kKeys, full);
             else tma_load_2d(dst, &maps.r, 0, own0 + j * kKeys, full);
             if (++at == T::kRing) at = 0;
@@ -329,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // S_q of a key tile.
       auto scores = [&](int q, const uint32_t* kt) {
-        const uint32_t qt = sq + q * (T::kQ >> 4);
+        const uint32_t qt = sq + (lone ? 0 : q) * (T::kQ >> 4);
         if (elect_one()) {
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b)
@@ -351,60 +368,102 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) tc_commit(&sh.empty[0]);
         __syncwarp();
       }
-      for (int j = 0; j < steps && ok; ++j) {
-        const int unit = 2 * j + 1;
-        ok = warp_wait(&sh.full[unit % kUnits], (unit / kUnits) & 1);
-        if (!ok) break;
+      // The blocks of value tile j; rows behind the sequence's last key are zeroed.
+      // Whether they lie in a row.
+      auto values = [&](int j) {
         const int first_block = at;
         blocks(sv, vb, vt);
         const int valid = uniform(keys - begin * kKeys) - j * kKeys;
-        if (valid < kKeys) {  // rows behind the sequence's last key
+        if (valid < kKeys) {
           for (int b = 0; b < vb; ++b) {
-            uint8_t* tile = ring + (first_block + b < T::kRing ? first_block + b : first_block + b - T::kRing) * T::kBlock;
+            const int block = first_block + b < T::kRing ? first_block + b : first_block + b - T::kRing;
             for (int i = lane; i < (kKeys - valid) * 8; i += 32)
-              reinterpret_cast<uint4*>(tile + valid * 128)[i] = make_uint4(0, 0, 0, 0);
+              reinterpret_cast<uint4*>(ring + block * T::kBlock + valid * 128)[i] = make_uint4(0, 0, 0, 0);
           }
           fence_async_smem();
           __syncwarp();
         }
-        const bool joined = vb == 1 || first_block + 1 < T::kRing;  // the value blocks lie in a row
-        const bool more = j + 1 < steps;
-        bool next = !more;  // key tile j + 1 has arrived
+        return vb == 1 || first_block + 1 < T::kRing;
+      };
+      // O_q (+)= P_q V; one thread.
+      auto product = [&](int q, bool joined, bool more) {
+        if (joined) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int n = q ? n1 : n0;
-          if (!ok || j >= n) continue;
-          ok = warp_wait(&sh.p_ready[q], j & 1);
-          if (!ok) continue;
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            tc_mma_f16_ts(td + 256 + q * 128, td + q * 128 + kk * 8, desc_of(vt[0] + (kk * 2048 >> 4)), value_desc,
+                          kk > 0 || more);
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+              tc_mma_f16_ts(td + 256 + q * 128 + 64 * b, td + q * 128 + kk * 8, desc_of(vt[b] + (kk * 2048 >> 4)),
+                            half_desc, kk > 0 || more);
+        }
+      };
+      if (lone) {
+        int unit = 1;
+        // The next unit, a key tile, against Q_0 into S_q.
+        auto next_scores = [&](int q) {
+          ok = warp_wait(&sh.full[unit % kUnits], (unit / kUnits) & 1);
+          if (!ok) return;
+          tc_fence_after();
+          blocks(sk, kBlocks, kt);
+          scores(q, kt);
+          if (elect_one()) tc_commit(&sh.empty[unit % kUnits]);
+          __syncwarp();
+          ++unit;
+        };
+        if (ok && steps > 1) next_scores(1);
+        for (int j = 0; j < steps && ok; ++j) {
+          const int q = j & 1;
+          ok = warp_wait(&sh.full[unit % kUnits], (unit / kUnits) & 1);
+          if (!ok) break;
+          const bool joined = values(j);
+          ok = warp_wait(&sh.p_ready[q], (j >> 1) & 1);
+          if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            if (joined) {
-#pragma unroll
-              for (int kk = 0; kk < kKeys / 16; ++kk)
-                tc_mma_f16_ts(td + 256 + q * 128, td + q * 128 + kk * 8, desc_of(vt[0] + (kk * 2048 >> 4)), value_desc,
-                              kk > 0 || j > 0);
-            } else {
-#pragma unroll
-              for (int kk = 0; kk < kKeys / 16; ++kk)
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-                  tc_mma_f16_ts(td + 256 + q * 128 + 64 * b, td + q * 128 + kk * 8, desc_of(vt[b] + (kk * 2048 >> 4)),
-                                half_desc, kk > 0 || j > 0);
-            }
-            if (j + 1 >= n) tc_commit(&sh.o_done[q]);
-            if (q == 1 || j >= n1) tc_commit(&sh.empty[unit % kUnits]);  // the value tile's last use
+            product(q, joined, j > 1);
+            if (j + 2 >= steps) tc_commit(&sh.o_done[q]);
+            tc_commit(&sh.empty[unit % kUnits]);
           }
           __syncwarp();
-          if (!next) {
-            ok = warp_wait(&sh.full[(unit + 1) % kUnits], ((unit + 1) / kUnits) & 1);
-            tc_fence_after();
-            blocks(sk, kBlocks, kt);
-            next = true;
-          }
-          if (ok && j + 1 < n) scores(q, kt);
+          ++unit;
+          if (j + 2 < steps) next_scores(q);
         }
-        if (ok && more && elect_one()) tc_commit(&sh.empty[(unit + 1) % kUnits]);
-        __syncwarp();
+      } else {
+        for (int j = 0; j < steps && ok; ++j) {
+          const int unit = 2 * j + 1;
+          ok = warp_wait(&sh.full[unit % kUnits], (unit / kUnits) & 1);
+          if (!ok) break;
+          const bool joined = values(j);
+          const bool more = j + 1 < steps;
+          bool next = !more;  // key tile j + 1 has arrived
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int n = q ? n1 : n0;
+            if (!ok || j >= n) continue;
+            ok = warp_wait(&sh.p_ready[q], j & 1);
+            if (!ok) continue;
+            tc_fence_after();
+            if (elect_one()) {
+              product(q, joined, j > 0);
+              if (j + 1 >= n) tc_commit(&sh.o_done[q]);
+              if (q == 1 || j >= n1) tc_commit(&sh.empty[unit % kUnits]);  // the value tile's last use
+            }
+            __syncwarp();
+            if (!next) {
+              ok = warp_wait(&sh.full[(unit + 1) % kUnits], ((unit + 1) / kUnits) & 1);
+              tc_fence_after();
+              blocks(sk, kBlocks, kt);
+              next = true;
+            }
+            if (ok && j + 1 < n) scores(q, kt);
+          }
+          if (ok && more && elect_one()) tc_commit(&sh.empty[(unit + 1) % kUnits]);
+          __syncwarp();
+        }
       }
     }
     if constexpr (kSplit) {
@@ -415,15 +474,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int q = (warp - 4) / 4, quad = warp & 3;
-    const int row = first + q * kTileQ + quad * 32 + lane;
+    const int row = first + (lone ? 0 : q) * kTileQ + quad * 32 + lane;
+    const int count = !lone ? tiles[q] : (all + 1 - q) / 2;  // key tiles of this group
     const int seen = (row < queries ? min(keys - queries + 1 + row, keys) : 0) - begin * kKeys;  // of the share
     const uint32_t lanes = static_cast<uint32_t>(32 * quad) << 16;
     const uint32_t ts = tmem + lanes + q * 128, to = tmem + lanes + 256 + q * 128;
     const float c = fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
-    for (int j = 0; j < tiles[q]; ++j) {
-      ok = mbar_wait(&sh.s_full[q], j & 1);
+    for (int t = 0; t < count; ++t) {
+      const int j = lone ? 2 * t + q : t;
+      ok = mbar_wait(&sh.s_full[q], t & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t s[kKeys];
@@ -475,12 +536,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         sum = (s0 + s1) + (s2 + s3);
         grown = fmaxf(top[0], top[1]);
       };
-      if (j == 0) m = largest();
+      if (t == 0) m = largest();
       weigh();
       // Rarely a score has outgrown m: raise it, multiply what was summed, weigh
-      // the tile again.  PV of tile j - 1 is complete (this tile's scores were
-      // committed after it).
-      if (j > 0 && __any_sync(0xffffffffu, grown > kLift + kLag || (m == -INFINITY && grown > -INFINITY))) {
+      // the tile again.  PV of the group's last tile is complete (this tile's scores
+      // were committed after it).
+      if (t > 0 && __any_sync(0xffffffffu, grown > kLift + kLag || (m == -INFINITY && grown > -INFINITY))) {
         const float best = largest();
         const float keep = best > m ? exp2_fast((m - best) * c) : 1.0f;
         m = best;
@@ -502,24 +563,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       mbar_arrive(&sh.p_ready[q]);
     }
-    if (tiles[q] > 0 && ok) ok = mbar_wait(&sh.o_done[q], 0);
+    if (count > 0 && ok) ok = mbar_wait(&sh.o_done[q], 0);
     tc_fence_after();
-    if constexpr (kSplit) {
-      // The share's sums and outputs, over the operand tiles once both query
-      // tiles are done with them; 16-byte pieces swizzled by the row.
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const int r = q * kTileQ + quad * 32 + lane;
-      stats[r] = make_float2(m * c - kLift, ok ? l : NAN);
-      for (int i = 0; tiles[q] > 0 && i < 64 * vb; i += 32) {
+    // A lone tile's second group, and every CTA of a cluster, leaves its output in
+    // shared memory, over the operand tiles once both groups are done with them;
+    // 16-byte pieces swizzled by the row.
+    float unit = m * c - kLift, other = 0.0f, own = 1.0f;  // what O counts, log2; the parts' factors
+    const int r = q * kTileQ + quad * 32 + lane;
+    auto stage = [&](bool add) {
+      for (int i = 0; i < 64 * vb; i += 32) {
         uint32_t o[32];
         tc_ld32(to + i, o);
         tc_wait_ld();
         tc_settle<32>(o);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          staged[r * 32 + ((i / 4 + e) ^ (r & 7))] =
-              make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                          __uint_as_float(o[4 * e + 3]));
+        for (int e = 0; e < 8; ++e) {
+          float4 v = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                 __uint_as_float(o[4 * e + 3]));
+          if (add) v = join(v, own, staged[(r + kTileQ) * 32 + ((i / 4 + e) ^ (r & 7))], other);
+          staged[r * 32 + ((i / 4 + e) ^ (r & 7))] = v;
+        }
+      }
+    };
+    const bool both = lone && all > 1;  // the same for all threads
+    if (kSplit || both) asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (both) {
+      if (q == 1) {
+        stats[r] = make_float2(unit, ok ? l : NAN);
+        stage(false);
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (q == 0) {
+        const float2 v = stats[r + kTileQ];
+        const float top = fmaxf(l != 0.0f ? unit : -INFINITY, v.y != 0.0f ? v.x : -INFINITY);
+        own = l != 0.0f ? exp2_fast(unit - top) : 0.0f;
+        other = v.y != 0.0f ? exp2_fast(v.x - top) : 0.0f;
+        l = l * own + v.y * other;
+        unit = top;
+      }
+    }
+    if constexpr (kSplit) {
+      // (rows of a lone tile's second group are no query's)
+      if (!(lone && q == 1)) {
+        stats[r] = make_float2(unit, ok ? l : NAN);
+        if (count > 0) stage(both);
       }
       __syncwarp();
       cluster_sync();
@@ -571,18 +658,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       cluster_sync();  // no CTA leaves while its part is read
-    } else {
+    } else if (!(lone && q == 1)) {
       const bool store = row < queries;
       const int64_t at = (static_cast<int64_t>(q0) + row) * a.heads + head;
       if (a.lse && part == 0 && store)
-        a.lse[at] = !ok ? NAN : l > 0.0f ? (m * c - kLift + log2f(l)) * 0.6931471805599453f : (l == 0.0f ? -INFINITY : l);
+        a.lse[at] = !ok ? NAN : l > 0.0f ? (unit + log2f(l)) * 0.6931471805599453f : (l == 0.0f ? -INFINITY : l);
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       for (int i = 0; i < 64 * vb; i += 32) {
         uint32_t o[32];
-        if (tiles[q] > 0) {
+        if (count > 0) {
           tc_ld32(to + i, o);
           tc_wait_ld();
           tc_settle<32>(o);
+        }
+        if (both) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 p = staged[(r + kTileQ) * 32 + ((i / 4 + e) ^ (r & 7))];
+            o[4 * e] = __float_as_uint(fmaf(__uint_as_float(o[4 * e]), own, p.x * other));
+            o[4 * e + 1] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 1]), own, p.y * other));
+            o[4 * e + 2] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 2]), own, p.z * other));
+            o[4 * e + 3] = __float_as_uint(fmaf(__uint_as_float(o[4 * e + 3]), own, p.w * other));
+          }
         }
         uint4 w[4];
 #pragma unroll

@@ -463,6 +463,27 @@ def test_prompt_with_keys_shared_by_several_ctas(dtype, queries, keys, heads, no
     assert torch.equal(_prompt(q, k, kr, v, queries, keys, 1.5 * (nope + 64) ** -0.5), got)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("queries, keys, heads, nope, value", [
+    ([128], [640], 2, 128, 128), ([17, 100], [700, 900], 2, 192, 192), ([1, 1, 1], [129, 256, 2000], 3, 64, 256),
+    ([384, 60], [384, 60], 30, 64, 64),
+])
+def test_prompt_lone_tiles_of_queries(dtype, queries, keys, heads, nope, value):
+    """At most 128 queries in a tile of 256: its keys go to two groups in turn,
+    whose maxima differ with rising, falling and mixed scores."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(sum(keys) + heads)
+    q, k, kr, v = _operands(g, queries, keys, heads, nope, value, torch_dtype(dtype))
+    _prompt(q, k, kr, v, queries, keys, 1.5 * (nope + 64) ** -0.5)
+    n = sum(keys)
+    q[..., 0] = 8.0
+    ramp = torch.linspace(-6, 6, n, device="cuda")
+    for order in (ramp, ramp.flip(0), ramp[torch.randperm(n, generator=g, device="cuda")]):
+        k[:, :, 0] = order.to(k.dtype)[:, None]
+        _prompt(q, k, kr, v, queries, keys, 0.5)
+
+
 def test_prompt_takes_views_and_leaves_other_rows():
     import torch
 
