@@ -21,7 +21,8 @@
 //
 // Work is the flat list of (sequence, row tile, 64 tokens), cut evenly over
 // the CTAs (one per SM) whatever the lengths; a sequence cut in two or more
-// leaves float32 parts in the workspace, which a second kernel joins.
+// leaves float32 parts in the workspace, which a second kernel joins, in the
+// order of the list.
 //
 // Warp 0 loads (TMA; one box per page or 16 to 64 of its tokens), warps 1 and 2
 // issue the two products, so that the scores of the next tile are formed while
@@ -38,8 +39,8 @@
 // that it concerns.
 //
 // 64 heads of rank 512, bfloat16: 64 sequences of up to 12000 tokens 139 us (4.8
-// TB/s of cache; HBM bound but for the slowest CTA and the join, 12 and 7 us);
-// one of 16000 18.5 us (parts written and joined, 10 us of it).
+// TB/s of cache; HBM bound but for the first and last tiles and the join, 7 us);
+// one of 16000 18.6 us (parts written and joined, 10 us of it).
 
 #include <cuda.h>
 
@@ -77,12 +78,23 @@ __device__ __forceinline__ int tokens_of(const Work& w, int64_t b) {
 }
 __device__ __forceinline__ int tiles_of(const Work& w, int64_t b) { return (tokens_of(w, b) + kTile - 1) / kTile; }
 
-// Tiles of all sequences, and the CTAs that share them; the calling warp takes
-// part as a whole.  A CTA takes two tiles at least, where one each would cut
-// sequences in more than half as many places as there are CTAs (the parts are
-// what a short call spends its time on: 9 sequences of up to 1167 tokens and 64
-// rows, 25 us with two and 29 with one; 5 of up to 700 and 60 rows, 23 and 19).
-__device__ void total_tiles(const Work& w, int ctas, int lane, int64_t* total, int64_t* sharers) {
+// The list that the CTAs share: every (sequence, row tile) has its tiles and
+// `extra` further places that stand for what a segment costs besides them
+// (queries, first scores, output), where shares are long enough to be evened
+// out (21 sequences of up to 291 tokens and 320 rows: 30 us without, 26 with; 3 of
+// up to 28084 and 40 rows: 36 and 34; 64 of up to 12000 and 64 rows: 138 both).
+struct List {
+  int64_t total, sharers;  // places, CTAs
+  int extra;
+};
+constexpr int kSegmentCost = 2;
+
+// The calling warp takes part as a whole.  A CTA takes two tiles at least, where
+// one each would cut sequences in more than half as many places as there are
+// CTAs (the parts are what a short call spends its time on: 9 sequences of up to
+// 1167 tokens and 64 rows, 25 us with two and 29 with one; 5 of up to 700 and 60
+// rows, 23 and 19).
+__device__ List list_of(const Work& w, int ctas, int lane) {
   int64_t n = 0, sequences = 0;
   for (int64_t b = lane; b < w.batch; b += 32) {
     const int tiles = tiles_of(w, b);
@@ -94,44 +106,68 @@ __device__ void total_tiles(const Work& w, int ctas, int lane, int64_t* total, i
     n += __shfl_xor_sync(0xffffffffu, n, off);
     sequences += __shfl_xor_sync(0xffffffffu, sequences, off);
   }
-  *total = n * w.row_tiles;
-  const int64_t least = (n - sequences) * w.row_tiles > ctas / 2 ? 2 : 1, most = (*total + least - 1) / least;
-  *sharers = most < ctas ? most : ctas;
+  n *= w.row_tiles;
+  sequences *= w.row_tiles;
+  const int64_t least = n - sequences > ctas / 2 ? 2 : 1, most = (n + least - 1) / least;
+  const int extra = n > 2 * ctas ? kSegmentCost : 0;
+  return List{n + extra * sequences, most < ctas ? most : ctas, extra};
 }
 
-// The sequence of flat tile `at` (at < total), and the tiles before it.
-__device__ void find_sequence(const Work& w, int64_t at, int lane, int64_t* sequence, int64_t* before) {
-  int64_t base = 0;
+// A place of the list: its sequence and row tile, that one's first place, the
+// tile (its number of tiles: one of the extra places), and the tiles before it.
+struct Spot {
+  int64_t sequence, start, before;
+  int rt, tile, tokens, tiles;
+};
+__device__ Spot find_place(const Work& w, const List& list, int64_t at, int lane) {
+  int64_t base = 0, sequences = 0;
   for (int64_t b0 = 0; b0 < w.batch; b0 += 32) {
     const int64_t b = b0 + lane;
-    const int64_t n = b < w.batch ? static_cast<int64_t>(tiles_of(w, b)) * w.row_tiles : 0;
+    const int tokens = b < w.batch ? tokens_of(w, b) : 0, tiles = (tokens + kTile - 1) / kTile;
+    const int64_t n = tiles > 0 ? static_cast<int64_t>(tiles + list.extra) * w.row_tiles : 0;
     int64_t end = n;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const int64_t other = __shfl_up_sync(0xffffffffu, end, off);
       if (lane >= off) end += other;
     }
-    const uint32_t mine = __ballot_sync(0xffffffffu, at < base + end);
+    const uint32_t some = __ballot_sync(0xffffffffu, tiles > 0), mine = __ballot_sync(0xffffffffu, at < base + end);
     if (mine) {
       const int which = __ffs(mine) - 1;
-      *sequence = b0 + which;
-      *before = base + __shfl_sync(0xffffffffu, end - n, which);
-      return;
+      Spot p;
+      p.sequence = b0 + which;
+      p.tokens = __shfl_sync(0xffffffffu, tokens, which);
+      p.tiles = __shfl_sync(0xffffffffu, tiles, which);
+      p.start = base + __shfl_sync(0xffffffffu, end - n, which);
+      sequences += __popc(some & ((1u << which) - 1));
+      p.before = p.start - list.extra * w.row_tiles * sequences;
+      p.tile = static_cast<int>(at - p.start);
+      p.rt = 0;
+      if (w.row_tiles > 1) {
+        const int64_t unit = p.tiles + list.extra;
+        p.rt = static_cast<int>((at - p.start) / unit);
+        p.tile = static_cast<int>((at - p.start) % unit);
+        p.start += p.rt * unit;
+        p.before += static_cast<int64_t>(p.rt) * p.tiles;
+      }
+      p.tile = min(p.tile, p.tiles);
+      p.before += p.tile;
+      return p;
     }
     base += __shfl_sync(0xffffffffu, end, 31);
+    sequences += __popc(some);
   }
-  *sequence = w.batch;
-  *before = base;
+  return Spot{w.batch, base, base - list.extra * w.row_tiles * sequences, 0, 0, 0, 0};
 }
 
-// The first tile of CTA i of n that share `total`.
+// The first place of CTA i of n that share `total`.
 __device__ __forceinline__ int64_t first_tile(int64_t i, int64_t total, int64_t n) {
   // (a 64-bit division takes longer than the lists that need one are common)
   if (total < (1 << 20)) return static_cast<uint32_t>(i) * static_cast<uint32_t>(total) / static_cast<uint32_t>(n);
   return i * total / n;
 }
 
-// The CTA of flat tile x: the last whose first tile is not behind it.
+// The CTA of place x: the last whose first place is not behind it.
 __device__ __forceinline__ int64_t owner_of(int64_t x, int64_t total, int64_t n) {
   if (total < (1 << 20)) return (static_cast<uint32_t>(x + 1) * static_cast<uint32_t>(n) - 1) / static_cast<uint32_t>(total);
   return ((x + 1) * n - 1) / total;
@@ -182,7 +218,8 @@ struct Shared {
   uint64_t full[kMaxPairs], empty[kMaxPairs], rope_full[2], rope_empty[2];
   uint32_t tmem;
   Walk walk;
-  int64_t at, total, sharers;  // the share's first tile; of all CTAs
+  List list;
+  int64_t start;  // first place of the (sequence, row tile) in which the share begins
   __align__(16) float base[64];
   __align__(16) float factor[64];
   float m[64];
@@ -281,23 +318,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int blocks = a.rank / 64, tile_pairs = a.rank / 128;
   if (warp == 0) {
     pdl_wait();
-    int64_t total, n;
-    total_tiles(w, gridDim.x, lane, &total, &n);
+    const List list = list_of(w, gridDim.x, lane);
     Walk walk{};
-    if (blockIdx.x < n) {
-      const int64_t at = first_tile(blockIdx.x, total, n);
-      int64_t sequence, before;
-      find_sequence(w, at, lane, &sequence, &before);
-      walk.b = sequence;
-      walk.left = first_tile(blockIdx.x + 1, total, n) - at;
-      walk.tokens = tokens_of(w, sequence);
-      walk.tiles = (walk.tokens + kTile - 1) / kTile;
-      walk.rt = static_cast<int>((at - before) / walk.tiles);
-      walk.tile = static_cast<int>((at - before) % walk.tiles);
+    if (blockIdx.x < list.sharers) {
+      const int64_t next = first_tile(blockIdx.x + 1, list.total, list.sharers);
+      const Spot p = find_place(w, list, first_tile(blockIdx.x, list.total, list.sharers), lane);
+      const int64_t end = list.extra > 0 ? find_place(w, list, next, lane).before : next;
+      walk = Walk{p.sequence, end - p.before, p.rt, p.tile, p.tokens, p.tiles, 0, 0};
       if (lane == 0) {
-        sh.at = at;
-        sh.total = total;
-        sh.sharers = n;
+        sh.list = list;
+        sh.start = p.start;
       }
     }
     if (lane == 0) sh.walk = walk;
@@ -474,11 +504,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 3) {  // what the join needs to know
     if (lane == 0) {
       Cut cut{walk.b, walk.rt, 0, 0, 0};
-      if (walk.tile > 0) {
-        const int64_t start = sh.at - walk.tile;
-        cut.first = static_cast<int>(owner_of(start, sh.total, sh.sharers));
-        cut.count = static_cast<int>(owner_of(start + walk.tiles - 1, sh.total, sh.sharers)) - cut.first + 1;
-        cut.slot = cut.first + (first_tile(cut.first, sh.total, sh.sharers) < start ? gridDim.x : 0);
+      if (walk.tile > 0 && walk.tile < walk.tiles) {
+        const List list = sh.list;
+        cut.first = static_cast<int>(owner_of(sh.start, list.total, list.sharers));
+        cut.count =
+            static_cast<int>(owner_of(sh.start + walk.tiles - 1, list.total, list.sharers)) - cut.first + 1;
+        // (tiles of its own before these, not only extra places)
+        const bool second = first_tile(cut.first, list.total, list.sharers) < sh.start - list.extra;
+        cut.slot = cut.first + (second ? gridDim.x : 0);
       }
       cuts[blockIdx.x] = cut;
     }

@@ -214,6 +214,24 @@ def test_absorbed_matches_the_formula(dtype, lengths, queries, heads, rank, page
     _absorbed(ql, qr, cache, table, lengths, 2.0 * (rank + 64) ** -0.5)
 
 
+@pytest.mark.parametrize("lengths, queries, heads, rank, page", [
+    ([7000, 1, 0, 64, 9000, 4500, 130], 2, 40, 128, 64), ([500 + 7 * i for i in range(70)], 1, 64, 128, 16),
+    ([3000] * 20 + [0, 1] * 9, 1, 16, 256, 48), ([65] * 160, 3, 48, 128, 80), ([200] * 150, 1, 8, 384, 32),
+])
+def test_absorbed_shares_of_many_segments(lengths, queries, heads, rank, page):
+    """Enough tiles that the segments' own cost is evened out over the CTAs:
+    shares that begin and end inside, between and behind sequences."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(sum(lengths) + heads)
+    cache, table = _paged(g, lengths, rank, page, torch.bfloat16, garbage=float("nan"))
+    ql = torch.randn(len(lengths), queries, heads, rank, generator=g, device="cuda").bfloat16()
+    qr = torch.randn(len(lengths), queries, heads, 64, generator=g, device="cuda").bfloat16()
+    scale = 2.0 * (rank + 64) ** -0.5
+    got = _absorbed(ql, qr, cache, table, lengths, scale)
+    assert torch.equal(_absorbed(ql, qr, cache, table, lengths, scale), got)
+
+
 @pytest.mark.parametrize("garbage", [float("nan"), float("inf"), -3e38])
 def test_absorbed_ignores_what_lies_past_a_length(garbage):
     import torch
@@ -615,3 +633,34 @@ def test_absorbed_many_short_sequences():
     half = 2.0 ** -8  # rounded weights, rounded output; scores and sums in float32 are far below
     expected, weight = (torch.einsum("bhn,bnd->bhd", p, r) for r in (rows, rows.abs()))
     _close(got[:, 0], expected, 1.02 * half * (weight + expected.abs()) + 2.0 ** -25)
+
+
+def test_attention_forms_side_by_side_on_two_streams():
+    """Calls that overlap on the GPU, each with its own workspace."""
+    import torch
+
+    from mlxlr8_b200.latent import latent_attention, latent_prompt_attention
+
+    g = torch.Generator(device="cuda").manual_seed(97)
+    q, k, kr, v = _operands(g, [165], [2165], 4, 128, 128, torch.bfloat16)
+    qs, ks = (torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (165, 2165))
+    cache, table = _paged(g, [5000, 900], 512, 64, torch.bfloat16)
+    lengths = torch.tensor([5000, 900], dtype=torch.int32, device="cuda")
+    ql, qr = (torch.randn(2, 1, 64, n, generator=g, device="cuda").bfloat16() for n in (512, 64))
+
+    def prompt():
+        return latent_prompt_attention(q, k, kr, v, qs, ks, 0.1)
+
+    def absorbed():
+        return latent_attention(ql, qr, cache, table, lengths, 0.05)
+
+    first = prompt(), absorbed()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(4):
+        for stream, call in zip(streams, (prompt, absorbed, absorbed)):
+            with torch.cuda.stream(stream):
+                got.append((call is absorbed, call()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, first[which]) for which, out in got)
