@@ -227,6 +227,8 @@ struct Shared {
   int limit[64];
 };
 
+static_assert(sizeof(Shared) <= 3072, "leaves room for two tiles of rank 512 beside 64 rows");
+
 // A tile of the ring and the parity of its round.  (Counted, not divided, and
 // of whole tiles, so that the issuing warps add constants to one base a tile:
 // with a division, and later a broadcast, per pair they were the bound.)
@@ -308,8 +310,8 @@ __device__ __forceinline__ float fold(const float (&v)[kN], int lane, F f) {
 // [kN][2 * CTAs] pairs (log2 of the unit of O and the sum, the sum).
 template <int kAct, int kN>
 __global__ void __launch_bounds__(kThreads, 1)
-    latent_attention_kernel(const __grid_constant__ Maps maps, const LatentAttentionArgs a, const Work w, const Layout lay,
-                            int box, uint32_t columns, float* __restrict__ parts, float2* __restrict__ sums,
+    latent_attention_kernel(const __grid_constant__ Maps maps, const LatentAttentionArgs a, const Work w,
+                            const Layout lay, int box, uint32_t columns, float* __restrict__ parts, float2* __restrict__ sums,
                             Cut* __restrict__ cuts) {
   pdl_launch_dependents();
   extern __shared__ __align__(1024) uint8_t smem[];  // (nothing static lies before it)
