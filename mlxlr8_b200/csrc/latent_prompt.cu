@@ -80,11 +80,13 @@ struct Tiles {
   static constexpr uint32_t kBlock = kKeys * 128;    // 64 channels of a key or value tile
   static constexpr int kRing = (kSmem - 2 * kQ) / kBlock;
   static_assert(kRing >= kBlocks + 4, "a key tile and two value tiles");
+  // Of eight units in a row three at least are key tiles, the others a block each.
+  static_assert(3 * kBlocks + 5 > kRing, "kUnits units lie in the ring at once");
 };
 
 constexpr int kSplitGroups = 80;  // tiles of queries from which no two CTAs per tile would fit the GPU
 
-constexpr int kUnits = 8;  // key and value tiles that the barriers tell apart; the ring holds five at most
+constexpr int kUnits = 8;  // key and value tiles that the barriers tell apart
 
 struct Shared {
   uint64_t q_full, full[kUnits], empty[kUnits];
