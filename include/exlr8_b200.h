@@ -582,8 +582,9 @@ int exlr8_residual_rms_norm(const void* x, const void* residual, const void* wei
  * and per group of `group` channels (32, 64, 128 or hidden; a divisor of
  * hidden)
  *   scale = max|y| / 448,  code = e4m3(y / scale).
- * A group of zeros has scale 0 and codes 0; a group with a value that is not
- * finite has scale NaN and codes 0.  codes uint8 [rows][hidden], scales
+ * A group of zeros, or whose scale lies below the smallest float32, has scale 0
+ * and codes 0; a group with a value that is not finite has scale NaN and codes
+ * 0.  codes uint8 [rows][hidden], scales
  * float32 [rows][hidden / group].  No counterpart in the reference, whose
  * norm (exlr8/fast_norm.py) has 16-bit outputs. */
 int exlr8_residual_rms_norm_q8(const void* x, const void* residual, const void* weight, int x_dtype, int64_t rows,

@@ -7,7 +7,8 @@
 // roundings are h (an output in the activation type, as in norm.cu) and the
 // code, which saturates at 448 by construction.  A group of zeros has scale 0
 // and codes 0; a group with a value that is not finite has scale NaN and
-// codes 0, so that every value it stands for is NaN.
+// codes 0, so that every value it stands for is NaN.  A scale below the smallest
+// float32 is 0, and its codes with it.
 //
 // Bound by memory: 8192 x 6144 bfloat16 with residual and groups of 128, 354 MB,
 // 61.7 us or 5.7 TB/s; one scale a row 52.7 us; one row 2.2 us, a launch.
@@ -34,6 +35,22 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+
+// The codes come from h w and its largest magnitude t over the group, the scale
+// from t inv: 448 / t is infinite for t below 2^-119, and h w may leave float32's
+// range where h inv w does not.  Where t is outside [2^-100, the largest float],
+// and not 0, h is lifted by this power of two before the product with w, and
+// the scale takes it back.  (|h| is below 2^64 or the sum of its squares
+// infinite; then inv is 0 and the product with it is the formula's own.)
+__device__ __forceinline__ bool outside(float t) {
+  constexpr uint32_t kLeast = (127 - 100) << 23, kInfinity = 0x7f800000;
+  // (the common answer takes one comparison; zeros and NaN are not lifted)
+  return __float_as_uint(t) - kLeast >= kInfinity - kLeast && t > 0.0f;
+}
+__device__ __forceinline__ float lift_of(float t, float inv) {
+  return inv == 0.0f ? 0.0f : t < 1.0f ? 0x1p64f : 0x1p-64f;
+}
+__device__ __forceinline__ float unlift_of(float t) { return t < 1.0f ? 0x1p-64f : 0x1p64f; }
 
 // Eight channels as stored: four words of two 16-bit values, or eight floats.
 template <int kAct>
@@ -147,14 +164,65 @@ __global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024)
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top[0] = max_nan(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
   }
+  // The products of vector i again, h lifted, from the inputs; their largest.
+  auto lifted = [&](int i, float lift) {
+    const int v = i * blockDim.x + threadIdx.x;
+    float most = 0.0f;
+    if (v < vecs) {
+      Eight<kAct> sum, other;
+      sum.load(x, base + 8 * v);
+      if (residual) {
+        other.load(residual, base + 8 * v);
+        sum.add(other);
+      }
+      other.load(w, 8 * v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[i][e] = sum.at(e) * lift * other.at(e);
+        most = max_nan(most, fabsf(y[i][e]));
+      }
+    }
+    return most;
+  };
+  float unlift[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) unlift[i] = 1.0f;
+  if (kWhole && outside(top[0])) {  // the same for all threads
+    const float lift = lift_of(top[0], inv);
+    unlift[0] = unlift_of(top[0]);
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) most = max_nan(most, lifted(i, lift));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
+    __syncthreads();  // the maxima of the products are read
+    if (lane == 0) red[1][threadIdx.x >> 5] = most;
+    __syncthreads();
+    top[0] = lane < warps ? red[1][lane] : 0.0f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top[0] = max_nan(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+  }
   const int lanes = group >> 3;  // threads of a group
+  bool some = false;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) some = some || outside(top[i]);
+  if (!kWhole && some) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      if (!outside(top[i])) continue;  // the same for the group's threads
+      const uint32_t mask = ((1u << lanes) - 1) << (lane & ~(lanes - 1));
+      unlift[i] = unlift_of(top[i]);
+      top[i] = lifted(i, lift_of(top[i], inv));
+      for (int off = lanes / 2; off > 0; off >>= 1) top[i] = max_nan(top[i], __shfl_xor_sync(mask, top[i], off));
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
     const int v = i * blockDim.x + threadIdx.x;
     if (v >= vecs) continue;
     const float t = kWhole ? top[0] : top[i];
     // inv is 0 in a row with an infinity, NaN in one with a NaN.
-    const float scale = t * inv / 448.0f;
+    const float scale = t * inv / 448.0f * unlift[kWhole ? 0 : i];
     const bool finite = t < __int_as_float(0x7f800000) && scale < __int_as_float(0x7f800000);
     const float mul = scale > 0.0f && finite ? 448.0f / t : 0.0f;
     uint32_t two[4];
@@ -173,7 +241,7 @@ __global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024)
 
 // One CTA per row, any hidden size and alignment.  kCached keeps h w of the row
 // in shared memory, so that the inputs are read once; rows beyond kCachedMax
-// channels read them again.  Single loads: 5000 x 7999 bfloat16 88 us, 3.2 TB/s
+// channels read them again.  Single loads: 5000 x 7999 bfloat16 84 us, 3.3 TB/s
 // (106 us with the inputs read three times).
 constexpr int kCachedMax = 24 * 1024;  // two CTAs of 96 KB per SM
 
@@ -194,7 +262,8 @@ __global__ void __launch_bounds__(kThreads) residual_rms_q8_any_kernel(const voi
     const float h = load_act(x, kAct, base + i);
     return residual ? round_to(kAct, h + load_act(residual, kAct, base + i)) : h;
   };
-  auto weighted = [&](int i) { return kCached ? cache[i] : sum_at(i) * load_act(w, kAct, i); };
+  float lift = 1.0f;
+  auto weighted = [&](int i) { return kCached ? cache[i] : sum_at(i) * lift * load_act(w, kAct, i); };
   float acc = 0.0f, row_top = 0.0f;
 #pragma unroll 4
   for (int i = threadIdx.x; i < hidden; i += kThreads) {
@@ -230,15 +299,35 @@ __global__ void __launch_bounds__(kThreads) residual_rms_q8_any_kernel(const voi
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
     }
-    const float scale = top * inv / 448.0f;
+    const int first = groups == 1 ? threadIdx.x : lane, step = groups == 1 ? kThreads : 32;
+    float unlift = 1.0f;
+    if (outside(top)) {  // the same for the threads of a group
+      lift = lift_of(top, inv);
+      unlift = unlift_of(top);
+      top = 0.0f;
+      for (int i = gi * group + first; i < (gi + 1) * group; i += step) {
+        const float y = sum_at(i) * lift * load_act(w, kAct, i);
+        if (kCached) cache[i] = y;
+        top = max_nan(top, fabsf(y));
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
+      if (groups == 1) {
+        __syncthreads();  // the maxima of the products are read
+        if (lane == 0) red[1][warp] = top;
+        __syncthreads();
+        for (int i = 0; i < kThreads / 32; ++i) top = max_nan(top, red[1][i]);
+      }
+    }
+    const float scale = top * inv / 448.0f * unlift;
     const bool finite = top < __int_as_float(0x7f800000) && scale < __int_as_float(0x7f800000);
     const float mul = scale > 0.0f && finite ? 448.0f / top : 0.0f;
-    const int first = groups == 1 ? threadIdx.x : lane, step = groups == 1 ? kThreads : 32;
 #pragma unroll 4
     for (int i = gi * group + first; i < (gi + 1) * group; i += step)
       codes[base + i] = finite ? to_e4m3(weighted(i) * mul) : 0;
     if (groups == 1 ? threadIdx.x == 0 : lane == 0)
       scales[static_cast<int64_t>(blockIdx.x) * groups + gi] = finite ? scale : __int_as_float(0x7fc00000);
+    lift = 1.0f;
   }
 }
 

@@ -122,3 +122,64 @@ def test_no_rows_and_refusals():
         residual_rms_norm_q8(x.double(), w)
     with pytest.raises(ValueError, match="CUDA"):
         residual_rms_norm_q8(x.cpu(), w)
+
+
+def _small_or_large(x, w, group, eps=1e-5):
+    """Codes and scales by the formula where a group's values are small or
+    large: a scale below the smallest float32 is 0, and its codes with it."""
+    import torch
+
+    from mlxlr8_b200.stack import residual_rms_norm_q8
+
+    codes, scales = residual_rms_norm_q8(x, w, eps, group=group)
+    _, blocks, es = _expected(x, w, None, group, eps, x.dtype)
+    s = scales.double().reshape(es.shape)
+    # float32 errors, and half a step of the smallest float32
+    assert bool(((s - es).abs() <= 48 * F32 * es + 2.0 ** -149).all())
+    q = codes.float().double().reshape(blocks.shape)
+    ratio = torch.where(s[..., None] > 0, blocks / es[..., None].clamp_min(1e-300), torch.zeros_like(blocks))
+    assert bool(((q - ratio).abs() <= ratio.abs() * (2.0 ** -4 + 96 * F32) + 2.0 ** -10).all())
+    return s
+
+
+TINY = (1e-44, 1e-42, 1e-40, 1e-38, 1e-37, 1e-36, 1.3e-36, 1.4e-36, 1e-33, 1e-30, 1e-24)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("hidden, group, offset", [
+    (512, 32, 0), (1024, 128, 0), (20480, 64, 0), (512, 64, 1), (33280, 128, 0),  # a group of an ordinary row
+    (512, 512, 0), (8192, 8192, 0), (333, 333, 0), (30001, 30001, 0), (512, 512, 1),  # the row
+])
+def test_groups_of_values_down_to_the_smallest(dtype, hidden, group, offset):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(hidden + group)
+    td = torch_dtype(dtype)
+    x = torch.randn(len(TINY), hidden, generator=g, device="cuda")
+    for i, top in enumerate(TINY):
+        part = x[i, : group]
+        part /= part.abs().max()
+        part[::3] = 0.0
+        part[1] = -1.0
+        # (products with the least values are formed without a flush to zero)
+        x[i, : group] = (part.double() * top).float()
+    w = (1.0 + 0.2 * torch.randn(hidden, generator=g, device="cuda")).to(td)
+    flat = torch.empty(x.numel() + offset, device="cuda", dtype=td)
+    flat[offset:] = x.to(td).flatten()
+    scales = _small_or_large(flat[offset:].view(x.shape), w, group)
+    assert bool((scales[3:, 0] > 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("hidden, group, offset", [(512, 32, 0), (512, 512, 0), (333, 333, 0), (512, 64, 1), (30001, 30001, 0)])
+def test_products_with_the_weight_past_the_largest_float(dtype, hidden, group, offset):
+    """h * w overflows, the normed h * w does not."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(hidden + group)
+    td = torch_dtype(dtype)
+    flat = (torch.randn(3 * hidden + offset, generator=g, device="cuda") * 1e12).to(td)
+    w = (1.0 + 0.2 * torch.randn(hidden, generator=g, device="cuda"))
+    w[: 16] *= 1e28
+    scales = _small_or_large(flat[offset:].view(3, hidden), w.to(td), group)
+    assert bool(scales.isfinite().all()) and bool((scales > 0).all())
