@@ -482,6 +482,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int r = 1; r < S::kGroups; ++r) v += sums[r * S::kOutputs + i];
     s_sum[i] = v;
   }
+  // (a cluster's barrier wants whole warps)
+  __syncwarp();
   if (shares > 1) cluster_sync();
   else __syncthreads();
   for (int i = share * kThreads + threadIdx.x; i < S::kOutputs; i += shares * kThreads) {
@@ -492,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int r = 1; r < shares; ++r) v += load_cluster(&s_sum[i], r);
     store_act(a.out, a.out_dtype, token * a.out_features + o, v);
   }
+  __syncwarp();  // (some lanes stored, others had no row)
   if (shares > 1) cluster_sync();  // no CTA of the cluster leaves while its sums are read
 }
 

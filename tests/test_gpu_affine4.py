@@ -197,3 +197,20 @@ def test_no_rows_and_refusals():
                  lambda: Affine4Linear(codes, scales[:4])):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("outer", [1, 31, 129, 4100, 5001])
+def test_widths_that_end_inside_a_warp_share_channels(outer):
+    """A cluster's last barrier behind rows that only some lanes store."""
+    import torch
+
+    from mlxlr8_b200.affine4 import Affine4Linear
+
+    g = torch.Generator(device="cuda").manual_seed(outer)
+    weights = _weights(g, outer, 8192, 128, torch.float16, True)
+    layer = Affine4Linear(*weights)
+    for rows in (1, 8, 16):
+        x = torch.randn(rows, 8192, generator=g, device="cuda").half()
+        first = _check(x, *weights)
+        for _ in range(20):
+            assert torch.equal(layer(x), first)
