@@ -253,7 +253,11 @@ __device__ __forceinline__ float exp2_fast(float v) {
   return r;
 }
 
-__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+// (by whole warps, like the barrier of a vote below)
+__device__ __forceinline__ void group_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+}
 __device__ __forceinline__ bool group_any(int id, bool v) {
   uint32_t r;
   asm volatile(
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int u = 0, segment = 0, loaded = 0;  // tiles, segments and pairs so far
     Place place;
     for (; ok && walk.next(w); ++segment) {
-      if (segment > 0) ok = mbar_wait(&sh.q_empty, (segment - 1) & 1);
+      if (segment > 0) ok = warp_wait(&sh.q_empty, (segment - 1) & 1);
       if (!ok) break;
       if (lane == 0) {
         mbar_arrive_expect_tx(&sh.q_full, (blocks + 1) * kN * 128);
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; ok && i < tile_pairs; ++i, ++loaded) {
           const int slot = place.stage * tile_pairs + i;
           uint64_t* full = &sh.full[slot];
-          ok = mbar_wait(&sh.empty[slot], place.round ^ 1);  // (passes in the first round)
+          ok = warp_wait(&sh.empty[slot], place.round ^ 1);  // (passes in the first round)
           if (!ok) break;
           if (lane == 0) mbar_arrive_expect_tx(full, 2 * bytes);
           __syncwarp();
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         place.advance(lay.stages);
         const int r = u & (lay.ropes - 1);
-        ok = mbar_wait(&sh.rope_empty[r], ((u >> (lay.ropes - 1)) & 1) ^ 1);
+        ok = warp_wait(&sh.rope_empty[r], ((u >> (lay.ropes - 1)) & 1) ^ 1);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&sh.rope_full[r], bytes);
         __syncwarp();

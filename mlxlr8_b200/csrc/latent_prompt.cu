@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int t = 0; t < count; ++t) {
       const int j = lone ? 2 * t + q : t;
-      ok = mbar_wait(&sh.s_full[q], t & 1);
+      ok = warp_wait(&sh.s_full[q], t & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t s[kKeys];
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       mbar_arrive(&sh.p_ready[q]);
     }
-    if (count > 0 && ok) ok = mbar_wait(&sh.o_done[q], 0);
+    if (count > 0 && ok) ok = warp_wait(&sh.o_done[q], 0);
     tc_fence_after();
     // A lone tile's second group, and every CTA of a cluster, leaves its output in
     // shared memory, over the operand tiles once both groups are done with them;
@@ -633,6 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           a.lse[(static_cast<int64_t>(q0) + at) * a.heads + head] =
               sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
       }
+      __syncwarp();
       asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll 2
       for (int i = warp - 4; i < rows; i += 8) {

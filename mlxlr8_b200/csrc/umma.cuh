@@ -92,7 +92,9 @@ __device__ __forceinline__ uint32_t desc_lo_rows128(uint32_t saddr, uint32_t blo
 }
 __device__ __forceinline__ uint64_t desc_of(uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | lo; }
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
-// mbar_wait by a whole warp with one answer, so that what follows stays uniform.
+// mbar_wait by a whole warp with one answer, so that what follows stays uniform:
+// a wait that runs out in some lanes alone would leave the others at a warp's
+// barrier or vote for good.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }

@@ -664,3 +664,27 @@ def test_attention_forms_side_by_side_on_two_streams():
                 got.append((call is absorbed, call()))
     torch.cuda.synchronize()
     assert all(torch.equal(out, first[which]) for which, out in got)
+
+
+def test_many_calls_of_both_forms_repeat_their_bits():
+    """Several segments a CTA, clusters whose rows are no multiple of a warp,
+    lone tiles: call after call."""
+    import torch
+
+    from mlxlr8_b200.latent import latent_attention, latent_prompt_attention
+
+    g = torch.Generator(device="cuda").manual_seed(100)
+    calls = []
+    for queries, keys in (([165], [2165]), ([17, 100], [700, 900]), ([300, 1, 40], [300, 129, 500])):
+        operands = _operands(g, queries, keys, 3, 128, 192, torch.bfloat16)
+        starts = [torch.tensor([0] + list(torch.tensor(n).cumsum(0)), dtype=torch.int32, device="cuda") for n in (queries, keys)]
+        calls.append(lambda o=operands, s=starts: latent_prompt_attention(*o, *s, 0.1))
+    for lengths in ([3000, 70, 0, 1], [200 + i for i in range(200)]):
+        cache, table = _paged(g, lengths, 256, 16, torch.bfloat16)
+        ql, qr = (torch.randn(len(lengths), 2, 24, n, generator=g, device="cuda").bfloat16() for n in (256, 64))
+        n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        calls.append(lambda a=(ql, qr, cache, table, n): latent_attention(*a, 0.05))
+    first = [call() for call in calls]
+    assert all(bool(out.isfinite().all()) for out in first)
+    for _ in range(60):
+        assert all(torch.equal(call(), out) for call, out in zip(calls, first))
