@@ -86,7 +86,14 @@ __global__ void __launch_bounds__(kVecThreads) latent_append_vec_kernel(const La
     }
   }
   const int first = a.interleaved ? 16 * v : 8 * v, second = a.interleaved ? 16 * v + 8 : 32 + 8 * v;
-  auto rotate = [&](const void* src, int64_t from, void* dst, int64_t to, bool write) {
+  auto rotate = [&](const void* src, int64_t from, void* dst, int64_t to) {
+    if (!a.cos_sin) {  // (0 times an infinity would reach the pair's other channel)
+      auto* const at = static_cast<uint16_t*>(dst) + to;
+      auto* const of = static_cast<const uint16_t*>(src) + from;
+      *reinterpret_cast<uint4*>(at + first) = *reinterpret_cast<const uint4*>(of + first);
+      *reinterpret_cast<uint4*>(at + second) = *reinterpret_cast<const uint4*>(of + second);
+      return;
+    }
     float x[8], y[8];
     load8<kAct>(src, from + first, x);
     load8<kAct>(src, from + second, y);
@@ -107,10 +114,8 @@ __global__ void __launch_bounds__(kVecThreads) latent_append_vec_kernel(const La
         y[i] = p * n[i] + q * c[i];
       }
     }
-    if (write) {
-      store8<kAct>(dst, to + first, x);
-      store8<kAct>(dst, to + second, y);
-    }
+    store8<kAct>(dst, to + first, x);
+    store8<kAct>(dst, to + second, y);
   };
   if (warp == 0) {
     if (!store) return;
@@ -125,7 +130,7 @@ __global__ void __launch_bounds__(kVecThreads) latent_append_vec_kernel(const La
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc = fmaf(x[i][e], x[i][e], acc);
     }
-    if (lane < 4) rotate(a.rope_key, t * a.rope_stride, a.cache, row + a.rank, true);
+    if (lane < 4) rotate(a.rope_key, t * a.rope_stride, a.cache, row + a.rank);
     if (a.weight) {
       __syncwarp();
 #pragma unroll
@@ -149,7 +154,7 @@ __global__ void __launch_bounds__(kVecThreads) latent_append_vec_kernel(const La
   } else if (a.q_rope) {
 #pragma unroll 2
     for (int h = (threadIdx.x - 32) >> 2; h < a.heads; h += (kVecThreads - 32) / 4)
-      rotate(a.q_rope, t * a.q_token_stride + h * a.q_head_stride, a.q_out, (t * a.heads + h) * kLatentRope, true);
+      rotate(a.q_rope, t * a.q_token_stride + h * a.q_head_stride, a.q_out, (t * a.heads + h) * kLatentRope);
   }
 }
 
@@ -200,7 +205,8 @@ __global__ void __launch_bounds__(kThreads) latent_append_kernel(const LatentApp
       c = known ? a.cos_sin[(static_cast<int64_t>(position) * 32 + p) * 2] : __int_as_float(0x7fc00000);
       n = known ? a.cos_sin[(static_cast<int64_t>(position) * 32 + p) * 2 + 1] : 0.0f;
     }
-    const float x = u * c - v * n, y = u * n + v * c;
+    // (without a table 0 times an infinity would reach the pair's other channel)
+    const float x = a.cos_sin ? u * c - v * n : u, y = a.cos_sin ? u * n + v * c : v;
     if (h < 0) {
       if (store) {
         store_act(a.cache, kAct, row + a.rank + first, x);

@@ -688,3 +688,30 @@ def test_many_calls_of_both_forms_repeat_their_bits():
     assert all(bool(out.isfinite().all()) for out in first)
     for _ in range(60):
         assert all(torch.equal(call(), out) for call, out in zip(calls, first))
+
+
+# ---- append without rotation, and views that no vector load fits -------------------
+
+
+@pytest.mark.parametrize("offset", [0, 3])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_append_without_a_table_copies_what_it_is_given(offset, interleaved):
+    """Infinities, NaN and signed zeros of a key and of queries stay in their channel."""
+    import torch
+
+    from mlxlr8_b200.latent import latent_append
+
+    g = torch.Generator(device="cuda").manual_seed(98)
+    for dtype in (torch.bfloat16, torch.float16):
+        kv = torch.randn(5, 192 + offset, generator=g, device="cuda").to(dtype)[:, offset:]
+        q = torch.randn(5, 3, 64 + offset, generator=g, device="cuda").to(dtype)[..., offset:]
+        for at, value in ((0, math.inf), (7, -math.inf), (33, math.nan), (40, 0.0), (41, -0.0)):
+            kv[:, 128 + at], kv[:, at], q[..., at] = value, value, value
+        cache = torch.zeros(1, 16, 192, device="cuda", dtype=dtype)
+        got = latent_append(kv[:, :128], kv[:, 128:], cache, torch.arange(5, device="cuda"), q_rope=q,
+                            interleaved=interleaved)
+        for copy, given in ((cache[0, :5], kv), (got, q)):
+            assert torch.equal(copy.isnan(), given.isnan())
+            kept = ~given.isnan()
+            assert torch.equal(copy[kept].view(torch.int16), given[kept].view(torch.int16))
+        assert not bool(cache[0, 5:].any())
