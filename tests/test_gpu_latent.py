@@ -715,3 +715,79 @@ def test_append_without_a_table_copies_what_it_is_given(offset, interleaved):
             kept = ~given.isnan()
             assert torch.equal(copy[kept].view(torch.int16), given[kept].view(torch.int16))
         assert not bool(cache[0, 5:].any())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("tokens, rank, heads, norm, rope, interleaved, odd", [
+    (1, 512, 64, True, True, True, "latent"), (33, 128, 1, True, True, False, "key"), (70, 384, 20, False, True, True, "head"),
+    (300, 256, 3, True, False, True, "latent"), (5, 512, 0, True, True, False, "weight"), (9, 256, 5, True, True, False, "token"),
+    (12, 128, 40, False, False, False, "key"), (8, 512, 7, True, True, True, "table"),
+])
+def test_append_of_unaligned_views_matches_the_formula(dtype, tokens, rank, heads, norm, rope, interleaved, odd):
+    """One operand off its 16 bytes, or with rows that are."""
+    import torch
+
+    from mlxlr8_b200.latent import latent_append, rope_table
+
+    g = torch.Generator(device="cuda").manual_seed(tokens + rank + heads)
+    td = torch_dtype(dtype)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(td)
+
+    latent = normal(tokens, rank + 9)[:, 1 : 1 + rank] if odd == "latent" else normal(tokens, rank)
+    key = normal(tokens + 1, 65)[1:, :64] if odd == "key" else normal(tokens, 64)
+    q = None
+    if heads:
+        q = {"head": lambda: normal(tokens, heads, 67)[..., :64],
+             "token": lambda: normal(tokens, heads * 64 + 2)[:, 2:].view(tokens, heads, 64)}.get(
+                 odd, lambda: normal(heads, tokens, 64).transpose(0, 1))()
+    flat = (1 + 0.1 * torch.randn(rank + 1, generator=g, device="cuda")).to(td)
+    w = (flat[1:] if odd == "weight" else flat[:rank]) if norm else None
+    table = None
+    if rope:
+        table = rope_table(901)[1:].contiguous()
+        if odd == "table":
+            shifted = torch.empty(table.numel() + 1, device="cuda")
+            shifted[1:] = table.flatten()
+            table = shifted[1:].view(table.shape)
+    cache = normal(40, 16, rank + 64)
+    slots = torch.randperm(640, generator=g, device="cuda")[:tokens]
+    at = torch.randint(0, 900, (tokens,), generator=g, device="cuda", dtype=torch.int32) if rope else None
+    if tokens > 4:
+        slots[1], slots[3] = -1, 640
+        if rope:
+            at[2], at[0] = -1, 900
+    before = cache.clone()
+    got = latent_append(latent, key, cache, slots, weight=w, cos_sin=table, positions=at, q_rope=q, interleaved=interleaved)
+    known = (at >= 0) & (at < 900) if rope else torch.ones(tokens, dtype=torch.bool, device="cuda")
+
+    def rotated(v):
+        v = v.double()
+        if not rope:
+            return v, torch.zeros_like(v)
+        cs = table[at.long().clamp(0, 899)].double()
+        c, n = (cs[..., i].reshape((tokens,) + (1,) * (v.dim() - 2) + (32,)) for i in (0, 1))
+        a, b = (v[..., 0::2], v[..., 1::2]) if interleaved else (v[..., :32], v[..., 32:])
+        size = a.abs() + b.abs()
+
+        def back(x, y):
+            return torch.stack([x, y], -1).flatten(-2) if interleaved else torch.cat([x, y], -1)
+
+        return back(a * c - b * n, a * n + b * c), back(size, size)
+
+    e = latent.double()
+    if norm:
+        e = e / (e.square().mean(1, keepdim=True) + 1e-5).sqrt() * w.double()
+    k, size = rotated(key)
+    half = torch.finfo(td).eps / 2
+    expected = before.double().view(-1, rank + 64)
+    tol = torch.zeros_like(expected)
+    kept = (slots >= 0) & (slots < 640) & known
+    expected[slots[kept]] = torch.cat([e, k], 1)[kept]
+    tol[slots[kept]] = torch.cat([e.abs() * (half + 64 * STEP), k.abs() * half + size * 4 * STEP], 1)[kept] + 2.0 ** -25
+    _close(cache.view(-1, rank + 64), expected, tol)
+    if heads:
+        e, size = rotated(q)
+        assert got.is_contiguous() and bool(got[~known].isnan().all())
+        _close(got[known], e[known], (e.abs() * half + size * 4 * STEP + 2.0 ** -25)[known])
