@@ -623,8 +623,8 @@ int exlr8_affine4_linear(const void* x, int x_dtype, const float* x_scales, int 
  * else (i, i + 32).  A position outside the table writes no entry.  q_rope
  * (nullable) [tokens][heads][64] is rotated the same way into q_out (NaN for a
  * position outside the table).  Strides count elements; 64 channels (rank for
- * latent) are contiguous.  Two tokens of one call with one slot leave either
- * entry. */
+ * latent) are contiguous.  The slots of one call that lie in the cache have to
+ * differ: a row that two tokens write holds some of either. */
 int exlr8_latent_append(const void* latent, int64_t latent_stride, const void* rope_key, int64_t rope_stride,
                         int64_t tokens, int rank, int dtype, const void* weight, float eps, const float* cos_sin,
                         int64_t cos_rows, const int32_t* positions, int interleaved, const int64_t* slots, void* cache,

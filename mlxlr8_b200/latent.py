@@ -72,9 +72,9 @@ def latent_append(latent, rope_key, cache, slots, *, weight=None, eps: float = 1
     ``q_rope [tokens, heads, 64]`` where given, are rotated: channel pairs (2i, 2i
     + 1) when ``interleaved``, else (i, i + 32).  A slot outside the cache (-1
     for padding rows) writes nothing; so does a position outside the table,
-    whose rotated queries are NaN.  Two tokens with one slot leave either
-    entry.  Returns the rotated queries (a new
-    tensor), or None."""
+    whose rotated queries are NaN.  The slots inside the cache have to differ: a
+    row that two tokens write holds some of either.  Returns the rotated
+    queries (a new tensor), or None."""
     device = _lib.require_cuda(latent, rope_key, cache, slots, weight, cos_sin, positions, q_rope)
     pages, page_size, rank = _check_cache(cache)
     dtype = cache.dtype
