@@ -276,6 +276,12 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return r;
 }
 
+// A sum of weighted rows over the sum of its weights: 0 for a query that saw no
+// token, also where 0 times a row that is not finite made the sum NaN.
+__device__ __forceinline__ float share(uint32_t sum, float factor) {
+  return factor == 0.0f ? 0.0f : __uint_as_float(sum) * factor;
+}
+
 template <int kCols>
 __device__ __forceinline__ void load_columns(uint32_t taddr, uint32_t (&v)[kCols]) {
   if constexpr (kCols == 32) tc_ld32(taddr, v);
@@ -664,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!whole) sums[i * 2 * gridDim.x + slot] = make_float2(unit, ok ? sum : NAN);
         else if (a.lse && row < rows)
           a.lse[walk.b * rows + row] = !ok ? NAN : sum == 0.0f ? -INFINITY : (unit + log2f(sum)) * 0.6931471805599453f;
-        sh.factor[i] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        sh.factor[i] = !ok ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
       }
       group_sync(bar);
       if (ok) ok = mbar_wait(&sh.o_done, segment & 1);
@@ -694,8 +700,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < kCols; i += 4, dst += a.rank) {
             const float4 f = *reinterpret_cast<const float4*>(&sh.factor[col0 + i]);
-            const uint32_t two[2] = {pack<kAct>(__uint_as_float(o[i]) * f.x, __uint_as_float(o[i + 1]) * f.y),
-                                     pack<kAct>(__uint_as_float(o[i + 2]) * f.z, __uint_as_float(o[i + 3]) * f.w)};
+            const uint32_t two[2] = {pack<kAct>(share(o[i], f.x), share(o[i + 1], f.y)),
+                                     pack<kAct>(share(o[i + 2], f.z), share(o[i + 3], f.w))};
             uint32_t w[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {  // channels c, c + 1 of row 2 e + lane % 2
@@ -783,7 +789,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 4)
   };
   auto store = [&](int row, int vector, const float4& o, float inv) {
     uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (cut.sequence * rows + row) * a.rank);
-    dst[32 * vector + lane] = make_uint2(pack<kAct>(o.x * inv, o.y * inv), pack<kAct>(o.z * inv, o.w * inv));
+    dst[32 * vector + lane] = inv == 0.0f ? make_uint2(0, 0)  // (see share)
+                                          : make_uint2(pack<kAct>(o.x * inv, o.y * inv), pack<kAct>(o.z * inv, o.w * inv));
   };
   float top, sum;
   if (kn > workers) {

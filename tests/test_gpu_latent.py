@@ -791,3 +791,25 @@ def test_append_of_unaligned_views_matches_the_formula(dtype, tokens, rank, head
         e, size = rotated(q)
         assert got.is_contiguous() and bool(got[~known].isnan().all())
         _close(got[known], e[known], (e.abs() * half + size * 4 * STEP + 2.0 ** -25)[known])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_absorbed_queries_that_see_nothing_beside_a_token_that_is_not_finite(bad):
+    """Zeros, whole and joined from parts, whatever the cache holds."""
+    import torch
+
+    from mlxlr8_b200.latent import latent_attention
+
+    g = torch.Generator(device="cuda").manual_seed(99)
+    for lengths, queries, heads in (([1, 2, 40], 4, 10), ([70], 90, 16), ([1, 300], 5, 40), ([150], 200, 3)):
+        cache, table = _paged(g, lengths, 512, 16, torch.bfloat16)
+        for b in range(len(lengths)):
+            cache[table[b, 0].long(), 0] = bad
+        batch = len(lengths)
+        ql, qr = (torch.randn(batch, queries, heads, n, generator=g, device="cuda").bfloat16() for n in (512, 64))
+        got, lse = latent_attention(ql, qr, cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), 0.05,
+                                    return_lse=True)
+        for b, n in enumerate(lengths):
+            none = max(queries - n, 0)
+            assert bool((got[b, :none] == 0).all()) and bool((lse[b, :none] == -math.inf).all())
+            assert bool(got[b, none:].isnan().all())
