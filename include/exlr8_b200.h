@@ -55,7 +55,8 @@ enum exlr8_status {
   EXLR8_ERR_ID_RANGE = 13,  /* "Expert IDs must be in 0..256"                       experts.py:158-159 */
   EXLR8_ERR_UNSUPPORTED = 14,
   EXLR8_ERR_STATIC_LIMIT = 15, /* needs more scratch than EXLR8_NOALLOC_SCRATCH_BYTES */
-  EXLR8_ERR_SHAPE = 16        /* operand sizes or strides outside what the call takes */
+  EXLR8_ERR_SHAPE = 16,       /* operand sizes or strides outside what the call takes */
+  EXLR8_ERR_OVERLAP = 17      /* an output or the workspace overlaps another operand */
 };
 
 /* Library ABI version (EXLR8_ABI_VERSION). */
@@ -592,7 +593,10 @@ int exlr8_residual_rms_norm_q8(const void* x, const void* residual, const void* 
                                void* stream);
 
 /* ---- attention half of a decoder block ------------------------------------
- * No output of these calls may overlap an input. */
+ * No output of these calls, nor the workspace, may overlap another operand (the
+ * cache of exlr8_latent_append is an output); the bytes from an operand's first
+ * element to its last count, gaps between its rows among them
+ * (EXLR8_ERR_OVERLAP).  The same holds for exlr8_residual_rms_norm_q8. */
 
 /* Linear layer with 4-bit affine weights (the affine4 dense format of
  * exlr8/dense.py:19-67; MLX quantize(bits=4)): codes uint32 [out][in / 8], low

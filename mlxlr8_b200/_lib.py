@@ -21,7 +21,7 @@ E4M3_CODE = 3  # 8-bit activations, where a call takes them
 SCALE_CODES = {torch.float32: 0, torch.float16: 1}
 
 # Status codes whose reference behaviour is a ValueError.
-VALUE_ERRORS = {1, 2, 3, 4, 5, 6, 7, 8, 13, 15, 16}
+VALUE_ERRORS = {1, 2, 3, 4, 5, 6, 7, 8, 13, 15, 16, 17}
 
 
 class TrellisExperts(ctypes.Structure):

@@ -476,6 +476,7 @@ const char* exlr8_status_string(int status) {
     case EXLR8_ERR_STATIC_LIMIT:
       return "request needs more scratch than the fixed no-allocation buffer (EXLR8_NOALLOC_SCRATCH_BYTES)";
     case EXLR8_ERR_SHAPE: return "operand sizes or strides are outside what the operator takes";
+    case EXLR8_ERR_OVERLAP: return "an output or the workspace overlaps another operand";
     default: return "unknown status";
   }
 }

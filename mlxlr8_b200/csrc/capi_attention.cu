@@ -5,6 +5,7 @@
 // pages, lengths) is bounded by the kernels.
 
 #include <cmath>
+#include <initializer_list>
 
 #include "affine4.cuh"
 #include "capi_util.cuh"
@@ -23,6 +24,37 @@ bool pages_ok(int64_t pages, int page_size) {
          pages * page_size <= kMaxGrid;
 }
 
+// The bytes from an operand's first element to its last, gaps between rows
+// among them; empty without a pointer.
+struct Span {
+  __int128 begin = 0, end = 0;
+  Span(const void* p, __int128 bytes) {
+    if (p == nullptr || bytes <= 0) return;
+    begin = reinterpret_cast<uintptr_t>(p);
+    end = begin + bytes;
+  }
+  // Rows of `width` 16-bit channels, [n][m] of them with element strides of
+  // either sign.
+  Span(const void* p, int64_t n, int64_t n_stride, int64_t m, int64_t m_stride, int width) {
+    if (p == nullptr || n <= 0 || m <= 0) return;
+    const __int128 a = static_cast<__int128>(n - 1) * n_stride, b = static_cast<__int128>(m - 1) * m_stride;
+    begin = reinterpret_cast<uintptr_t>(p) + 2 * ((a < 0 ? a : 0) + (b < 0 ? b : 0));
+    end = reinterpret_cast<uintptr_t>(p) + 2 * ((a > 0 ? a : 0) + (b > 0 ? b : 0) + width);
+  }
+  bool meets(const Span& o) const { return begin < o.end && o.begin < end && begin < end && o.begin < o.end; }
+};
+// Whether a written span meets one that is read, or another written one.
+bool overlap(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  for (const Span* w = written.begin(); w != written.end(); ++w) {
+    for (const Span& r : read)
+      if (w->meets(r)) return true;
+    for (const Span* v = w + 1; v != written.end(); ++v)
+      if (w->meets(*v)) return true;
+  }
+  return false;
+}
+int size_of(int dtype) { return dtype == EXLR8_DTYPE_F32 ? 4 : dtype == EXLR8_DTYPE_E4M3 ? 1 : 2; }
+
 }  // namespace
 
 extern "C" {
@@ -35,6 +67,11 @@ int exlr8_residual_rms_norm_q8(const void* x, const void* residual, const void* 
   if (group != hidden && ((group != 32 && group != 64 && group != 128) || hidden % group)) return EXLR8_ERR_SHAPE;
   if (rows == 0) return EXLR8_OK;
   if (!x || !weight || !codes || !scales || !(eps >= 0.0f)) return EXLR8_ERR_ARG;
+  const __int128 n = static_cast<__int128>(rows) * hidden;
+  const int size = size_of(x_dtype);
+  if (overlap({{h_out, n * size}, {codes, n}, {scales, n / group * 4}},
+              {{x, n * size}, {residual, n * size}, {weight, static_cast<__int128>(hidden) * size}}))
+    return EXLR8_ERR_OVERLAP;
   EXLR8_TIMED(EXLR8_KERNEL_NORM, as_stream(stream),
               launch_residual_rms_q8(x, residual, weight, x_dtype, rows, hidden, group, eps, h_out, codes, scales,
                                      as_stream(stream)));
@@ -56,6 +93,14 @@ int exlr8_affine4_linear(const void* x, int x_dtype, const float* x_scales, int 
   if (rows == 0) return EXLR8_OK;
   if (!x || !codes || !scales || !out || q8 != (x_scales != nullptr)) return EXLR8_ERR_ARG;
   if (!aligned16(x) || !aligned16(codes)) return EXLR8_ERR_ALIGN;
+  const __int128 w = static_cast<__int128>(out_features) * in_features, scale_bytes = w / group * size_of(scale_dtype);
+  if (overlap({{out, static_cast<__int128>(rows) * out_features * size_of(out_dtype)}},
+              {{x, static_cast<__int128>(rows) * in_features * size_of(x_dtype)},
+               {x_scales, q8 ? static_cast<__int128>(rows) * (in_features / x_group) * 4 : 0},
+               {codes, w / 2},
+               {scales, scale_bytes},
+               {biases, scale_bytes}}))
+    return EXLR8_ERR_OVERLAP;
   const Affine4Args a{x,     x_dtype, x_scales, q8 ? x_group : in_features, rows, in_features, out_features, codes, scales,
                       biases, scale_dtype, group, out, out_dtype};
   EXLR8_TIMED(EXLR8_KERNEL_LINEAR4, as_stream(stream), launch_affine4_linear(a, as_stream(stream)));
@@ -75,6 +120,16 @@ int exlr8_latent_append(const void* latent, int64_t latent_stride, const void* r
   if (!latent || !rope_key || !slots || (pages > 0 && !cache) || !(eps >= 0.0f) || (cos_sin && !positions) ||
       (q_rope && !q_out))
     return EXLR8_ERR_ARG;
+  if (overlap({{cache, static_cast<__int128>(pages) * page_size * (rank + kLatentRope) * 2},
+               {q_rope ? q_out : nullptr, static_cast<__int128>(tokens) * heads * kLatentRope * 2}},
+              {{latent, tokens, latent_stride, 1, 0, rank},
+               {rope_key, tokens, rope_stride, 1, 0, kLatentRope},
+               {q_rope, tokens, q_token_stride, heads, q_head_stride, kLatentRope},
+               {weight, rank * 2},
+               {cos_sin, static_cast<__int128>(cos_rows) * kLatentRope * 4},
+               {cos_sin ? positions : nullptr, static_cast<__int128>(tokens) * 4},
+               {slots, static_cast<__int128>(tokens) * 8}}))
+    return EXLR8_ERR_OVERLAP;
   const LatentAppendArgs a{latent,  latent_stride, rope_key,    rope_stride, tokens, rank,  dtype,
                            weight,  eps,           cos_sin,     cos_rows,    positions, interleaved != 0, slots,
                            cache,   pages * page_size, q_rope,  q_token_stride, q_head_stride, heads, q_out};
@@ -105,6 +160,14 @@ int exlr8_latent_attention(const void* q_latent, const void* q_rope, int64_t bat
   if (!aligned16(q_latent) || !aligned16(q_rope) || !aligned16(cache) || !aligned16(out)) return EXLR8_ERR_ALIGN;
   if (need > 0 && (!workspace || workspace_bytes < need)) return EXLR8_ERR_WORKSPACE;
   if (need > 0 && !aligned16(workspace)) return EXLR8_ERR_ALIGN;
+  const __int128 rows = static_cast<__int128>(batch) * queries * heads;
+  if (overlap({{out, rows * rank * 2}, {lse, rows * 4}, {workspace, static_cast<__int128>(need)}},
+              {{q_latent, rows * rank * 2},
+               {q_rope, rows * kLatentRope * 2},
+               {cache, static_cast<__int128>(pages) * page_size * (rank + kLatentRope) * 2},
+               {block_table, static_cast<__int128>(batch) * table_width * 4},
+               {lengths, static_cast<__int128>(batch) * 4}}))
+    return EXLR8_ERR_OVERLAP;
   const LatentAttentionArgs a{q_latent,  q_rope,      batch,       queries, heads, rank, dtype, cache, pages,
                               page_size, block_table, table_width, lengths, scale, out,  lse,   workspace};
   EXLR8_TIMED(EXLR8_KERNEL_ATTENTION, as_stream(stream), launch_latent_attention(a, as_stream(stream)));
@@ -134,6 +197,15 @@ int exlr8_latent_prompt_attention(const void* q, int64_t q_token_stride, int64_t
   if (!q || !out || !q_starts || !k_starts || (total_k > 0 && (!k || !k_rope || !v)) || !std::isfinite(scale))
     return EXLR8_ERR_ARG;
   if (!aligned16(q) || !aligned16(k) || !aligned16(k_rope) || !aligned16(v) || !aligned16(out)) return EXLR8_ERR_ALIGN;
+  const __int128 results = static_cast<__int128>(total_q) * heads, starts = 4 * (static_cast<__int128>(seqs) + 1);
+  if (overlap({{out, results * value * 2}, {lse, results * 4}},
+              {{q, total_q, q_token_stride, heads, q_head_stride, nope + kLatentRope},
+               {k, total_k, k_token_stride, heads, k_head_stride, nope},
+               {k_rope, total_k, k_rope_stride, 1, 0, kLatentRope},
+               {v, total_k, v_token_stride, heads, v_head_stride, value},
+               {q_starts, starts},
+               {k_starts, starts}}))
+    return EXLR8_ERR_OVERLAP;
   const LatentPromptArgs a{q,       k,       k_rope, v,     q_token_stride, q_head_stride, k_token_stride,
                            k_head_stride, k_rope_stride, v_token_stride, v_head_stride, total_q, total_k, heads,
                            nope,    value,   dtype,  q_starts, k_starts, seqs, scale, out, lse};

@@ -73,8 +73,8 @@ def latent_append(latent, rope_key, cache, slots, *, weight=None, eps: float = 1
     + 1) when ``interleaved``, else (i, i + 32).  A slot outside the cache (-1
     for padding rows) writes nothing; so does a position outside the table,
     whose rotated queries are NaN.  The slots inside the cache have to differ: a
-    row that two tokens write holds some of either.  Returns the rotated
-    queries (a new tensor), or None."""
+    row that two tokens write holds some of either.  No other operand may lie
+    in the cache.  Returns the rotated queries (a new tensor), or None."""
     device = _lib.require_cuda(latent, rope_key, cache, slots, weight, cos_sin, positions, q_rope)
     pages, page_size, rank = _check_cache(cache)
     dtype = cache.dtype
@@ -126,7 +126,8 @@ def latent_attention(q_latent, q_rope, cache, block_table, lengths, scale: float
     ``return_lse`` also float32 ``[batch, queries, heads]``, the logarithm of the
     softmax's sum (-inf where nothing was seen), by which results over parts
     of a context can be joined.  ``workspace`` (optional uint8 tensor) is used
-    when it is large enough; calls that overlap need one each."""
+    when it is large enough; calls that overlap need one each, and no operand
+    may lie in it."""
     device = _lib.require_cuda(q_latent, q_rope, cache, block_table, lengths, out, workspace)
     pages, page_size, rank = _check_cache(cache)
     batch, queries, heads, width = q_latent.shape if q_latent.dim() == 4 else (0, 0, 0, 0)

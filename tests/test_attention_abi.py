@@ -128,3 +128,84 @@ def test_pages_are_handed_out_and_given_back():
                 lambda: LatentPages(4, 24)):
         with pytest.raises(ValueError):
             bad()
+
+
+# ---- outputs and workspaces over other operands: refused before any launch ---------
+# Operands lie a MB apart from each other; every case puts one over another.
+
+MB = 1 << 20
+
+
+def _apart(names):
+    return {name: (i + 1) * (16 * MB) for i, name in enumerate(names)}
+
+
+@pytest.mark.parametrize("change", [
+    ("h", "x", 0), ("h", "residual", 2 * 512 - 2), ("codes", "x", 3 * 512 * 2 - 8), ("scales", "w", 0), ("codes", "residual", 8),
+    ("scales", "codes", 3 * 512 - 4), ("h", "scales", -3 * 512 * 2 + 4),
+])
+def test_norm_outputs_over_other_operands(change):
+    at = _apart(["x", "residual", "w", "h", "codes", "scales"])
+    at[change[0]] = at[change[1]] + change[2]
+    assert _lib.load().exlr8_residual_rms_norm_q8(at["x"], at["residual"], at["w"], 2, 3, 512, 128, 1e-5, at["h"], at["codes"],
+                                                  at["scales"], None) == 17
+
+
+@pytest.mark.parametrize("other, by", [("x", 0), ("x", 2 * 3 * 512 - 4), ("codes", 40 * 256 - 4), ("scales", -3 * 40 * 2 + 2),
+                                       ("biases", 40 * 8 * 2 - 2)])
+def test_linear_output_over_other_operands(other, by):
+    at = _apart(["x", "codes", "scales", "biases"])
+    assert _lib.load().exlr8_affine4_linear(at["x"], 2, None, 0, 3, 512, 40, at["codes"], at["scales"], at["biases"], 1, 64,
+                                            at[other] + by, 2, None) == 17
+
+
+def test_linear_output_over_the_activations_scales():
+    assert _lib.load().exlr8_affine4_linear(MB, 3, 2 * MB, 128, 3, 512, 40, 3 * MB, 4 * MB, None, 1, 64, 2 * MB + 44, 2, None) == 17
+
+
+@pytest.mark.parametrize("name, by", [
+    ("latent", 0), ("latent", 4 * 16 * 192 * 2 - 2), ("latent", -(4 * 200 + 128) * 2 + 2), ("key", 64), ("weight", 0),
+    ("cos", 4096), ("positions", -16), ("slots", -36), ("q", -(4 * 300 + 64 + 64) * 2 + 2), ("q_out", 8),
+])
+def test_append_cache_over_other_operands(name, by):
+    at = _apart(["cache", "latent", "key", "weight", "cos", "positions", "slots", "q", "q_out"])
+    at[name] = at["cache"] + by
+    assert _lib.load().exlr8_latent_append(at["latent"], 200, at["key"], 200, 5, 128, 2, at["weight"], 1e-5, at["cos"], 40,
+                                           at["positions"], 1, at["slots"], at["cache"], 4, 16, at["q"], 300, 64, 2, at["q_out"],
+                                           None) == 17
+
+
+def test_append_rows_with_negative_strides_over_the_cache():
+    at = _apart(["cache", "latent", "key", "slots"])
+    latent = at["cache"] + 4 * 16 * 192 * 2 + 3 * 200 * 2  # the last of five rows ends over the cache
+    assert _lib.load().exlr8_latent_append(latent, -200, at["key"], 64, 5, 128, 2, None, 1e-5, None, 0, None, 1, at["slots"],
+                                           at["cache"], 4, 16, None, 0, 0, 0, None, None) == 17
+
+
+@pytest.mark.parametrize("name, other, by", [
+    ("out", "ql", 0), ("out", "cache", 4 * 16 * 576 * 2 - 16), ("out", "lengths", 0), ("lse", "out", 3 * 8 * 512 * 2 - 16),
+    ("ws", "ql", 1024), ("ws", "qr", 0), ("ws", "cache", 0), ("ws", "table", -16), ("ws", "out", 0), ("ws", "lse", -16),
+    ("lse", "qr", 0), ("table", "out", 16),
+])
+def test_attention_outputs_and_workspace_over_other_operands(name, other, by):
+    names = ["ql", "qr", "cache", "table", "lengths", "out", "lse", "ws"]
+    at = _apart(names)
+    at[name] = at[other] + by
+    assert _lib.load().exlr8_latent_attention(at["ql"], at["qr"], 3, 1, 8, 512, 2, at["cache"], 4, 16, at["table"], 4, at["lengths"],
+                                              0.1, at["out"], at["lse"], at["ws"], 1 << 40, None) == 17
+
+
+@pytest.mark.parametrize("name, other, by", [
+    ("out", "q", (4 * 768 + 3 * 192 + 192) * 2 - 16), ("out", "k", 16), ("out", "kr", 0), ("out", "v", 0), ("out", "qs", 0),
+    ("out", "ks", 0), ("lse", "out", 0), ("lse", "v", (6 * 512 + 3 * 128 + 128) * 2 - 4),
+])
+def test_prompt_outputs_over_other_operands(name, other, by):
+    at = _apart(["q", "k", "kr", "v", "qs", "ks", "out", "lse"])
+    at[name] = at[other] + by
+    assert _lib.load().exlr8_latent_prompt_attention(at["q"], 768, 192, at["k"], 512, 128, at["kr"], 64, at["v"], 512, 128, 5, 7, 4,
+                                                     128, 128, 1, at["qs"], at["ks"], 1, 0.1, at["out"], at["lse"], None) == 17
+
+
+def test_overlap_status_is_a_value_error():
+    with pytest.raises(ValueError, match="overlaps"):
+        _lib.check(17)

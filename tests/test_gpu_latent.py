@@ -813,3 +813,29 @@ def test_absorbed_queries_that_see_nothing_beside_a_token_that_is_not_finite(bad
             none = max(queries - n, 0)
             assert bool((got[b, :none] == 0).all()) and bool((lse[b, :none] == -math.inf).all())
             assert bool(got[b, none:].isnan().all())
+
+
+def test_caches_and_workspaces_over_other_operands_are_refused():
+    import torch
+
+    from mlxlr8_b200.latent import latent_append, latent_attention
+
+    cache = torch.zeros(4, 16, 576, device="cuda", dtype=torch.bfloat16)
+    rows = cache.view(64, 576)
+    kv = torch.ones(3, 576, device="cuda", dtype=torch.bfloat16)
+    slots = torch.arange(3, device="cuda")
+    for call in (lambda: latent_append(rows[8:11, :512], kv[:, 512:], cache, slots),
+                 lambda: latent_append(kv[:, :512], rows[61:, 512:], cache, slots),
+                 lambda: latent_append(kv[:, :512], kv[:, 512:], cache, slots, weight=rows[0, :512]),
+                 lambda: latent_append(kv[:, :512], kv[:, 512:], cache, slots, q_rope=rows[:3, None, :64])):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+    assert not bool(cache.any())
+    table, lengths = (torch.zeros(n, device="cuda", dtype=torch.int32) for n in ((2, 2), (2,)))
+    ql, qr = (torch.zeros(2, 1, 8, n, device="cuda", dtype=torch.bfloat16) for n in (512, 64))
+    big = torch.zeros(64 << 20, device="cuda", dtype=torch.uint8)
+    half = big[: 4 * 16 * 576 * 2].view(torch.bfloat16).view(4, 16, 576)
+    out = big[: 2 * 8 * 512 * 2].view(torch.bfloat16).view(2, 1, 8, 512)
+    for more in (dict(cache=half), dict(cache=cache, out=out)):
+        with pytest.raises(ValueError, match="overlaps"):
+            latent_attention(ql, qr, more.pop("cache"), table, lengths, 1.0, workspace=big, **more)
