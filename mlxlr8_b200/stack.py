@@ -84,7 +84,9 @@ class MoEStack:
     hidden]."""
 
     def __init__(self, blocks, eps: float = 1e-5):
-        self.blocks = [tuple(block) if len(block) == 3 else (*block, None) for block in blocks]
+        self.blocks = [tuple(block) for block in blocks]
+        if any(len(block) not in (2, 3) for block in self.blocks):
+            raise ValueError("a block is (norm weight, MoE layer) or (norm weight, MoE layer, attention)")
         self.eps = eps
 
     def __len__(self):
@@ -95,7 +97,8 @@ class MoEStack:
         (MoE residual, normalised input, block output) per block.  ``step`` is
         passed to the blocks' attentions."""
         steps = []
-        for w, layer, attention in self.blocks:
+        for w, layer, *attention in self.blocks:
+            attention = attention[0] if attention else None
             if attention is None:
                 xn = residual_rms_norm(h, w, self.eps)
             else:

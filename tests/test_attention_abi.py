@@ -209,3 +209,23 @@ def test_prompt_outputs_over_other_operands(name, other, by):
 def test_overlap_status_is_a_value_error():
     with pytest.raises(ValueError, match="overlaps"):
         _lib.check(17)
+
+
+def test_stack_blocks_stay_as_they_are_given(monkeypatch):
+    """Pairs are pairs, as callers walk and extend them; a third entry is the
+    block's attention."""
+    from mlxlr8_b200 import stack
+
+    def norm(x, weight, eps, residual=0, return_sum=False):
+        return (x + residual, (x + residual) * weight) if return_sum else x * weight
+
+    monkeypatch.setattr(stack, "residual_rms_norm", norm)
+    made = stack.MoEStack((w, lambda xn, h: xn + h) for w in (2, 3))
+    assert [w for w, layer in made.blocks] == [2, 3] and len(made) == 2
+    made.blocks.append((5, lambda xn, h: xn - h))
+    assert made(1) == 3 * 4 * 4
+    made = stack.MoEStack([[2, lambda xn, h: xn + h, lambda h, step: h * step], (3, lambda xn, h: xn + h, None)])
+    assert made(1, step=10) == 11 * 3 * 4
+    for bad in ((1,), (1, 2, 3, 4)):
+        with pytest.raises(ValueError):
+            stack.MoEStack([bad])
