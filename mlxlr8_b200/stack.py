@@ -29,7 +29,9 @@ def residual_rms_norm(x, weight, eps: float = 1e-5, residual=None, return_sum: b
     """``rms_norm(x + residual, weight, eps)`` in x's dtype
     (model.py:383-384; fast_norm.residual_rms_pair).  With ``return_sum`` the
     rounded sum ``h`` is returned as well."""
-    device = _lib.require_cuda(x)
+    if residual is not None and residual.numel() != x.numel():
+        raise ValueError("the residual must have the size of x")
+    device = _lib.require_cuda(x, weight, residual)
     hidden = x.shape[-1]
     if weight.shape != (hidden,):
         raise ValueError("norm weight must have one entry per hidden channel")
@@ -102,7 +104,7 @@ class MoEStack:
             if attention is None:
                 xn = residual_rms_norm(h, w, self.eps)
             else:
-                h, xn = residual_rms_norm(attention(h, step), w, self.eps, residual=h, return_sum=True)
+                h, xn = residual_rms_norm(h, w, self.eps, residual=attention(h, step), return_sum=True)
             out = layer(xn, h)
             if trace:
                 steps.append((h, xn, out))

@@ -229,3 +229,18 @@ def test_stack_blocks_stay_as_they_are_given(monkeypatch):
     for bad in ((1,), (1, 2, 3, 4)):
         with pytest.raises(ValueError):
             stack.MoEStack([bad])
+
+
+def test_residuals_of_another_size_are_refused():
+    """As what an attention returns: the kernel would read past one of the two."""
+    import torch
+
+    from mlxlr8_b200 import stack
+
+    x, w = torch.zeros(4, 128), torch.ones(128)
+    for rows in (3, 5):
+        with pytest.raises(ValueError, match="size of x"):
+            stack.residual_rms_norm(x, w, residual=torch.zeros(rows, 128))
+        made = stack.MoEStack([(w, lambda xn, h: h, lambda h, step: torch.zeros(rows, 128))])
+        with pytest.raises(ValueError, match="size of x"):
+            made(x)

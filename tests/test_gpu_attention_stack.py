@@ -177,3 +177,21 @@ def test_decode_step_in_a_graph():
         assert torch.equal(out, eager(h, step))
     with pytest.raises(ValueError, match="of the step"):
         eager(h[:1], step)
+
+
+def test_hidden_state_keeps_its_type_beside_an_attention_of_another():
+    import torch
+
+    from mlxlr8_b200.stack import MoEStack, residual_rms_norm
+
+    g = torch.Generator(device="cuda").manual_seed(50)
+    h, r = (torch.randn(3, HIDDEN, generator=g, device="cuda") for _ in range(2))
+    h, w = h.bfloat16(), torch.ones(HIDDEN, device="cuda", dtype=torch.bfloat16)
+    out, steps = MoEStack([(w, lambda xn, h: xn + h, lambda h, step: r)])(h, trace=True)
+    total, xn = residual_rms_norm(h, w, residual=r.bfloat16(), return_sum=True)
+    assert out.dtype == torch.bfloat16 and torch.equal(steps[0][0], total) and torch.equal(steps[0][1], xn)
+    for other in (w.cpu(), w[:-1]):
+        with pytest.raises(ValueError):
+            residual_rms_norm(h, other)
+    with pytest.raises(ValueError):
+        residual_rms_norm(h, w, residual=r.cpu())
