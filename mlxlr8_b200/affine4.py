@@ -79,6 +79,8 @@ class Affine4Linear:
 
     def __init__(self, codes, scales, biases=None):
         self.in_features, self.out_features, self.group = _check_weights(codes, scales, biases)
+        if any(t is not None and t.device != codes.device for t in (scales, biases)):
+            raise ValueError("operands are on different devices")
         self.codes, self.scales = _lib.aligned(codes), scales.contiguous()
         self.biases = biases.contiguous() if biases is not None else None
 

@@ -244,3 +244,15 @@ def test_residuals_of_another_size_are_refused():
         made = stack.MoEStack([(w, lambda xn, h: h, lambda h, step: torch.zeros(rows, 128))])
         with pytest.raises(ValueError, match="size of x"):
             made(x)
+
+
+def test_weights_of_a_layer_lie_on_one_device():
+    import torch
+
+    from mlxlr8_b200.affine4 import Affine4Linear
+
+    codes, scales = torch.zeros(8, 32, dtype=torch.int32), torch.ones(8, 4)
+    assert Affine4Linear(codes, scales, scales).group == 64
+    for parts in ((scales.to("meta"), None), (scales, scales.to("meta"))):
+        with pytest.raises(ValueError, match="different devices"):
+            Affine4Linear(codes, *parts)
