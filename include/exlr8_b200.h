@@ -608,7 +608,9 @@ int exlr8_residual_rms_norm_q8(const void* x, const void* residual, const void* 
  * a divisor of in_features).  out [rows][out] in out_dtype.  x and codes
  * 16-byte aligned.  Sums are float32.  Made for decode: up to 16 rows share
  * one pass over the weights, more rows (at most 2^19) make more passes.  An
- * infinite channel of x gives NaN in its row, where w * x might be infinite. */
+ * infinite channel of x leaves infinities or NaN in its row of out, not
+ * always those of w * x.  Rounding is that of float32 sums of |s| (16 + q) |x|
+ * and |b - 16 s| |x|, also where the weights s q + b are near zero. */
 int exlr8_affine4_linear(const void* x, int x_dtype, const float* x_scales, int x_group, int64_t rows,
                          int in_features, int out_features, const uint32_t* codes, const void* scales,
                          const void* biases, int scale_dtype, int group, void* out, int out_dtype, void* stream);

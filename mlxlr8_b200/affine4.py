@@ -39,7 +39,9 @@ def affine4_linear(x, codes, scales, biases=None, *, x_scales=None, out_dtype=No
     """``x @ w.T`` for ``x [..., in]`` -> ``[..., out]``, summed in float32 and
     rounded once to ``out_dtype`` (x's; bfloat16 for E4M3 codes).
 
-    An infinite channel makes its row NaN.  ``x_scales [..., in / g]`` (float32, ``g`` 32, 64, 128 or ``in``) belongs to
+    An infinite channel leaves infinities or NaN in its row.  The sums round
+    like sums of ``scale * (16 + q) * x``, also where weights are near zero.
+    ``x_scales [..., in / g]`` (float32, ``g`` 32, 64, 128 or ``in``) belongs to
     ``x`` of dtype float8_e4m3fn.  ``out`` (optional) receives the result."""
     device = _lib.require_cuda(x, codes, scales, biases, x_scales, out)
     in_features, out_features, group = _check_weights(codes, scales, biases)

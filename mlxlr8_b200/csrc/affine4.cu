@@ -19,10 +19,12 @@
 //   float16:   y = sum_u s_u * (sum_{k in u} q_k x_k) + b_u * (sum_{k in u} x_k)
 //   bfloat16:  y = sum_u 16 s_u * (sum_{k in u} v_k x_k)
 //                  + (b_u - 16 s_u) * (sum_{k in u} x_k)
-// (b = -8 s without biases).  Products are exact and sums float32; v lies in
-// [1, 2), so what cancels is no more than three times the sum of |q - 8| x.  The
-// second sum is a product with ones, which lands it in the accumulator's
-// layout.
+// (b = -8 s without biases).  Products are exact and sums float32.  The two terms
+// cancel: their rounding is that of sums of |s| (16 + q) |x| and |b - 16 s| |x|
+// (float16: of |s| q |x| and |b| |x|), which for weights near zero, codes of 7 to 9
+// without biases, are some 70 times the result's own terms |q - 8| |s| |x|; a
+// 16-bit output does not show it.  The second sum is a product with ones, which
+// lands it in the accumulator's layout.
 //
 // A warp takes 64 rows (32 when x has more than eight) of a stage; lane t of a
 // quad takes word 4 j + t of a row's 16, so that place j is 32 channels: units

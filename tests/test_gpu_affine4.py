@@ -199,6 +199,65 @@ def test_no_rows_and_refusals():
             call()
 
 
+def _bound(xv, q, s, b, inner):
+    """What the sums of a bfloat16 or float32 row may be off by: 16 s v x with v =
+    1 + q / 16, and (b - 16 s) x beside it, in chains of at most in / 8 + 64
+    additions that are off by a whole step each (the float16 and E4M3 sums, of
+    q s x and b x, have smaller terms)."""
+    terms = ((16.0 + q) * s).abs() + (b - 16.0 * s).abs()
+    return (inner / 8 + 64) * 2.0 ** -23 * (xv.abs() @ terms.t())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32", "e4m3"])
+@pytest.mark.parametrize("low, high", [(7, 9), (8, 8), (0, 0), (15, 15)])
+@pytest.mark.parametrize("rows, inner, outer, group", [(1, 4096, 130, 128), (9, 1024, 33, 32), (3, 512, 600, 64)])
+def test_codes_of_a_narrow_range_with_a_float32_output(dtype, low, high, rows, inner, outer, group):
+    """Weights near zero, whose terms cancel, and weights of one value."""
+    import torch
+
+    from mlxlr8_b200.affine4 import affine4_linear
+
+    g = torch.Generator(device="cuda").manual_seed(low * 31 + inner)
+    q = torch.randint(low, high + 1, (outer, inner), generator=g, device="cuda")
+    words = (q.view(outer, -1, 8) << torch.arange(0, 32, 4, device="cuda")).sum(-1)
+    codes = torch.where(words >= 1 << 31, words - (1 << 32), words).int()
+    scales = (torch.randn(outer, inner // group, generator=g, device="cuda") * 0.02).half()
+    x = torch.randn(rows, inner, generator=g, device="cuda") + 1.0
+    xs = None
+    if dtype == "e4m3":
+        x, xs = x.to(torch.float8_e4m3fn), torch.ones(rows, 1, device="cuda")
+    else:
+        x = x.to(torch_dtype(dtype))
+    for biases in (None, (-7.5 * scales.float()).half()):
+        got = affine4_linear(x, codes, scales, biases, x_scales=xs, out_dtype=torch.float32)
+        s = scales.double().repeat_interleave(group, 1)
+        b = -8.0 * s if biases is None else biases.double().repeat_interleave(group, 1)
+        xv = x.float().double()
+        expected = xv @ (q.double() * s + b).t()
+        tol = expected.abs() * 2.0 ** -24 + _bound(xv, q.double(), s, b, inner) + 1e-30
+        assert bool(((got.double() - expected).abs() <= tol).all())
+
+
+def test_infinite_channels_leave_no_finite_output():
+    """An infinite channel: infinities or NaN in its row, the other rows as they were."""
+    import torch
+
+    from mlxlr8_b200.affine4 import affine4_linear
+
+    g = torch.Generator(device="cuda").manual_seed(13)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = torch.randn(3, 1024, generator=g, device="cuda").to(dtype)
+        for biases in (False, True):
+            weights = _weights(g, 300, 1024, 64, torch.float16, biases)
+            clean = affine4_linear(x, *weights)
+            for bad in (float("inf"), float("-inf"), float("nan")):
+                y = x.clone()
+                y[1, 900] = bad
+                got = affine4_linear(y, *weights)
+                assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2])
+                assert not bool(got[1].isfinite().any())
+
+
 @pytest.mark.parametrize("outer", [1, 31, 129, 4100, 5001])
 def test_widths_that_end_inside_a_warp_share_channels(outer):
     """A cluster's last barrier behind rows that only some lanes store."""
