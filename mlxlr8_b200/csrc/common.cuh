@@ -33,6 +33,22 @@ __device__ __forceinline__ float round_to(int dtype, float v) {
   return __bfloat162float(__float2bfloat16_rn(v));
 }
 
+// Two floats rounded to a 16-bit type, `lo` in the low half.
+template <int kAct>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  uint32_t r;
+  if (kAct == kF16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// 2^v, subnormal results flushed: the weights of a softmax.
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // Scale vectors are fp16 in EXLR8 checkpoints (experts.py:97-115); fp32 is
 // accepted as well.
 __device__ __forceinline__ float load_scale(const void* base, int dtype, int64_t i) {

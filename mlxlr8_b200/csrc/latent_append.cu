@@ -45,10 +45,7 @@ template <int kAct>
 __device__ __forceinline__ void store8(void* p, int64_t at, const float (&v)[8]) {
   uint32_t u[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (kAct == kBF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-  }
+  for (int i = 0; i < 4; ++i) u[i] = pack<kAct>(v[2 * i], v[2 * i + 1]);
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 

@@ -247,12 +247,6 @@ struct Maps {
   CUtensorMap q, r, cache;
 };
 
-__device__ __forceinline__ float exp2_fast(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // (by whole warps, like the barrier of a vote below)
 __device__ __forceinline__ void group_sync(int id) {
   __syncwarp();
@@ -266,14 +260,6 @@ __device__ __forceinline__ bool group_any(int id, bool v) {
       : "r"(id), "r"(static_cast<uint32_t>(v))
       : "memory");
   return r != 0;
-}
-
-template <int kAct>
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-  uint32_t r;
-  if (kAct == kF16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
 }
 
 // A sum of weighted rows over the sum of its weights: 0 for a query that saw no

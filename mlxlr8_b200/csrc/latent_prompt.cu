@@ -106,12 +106,6 @@ __device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, int
   else tma_load_3d(dst, map, channel, head, row, bar);
 }
 
-__device__ __forceinline__ float exp2_fast(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-
 // Two float32 in one register pair: sm_100 adds and multiplies both at once.
 __device__ __forceinline__ uint64_t both(float lo, float hi) {
   uint64_t r;
@@ -129,14 +123,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-template <int kAct>
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-  uint32_t r;
-  if (kAct == kF16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 

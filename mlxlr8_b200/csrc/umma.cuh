@@ -69,17 +69,10 @@ __host__ __device__ __forceinline__ uint32_t half_idesc(bool bf16, int n, bool n
          (b_rows ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// 128-byte swizzle with the M or N side contiguous: rows of 64 16-bit values
-// along it, eight rows of the contracted dimension per 1 KB atom; `block`
-// bytes between blocks of 64 along the contiguous side.
-__device__ __forceinline__ uint64_t umma_desc_rows128(uint32_t saddr, uint32_t block) {
-  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(block >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
-         (static_cast<uint64_t>(2) << 61);
-}
-
-// The 64-bit descriptors above, by their low words: the high word of both
-// 128-byte forms is kDescHi, and a step of `bytes` along a tile adds bytes / 16
+// 128-byte swizzled descriptors by their low words: K-major as above, and with
+// the M or N side contiguous (rows of 64 16-bit values along it, eight rows of
+// the contracted dimension per 1 KB atom, `block` bytes between blocks of 64
+// along the contiguous side).  The high word of both is kDescHi, and a step of `bytes` along a tile adds bytes / 16
 // to the low word.  Matrix instructions take their operands from uniform
 // registers, so a loop that issues them runs on a whole warp, with low words
 // made uniform by `uniform` and the instructions under `elect_one`: built from
