@@ -17,7 +17,9 @@
 // and O and the sums multiplied, only when a score has grown past it by 2^8,
 // so a tile needs no maximum over its tokens, only the vote that none has.
 // Weights stay below 2^14 and float16 ones keep full precision down to 2^-20
-// of the largest.  Sums are float32, of the unrounded weights.
+// of the largest.  They are rounded to the operands' type for the second product,
+// which takes no wider ones beside 16-bit values (the output's error grows by 6
+// to 18%); their sums are float32, of the unrounded weights.
 //
 // Work is the flat list of (sequence, row tile, 64 tokens), cut evenly over
 // the CTAs (one per SM) whatever the lengths; a sequence cut in two or more
@@ -38,9 +40,10 @@
 // reach the sum.  Waits are bounded; one that runs out leaves NaN in the rows
 // that it concerns.
 //
-// 64 heads of rank 512, bfloat16: 64 sequences of up to 12000 tokens 139 us (4.8
-// TB/s of cache; HBM bound but for the first and last tiles and the join, 7 us);
-// one of 16000 18.6 us (parts written and joined, 10 us of it).
+// 64 heads of rank 512, bfloat16: 64 sequences of up to 12000 tokens 137 us (4.9
+// TB/s of cache; HBM bound but for the first and last tiles and the join, 7 us) in
+// a burst at 1965 MHz, 158 us at the 1600 MHz that the power cap leaves after a
+// second; one of 16000 18.5 us (parts written and joined, 10 us of it).
 
 #include <cuda.h>
 

@@ -14,11 +14,14 @@
 // m is raised only when a row's maximum has grown by more than 2^8 (then O and
 // l are multiplied once and the tile is weighed again), so a tile is weighed
 // without a pass for its maximum first, and P stays below 2^14 and float16
-// weights keep their full precision down to 2^-20 of the largest.  Tensor memory
-// is full: S_0, S_1, O_0, O_1 of 128 columns each, P_q over S_q.  While the
-// threads of one query tile form its weights the tensor pipe works for the other
-// one, which is why two tiles share a CTA (and why each K and V tile is read
-// from L2 once for 256 queries).
+// weights keep their full precision down to 2^-20 of the largest.  P is rounded to
+// the operands' type for the second product, which takes no wider one beside
+// 16-bit values (the output's error grows by 22 to 30%); l is of the unrounded.
+//
+// Tensor memory is full: S_0, S_1, O_0, O_1 of 128 columns each, P_q over S_q.
+// While the threads of one query tile form its weights the tensor pipe works for
+// the other one, which is why two tiles share a CTA (and why each K and V tile
+// is read from L2 once for 256 queries).
 //
 // The two query tiles leave room for 1.6 tiles of keys and values (at 192 key
 // channels), so K and V tiles share one ring of blocks of 64 channels, in the
@@ -47,9 +50,11 @@
 // weights of the other (82 queries of six sequences over 2000 keys each, 24
 // heads: 40 -> 28 us).
 //
-// 8192 queries of 32 heads (128 + 64 key and 128 value channels): 551 to 600 us
-// with the power that is left, 1247 to 1146 TFLOP/s, the tensor pipe bound; 5 prompts of 1300 tokens, 16 heads: 25 us, the
-// longest one's keys in turn (2900 cycles a tile for 256 queries).
+// 8192 queries of 32 heads (128 + 64 key and 128 value channels): 549 us in a
+// burst at 1965 MHz, 1252 TFLOP/s, and 634 us, 1084 TFLOP/s, at the 1520 MHz that
+// the power cap leaves after a second, the tensor pipe bound; 5 prompts of 1300
+// tokens, 16 heads: 25 us, the longest one's keys in turn (2900 cycles a tile for
+// 256 queries).
 
 #include <cuda.h>
 

@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kVecs == 4 ? 512 : 1024)
 
 // One CTA per row, any hidden size and alignment.  kCached keeps h w of the row
 // in shared memory, so that the inputs are read once; rows beyond kCachedMax
-// channels read them again.  Single loads: 5000 x 7999 bfloat16 84 us, 3.3 TB/s
+// channels read them again.  Single loads: 5000 x 7999 bfloat16 85 us, 3.3 TB/s
 // (106 us with the inputs read three times).
 constexpr int kCachedMax = 24 * 1024;  // two CTAs of 96 KB per SM
 
