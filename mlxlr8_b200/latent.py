@@ -67,7 +67,8 @@ def latent_append(latent, rope_key, cache, slots, *, weight=None, eps: float = 1
     """Write ``latent [tokens, rank]`` and ``rope_key [tokens, 64]`` to the rows
     ``slots`` (int64 [tokens], ``page * page_size + offset``) of ``cache``.
 
-    With ``weight [rank]`` the latent is RMS-normed first.  With ``cos_sin``
+    With ``weight [rank]`` (taken in the cache's type) the latent is RMS-normed
+    first.  With ``cos_sin``
     (float32 [positions, 32, 2]) and ``positions`` (int32 [tokens]) the key, and
     ``q_rope [tokens, heads, 64]`` where given, are rotated: channel pairs (2i, 2i
     + 1) when ``interleaved``, else (i, i + 32).  A slot outside the cache (-1

@@ -56,8 +56,9 @@ def residual_rms_norm_q8(x, weight, eps: float = 1e-5, residual=None, group: int
     Returns ``(codes float8_e4m3fn [..., hidden], scales float32 [..., hidden
     // group])``, with ``return_sum`` the rounded sum ``h`` in front of them.
     The norm of ``h`` stays in float32 until ``code = e4m3(y / scale)``, ``scale
-    = max|y| / 448``.  A group of zeros has scale 0; a group with a value that
-    is not finite has scale NaN and codes 0."""
+    = max|y| / 448``.  A group of zeros, or whose scale lies below the smallest
+    float32, has scale 0; a group with a value that is not finite has scale NaN
+    and codes 0.  The residual and the weight are taken in x's dtype."""
     device = _lib.require_cuda(x, weight, residual)
     shape = x.shape
     if not shape or shape[-1] == 0:
